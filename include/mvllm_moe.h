@@ -516,6 +516,98 @@ MVLLM_API int mvllm_moe_dense_ffn_dev(void *stream, int fmt, int T, int H, int O
                                       float *y, int accumulate, void *workspace,
                                       size_t workspace_bytes);
 
+/* ---- the routed layer's steps on their own, with their gradients.  For a
+ *      caller whose experts are not mvllm_moe_layer_dev's fused FFN (biases,
+ *      adapters, another activation) or who trains what surrounds them: route
+ *      -> permute -> dispatch -> the experts' products -> combine, and back.
+ *      The reference has no backward pass and no such steps: it gathers and
+ *      scatters inside its layer loop (glm53.cpp:1958-1984).
+ *      Row matrices (x, xs, y, out, dx, ...) are device memory of dtype
+ *      MVLLM_DTYPE_*, row r at element r * ld; an input's ld may be 0 (one row
+ *      for all), an output's is at least its width.  tok_pos [T, KK], KK =
+ *      K + n_shared <= 64, rows, rw, nr, xoff are mvllm_moe_permute_dev's.
+ *      Positions outside [0, rows_cap) count as no slot; rows of an output
+ *      that no position names (behind the last segment) are left as they were.
+ *      Sums are f32 in a fixed order (results repeat to the bit) and round
+ *      once.  Inputs and outputs may not overlap.  Stream-ordered, no host
+ *      sync, no allocation, capturable; T = 0 (no rows) does nothing except
+ *      where an output is still to be cleared (drouter). ---- */
+/* xs[tok_pos[t, j]] = x[t]: a copy of the bits (xs of x's dtype). */
+MVLLM_API int mvllm_moe_dispatch_dev(void *stream, const void *x, int dtype, int64_t ldx,
+                                     const int *tok_pos, int T, int KK, int D, void *xs,
+                                     int64_t ldxs, int rows_cap);
+/* Its gradient: dx[t] = sum over j, positions ascending, of
+ * dxs[tok_pos[t, j]]; added to dx when accumulate.  A token without a slot
+ * gets 0. */
+MVLLM_API int mvllm_moe_dispatch_grad_dev(void *stream, const void *dxs, int dxs_dtype,
+                                          int64_t lddxs, int rows_cap, const int *tok_pos, int T,
+                                          int KK, int D, void *dx, int dx_dtype, int64_t lddx,
+                                          int accumulate);
+/* out[t] = sum over j, positions p = tok_pos[t, j] ascending (ascending
+ * expert id, the layer's order), of rw[p] y[p]; added to out when
+ * accumulate.  A token without a slot gets 0. */
+MVLLM_API int mvllm_moe_combine_dev(void *stream, const void *y, int y_dtype, int64_t ldy,
+                                    int rows_cap, const float *rw, const int *tok_pos, int T,
+                                    int KK, int D, void *out, int out_dtype, int64_t ldo,
+                                    int accumulate);
+/* Its gradients: dy[p] = rw[p] dout[t] (dy of y's dtype), and dwt[t, k] =
+ * <dout[t], y[p]> with p the position of expert idx[t, k] for token t: slots
+ * that repeat an id share it, since the forward pass adds their weights; 0
+ * where the token has no row for it (an id outside [0, E), a weight sum of 0
+ * that the permutation left out).  idx [T, K] as given to the permutation; a
+ * shared expert's weight (KK = K + 1) is the constant 1 and has no gradient. */
+MVLLM_API int mvllm_moe_combine_grad_dev(void *stream, const void *dout, int dout_dtype,
+                                         int64_t lddo, const void *y, int y_dtype, int64_t ldy,
+                                         int rows_cap, const float *rw, const int *tok_pos,
+                                         const int *idx, int T, int K, int KK, int D, void *dy,
+                                         int64_t lddy, float *dwt);
+/* The gradient of mvllm_moe_route_ex_dev's weights: from dwt [T, K] to the
+ * token rows, dx[t] = sum_k dz_k router[idx[t, k]], and to the router,
+ * drouter[e] = sum over the tokens routed to e of dz x[t], where dz is the
+ * gradient of the logit through score_fn, the clamp at 0, the division by the
+ * weights' sum and routed_scale.  scores [T, E], idx: its outputs (ids outside
+ * [0, E) carry nothing); the choice of ids and the bias have no gradient.
+ * nr, xoff, rows, tok_pos: the permutation of that idx and its weights.  dx
+ * (dx_dtype) or drouter (f32 [E, H], contiguous) may be NULL; both are added
+ * to when accumulate.  E <= 1024, K <= 32. */
+MVLLM_API size_t mvllm_moe_route_grad_workspace(int T, int H, int E, int K);
+MVLLM_API int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t ldx,
+                                       int T, int H, const float *router, int E, int K,
+                                       const int *idx, const float *scores, const float *dwt,
+                                       int score_fn, float routed_scale, const int *nr,
+                                       const int *xoff, const int *rows, const int *tok_pos,
+                                       int KK, void *dx, int dx_dtype, int64_t lddx,
+                                       float *drouter, int accumulate, void *workspace,
+                                       size_t workspace_bytes);
+/* Few rows times a 4-bit matrix (fmt 4 or 7): y[r] = W x[r] for S rows, y
+ * [S, O], in tolerance mode: f32 sums in another order than
+ * mvllm_matmul_dev's, f32 rows of x to f32 precision.  Weights are read once
+ * for up to 8 rows; any S runs, but hundreds of rows per matrix are
+ * mvllm_moe_layer_dev's tensor-core path's work.  Every alignment and odd I
+ * run; rows of 16-byte multiples run fastest. */
+MVLLM_API int mvllm_matvec_q4_dev(void *stream, int fmt, const void *x, int x_dtype, int64_t ldx,
+                                  const void *w, const void *scales, int S, int I, int O, void *y,
+                                  int y_dtype, int64_t ldy);
+/* Its gradient for the rows, the weights being frozen: dx[r] = W^T dy[r],
+ * dy [S, O], dx [S, I]. */
+MVLLM_API int mvllm_matvec_q4_grad_dev(void *stream, int fmt, const void *dy, int dy_dtype,
+                                       int64_t lddy, const void *w, const void *scales, int S,
+                                       int I, int O, void *dx, int dx_dtype, int64_t lddx);
+/* The same for the expert-sorted rows that mvllm_moe_dispatch_dev writes: row
+ * r of segment e (xoff[e] <= r < xoff[e] + nr[e], segments disjoint, clipped
+ * to rows_cap) times expert e's matrix.  w, scales: DEVICE arrays of nb device
+ * pointers (nb <= 1024); an expert whose pointer is null has rows of zeros.
+ * Rows outside every segment are left as they were. */
+MVLLM_API int mvllm_moe_matvec_q4_dev(void *stream, int fmt, int nb, const void *x, int x_dtype,
+                                      int64_t ldx, int rows_cap, const int *nr, const int *xoff,
+                                      const void *const *w, const void *const *scales, int I,
+                                      int O, void *y, int y_dtype, int64_t ldy);
+MVLLM_API int mvllm_moe_matvec_q4_grad_dev(void *stream, int fmt, int nb, const void *dy,
+                                           int dy_dtype, int64_t lddy, int rows_cap,
+                                           const int *nr, const int *xoff, const void *const *w,
+                                           const void *const *scales, int I, int O, void *dx,
+                                           int dx_dtype, int64_t lddx);
+
 /* Health check of the bounded device waits that every pipeline kernel uses:
  * runs one small kernel that waits on an mbarrier one thread completes and
  * then on one that nothing completes.  *completed = 1 when the first wait

@@ -12,6 +12,7 @@
 #include "dense_ffn.cuh"
 #include "epilogue.cuh"
 #include "expert_tier.hpp"
+#include "host.hpp"
 
 #include <cudaTypedefs.h>
 
@@ -1187,6 +1188,25 @@ template <int KIND, bool PAIR> int mma_rate_t(int n, int iters, int sms, double 
     return MVLLM_OK;
 }
 } // namespace
+
+// What the other translation units use of this one (host.hpp).
+int mvb::host_fail(int code, const char *fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return fail(code, "%s", buf);
+}
+
+int mvb::host_device(int *device, int *sms) {
+    const Context &c = ctx();
+    if (!c.inited)
+        return fail(MVLLM_ERR_NOT_INIT, "mvllm_moe_init has not been called");
+    *device = c.device;
+    *sms = c.sms;
+    return MVLLM_OK;
+}
 
 extern "C" {
 

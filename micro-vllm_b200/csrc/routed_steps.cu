@@ -1,0 +1,265 @@
+// routed_steps.cu -- host entries of the routed layer's separate steps:
+// dispatch, combine and the router, with their gradients.
+#include "host.hpp"
+#include "route_grad.cuh"
+
+#include <algorithm>
+
+using namespace mvb;
+
+namespace {
+
+bool row_dtype(int d) { return d == MVLLM_DTYPE_F32 || d == MVLLM_DTYPE_BF16; }
+size_t dtype_bytes(int d) { return d == MVLLM_DTYPE_F32 ? 4 : 2; }
+
+// Largest power of two (at most 16) that divides the address, the pitch and
+// the row length, all in bytes.
+unsigned row_align(const void *p, int64_t ld, int D, int dtype) {
+    const uint64_t b = dtype_bytes(dtype);
+    const uint64_t v = reinterpret_cast<uintptr_t>(p) | uint64_t(ld) * b | uint64_t(D) * b | 16u;
+    return unsigned(v & (~v + 1));
+}
+
+// Elements per lane: 16 bytes of the widest-loaded type where everything is
+// aligned for it, 4 bytes' worth, or one element.
+int row_vec(unsigned align, size_t bytes) {
+    return align >= 16 ? int(16 / bytes) : align >= 4 ? int(4 / bytes) : 1;
+}
+
+constexpr int64_t kMaxGrid = 0x7fffffff;
+
+} // namespace
+
+extern "C" {
+
+int mvllm_moe_dispatch_dev(void *stream, const void *x, int dtype, int64_t ldx,
+                           const int *tok_pos, int T, int KK, int D, void *xs, int64_t ldxs,
+                           int rows_cap) {
+    if ((T > 0 && (!x || !tok_pos || (!xs && rows_cap > 0))) || T < 0 || KK < 1 ||
+        KK > kMaxSlots || D < 1 || ldx < 0 || ldxs < D || rows_cap < 0 || !row_dtype(dtype))
+        return host_fail(MVLLM_ERR_INVALID, "dispatch_dev: invalid arguments");
+    DeviceScope dev;
+    if (int rc = dev.enter())
+        return rc;
+    if (T == 0 || rows_cap == 0)
+        return MVLLM_OK;
+    const unsigned al = std::min(row_align(x, ldx, D, dtype), row_align(xs, ldxs, D, dtype));
+    const int64_t b = dtype_bytes(dtype), w = al >= 16 ? 16 : al >= 4 ? 4 : 2;
+    const int words = int(D * b / w);
+    const int seg = std::max(32, words), nseg = 1;
+    const int64_t units = int64_t(T) * nseg, grid = (units + 7) / 8;
+    if (grid > kMaxGrid)
+        return host_fail(MVLLM_ERR_INVALID, "dispatch_dev: T too large");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+#define MVB_DISPATCH(W)                                                                        \
+    MVB_TRY(launch_serial(dispatch_rows_kernel<W>, dim3(unsigned(grid)), dim3(256), 0, st,     \
+                          static_cast<const W *>(x), ldx *b / w, tok_pos, units, nseg, seg,    \
+                          KK, words, static_cast<W *>(xs), ldxs *b / w, rows_cap))
+    if (w == 16)
+        MVB_DISPATCH(uint4);
+    else if (w == 4)
+        MVB_DISPATCH(uint32_t);
+    else
+        MVB_DISPATCH(uint16_t);
+#undef MVB_DISPATCH
+    return MVLLM_OK;
+}
+
+} // extern "C"
+
+namespace {
+
+template <typename TY, typename TO>
+int combine_launch(cudaStream_t st, int n, const TY *y, int64_t ldy, int cap, const float *rw,
+                   const int *tok_pos, int T, int KK, int D, TO *out, int64_t ldo,
+                   int accumulate) {
+    const int nseg = 1, seg = D;
+    const int64_t units = int64_t(T) * nseg, grid = (units + 7) / 8;
+    if (grid > kMaxGrid)
+        return host_fail(MVLLM_ERR_INVALID, "combine: T too large");
+#define MVB_COMBINE(N)                                                                         \
+    MVB_TRY(launch_serial(combine_rows_kernel<TY, TO, N>, dim3(unsigned(grid)), dim3(256), 0,  \
+                          st, y, ldy, cap, rw, tok_pos, units, nseg, seg, KK, D, out, ldo,     \
+                          accumulate))
+    if (n == 16 / int(sizeof(TY)))
+        MVB_COMBINE(16 / int(sizeof(TY)));
+    else if (n == 4 / int(sizeof(TY)) && n > 1)
+        MVB_COMBINE(4 / int(sizeof(TY)));
+    else
+        MVB_COMBINE(1);
+#undef MVB_COMBINE
+    return MVLLM_OK;
+}
+
+int combine_any(const char *who, void *stream, const void *y, int y_dtype, int64_t ldy, int cap,
+                const float *rw, const int *tok_pos, int T, int KK, int D, void *out,
+                int out_dtype, int64_t ldo, int accumulate) {
+    if ((T > 0 && ((!y && cap > 0) || !tok_pos || !out)) || T < 0 || KK < 1 || KK > kMaxSlots ||
+        D < 1 || ldy < 0 || ldo < D || cap < 0 || !row_dtype(y_dtype) || !row_dtype(out_dtype))
+        return host_fail(MVLLM_ERR_INVALID, "%s: invalid arguments", who);
+    DeviceScope dev;
+    if (int rc = dev.enter())
+        return rc;
+    if (T == 0)
+        return MVLLM_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // N elements a lane for both matrices: y's vector, unless out's rows are
+    // aligned for less.
+    const int ey = int(dtype_bytes(y_dtype)), eo = int(dtype_bytes(out_dtype));
+    int n = row_vec(row_align(y, ldy, D, y_dtype), ey);
+    const unsigned ao = row_align(out, ldo, D, out_dtype);
+    if (ao < std::min(16u, unsigned(n * eo)))
+        n = std::min(n, row_vec(ao, ey));
+    if (ao < std::min(16u, unsigned(n * eo)))
+        n = 1;
+    const bool fy = y_dtype == MVLLM_DTYPE_F32, fo = out_dtype == MVLLM_DTYPE_F32;
+    using bf = __nv_bfloat16;
+    if (fy && fo)
+        return combine_launch(st, n, static_cast<const float *>(y), ldy, cap, rw, tok_pos, T, KK,
+                              D, static_cast<float *>(out), ldo, accumulate);
+    if (fy)
+        return combine_launch(st, n, static_cast<const float *>(y), ldy, cap, rw, tok_pos, T, KK,
+                              D, static_cast<bf *>(out), ldo, accumulate);
+    if (fo)
+        return combine_launch(st, n, static_cast<const bf *>(y), ldy, cap, rw, tok_pos, T, KK, D,
+                              static_cast<float *>(out), ldo, accumulate);
+    return combine_launch(st, n, static_cast<const bf *>(y), ldy, cap, rw, tok_pos, T, KK, D,
+                          static_cast<bf *>(out), ldo, accumulate);
+}
+
+template <typename TD, typename TY>
+int combine_grad_launch(cudaStream_t st, int n, const TD *dout, int64_t lddo, const TY *y,
+                        int64_t ldy, int cap, const float *rw, const int *tok_pos,
+                        const int *idx, int T, int K, int KK, int D, TY *dy, int64_t lddy,
+                        float *dwt) {
+#define MVB_CGRAD(N)                                                                           \
+    MVB_TRY(launch_serial(combine_grad_kernel<TD, TY, N>, dim3(unsigned(T)), dim3(256), 0, st, \
+                          dout, lddo, y, ldy, cap, rw, tok_pos, idx, K, KK, D, dy, lddy, dwt))
+    if (n == 16 / int(sizeof(TY)))
+        MVB_CGRAD(16 / int(sizeof(TY)));
+    else if (n == 4 / int(sizeof(TY)) && n > 1)
+        MVB_CGRAD(4 / int(sizeof(TY)));
+    else
+        MVB_CGRAD(1);
+#undef MVB_CGRAD
+    return MVLLM_OK;
+}
+
+} // namespace
+
+extern "C" {
+
+int mvllm_moe_dispatch_grad_dev(void *stream, const void *dxs, int dxs_dtype, int64_t lddxs,
+                                int rows_cap, const int *tok_pos, int T, int KK, int D, void *dx,
+                                int dx_dtype, int64_t lddx, int accumulate) {
+    return combine_any("dispatch_grad_dev", stream, dxs, dxs_dtype, lddxs, rows_cap, nullptr,
+                       tok_pos, T, KK, D, dx, dx_dtype, lddx, accumulate);
+}
+
+int mvllm_moe_combine_dev(void *stream, const void *y, int y_dtype, int64_t ldy, int rows_cap,
+                          const float *rw, const int *tok_pos, int T, int KK, int D, void *out,
+                          int out_dtype, int64_t ldo, int accumulate) {
+    if (T > 0 && rows_cap > 0 && !rw)
+        return host_fail(MVLLM_ERR_INVALID, "combine_dev: invalid arguments");
+    return combine_any("combine_dev", stream, y, y_dtype, ldy, rows_cap, rw, tok_pos, T, KK, D,
+                       out, out_dtype, ldo, accumulate);
+}
+
+int mvllm_moe_combine_grad_dev(void *stream, const void *dout, int dout_dtype, int64_t lddo,
+                               const void *y, int y_dtype, int64_t ldy, int rows_cap,
+                               const float *rw, const int *tok_pos, const int *idx, int T, int K,
+                               int KK, int D, void *dy, int64_t lddy, float *dwt) {
+    if ((T > 0 && (!dout || !tok_pos || !idx || !dwt || (rows_cap > 0 && (!y || !rw || !dy)))) ||
+        T < 0 || K < 1 || KK < K ||
+        KK > kMaxSlots || D < 1 || lddo < 0 || ldy < 0 || lddy < D || rows_cap < 0 ||
+        !row_dtype(dout_dtype) || !row_dtype(y_dtype))
+        return host_fail(MVLLM_ERR_INVALID, "combine_grad_dev: invalid arguments");
+    DeviceScope dev;
+    if (int rc = dev.enter())
+        return rc;
+    if (T == 0)
+        return MVLLM_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int ey = int(dtype_bytes(y_dtype)), ed = int(dtype_bytes(dout_dtype));
+    int n = row_vec(std::min(row_align(y, ldy, D, y_dtype), row_align(dy, lddy, D, y_dtype)), ey);
+    const unsigned ad = row_align(dout, lddo, D, dout_dtype);
+    if (ad < std::min(16u, unsigned(n * ed)))
+        n = std::min(n, row_vec(ad, ey));
+    if (ad < std::min(16u, unsigned(n * ed)))
+        n = 1;
+    using bf = __nv_bfloat16;
+    const bool fd = dout_dtype == MVLLM_DTYPE_F32, fy = y_dtype == MVLLM_DTYPE_F32;
+    if (fd && fy)
+        return combine_grad_launch(st, n, static_cast<const float *>(dout), lddo,
+                                   static_cast<const float *>(y), ldy, rows_cap, rw, tok_pos, idx,
+                                   T, K, KK, D, static_cast<float *>(dy), lddy, dwt);
+    if (fd)
+        return combine_grad_launch(st, n, static_cast<const float *>(dout), lddo,
+                                   static_cast<const bf *>(y), ldy, rows_cap, rw, tok_pos, idx, T,
+                                   K, KK, D, static_cast<bf *>(dy), lddy, dwt);
+    if (fy)
+        return combine_grad_launch(st, n, static_cast<const bf *>(dout), lddo,
+                                   static_cast<const float *>(y), ldy, rows_cap, rw, tok_pos, idx,
+                                   T, K, KK, D, static_cast<float *>(dy), lddy, dwt);
+    return combine_grad_launch(st, n, static_cast<const bf *>(dout), lddo,
+                               static_cast<const bf *>(y), ldy, rows_cap, rw, tok_pos, idx, T, K,
+                               KK, D, static_cast<bf *>(dy), lddy, dwt);
+}
+
+size_t mvllm_moe_route_grad_workspace(int T, int H, int E, int K) {
+    if (T < 0 || H < 1 || E < 1 || K < 1)
+        return 0;
+    return (size_t(T) * K + 64) * sizeof(float) + 256;
+}
+
+int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t ldx, int T, int H,
+                             const float *router, int E, int K, const int *idx,
+                             const float *scores, const float *dwt, int score_fn,
+                             float routed_scale, const int *nr, const int *xoff, const int *rows,
+                             const int *tok_pos, int KK, void *dx, int dx_dtype, int64_t lddx,
+                             float *drouter, int accumulate, void *workspace,
+                             size_t workspace_bytes) {
+    if ((T > 0 && (!x || !idx || !scores || !dwt || !rows || !tok_pos || (!dx && !drouter))) ||
+        !router || !nr || !xoff || T < 0 || H < 1 || E < 1 || E > 1024 || K < 1 || K > 32 || KK < K ||
+        KK > kMaxSlots || ldx < 0 || (dx && lddx < H) || !row_dtype(x_dtype) ||
+        (dx && !row_dtype(dx_dtype)) ||
+        (score_fn != MVLLM_SCORE_SIGMOID && score_fn != MVLLM_SCORE_SQRT_SOFTPLUS) ||
+        int64_t(T) * KK > kMaxGrid)
+        return host_fail(MVLLM_ERR_INVALID, "route_grad_dev: invalid arguments");
+    if (!workspace || workspace_bytes < mvllm_moe_route_grad_workspace(T, H, E, K))
+        return host_fail(MVLLM_ERR_WORKSPACE, "route_grad_dev: workspace %zu < %zu",
+                         workspace_bytes, mvllm_moe_route_grad_workspace(T, H, E, K));
+    DeviceScope dev;
+    if (int rc = dev.enter())
+        return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    RouteGradArgs a{};
+    a.idx = idx, a.scores = scores, a.dwt = dwt, a.tok_pos = tok_pos, a.router = router;
+    a.T = T, a.K = K, a.KK = KK, a.E = E, a.H = H, a.cap = T * K;
+    a.score_fn = score_fn, a.accumulate = accumulate, a.scale = routed_scale;
+    a.dzp = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(workspace) + 255) &
+                                      ~uintptr_t(255));
+    using bf = __nv_bfloat16;
+    if (T > 0 && drouter)
+        MVB_TRY(launch_serial(route_dz_kernel, dim3((T + 7) / 8), dim3(256), 0, st, a));
+    if (T > 0 && dx) {
+        if (dx_dtype == MVLLM_DTYPE_F32)
+            MVB_TRY(launch_serial(route_dx_kernel<float>, dim3(T), dim3(256), 0, st, a,
+                                  static_cast<float *>(dx), lddx));
+        else
+            MVB_TRY(launch_serial(route_dx_kernel<bf>, dim3(T), dim3(256), 0, st, a,
+                                  static_cast<bf *>(dx), lddx));
+    }
+    if (drouter) {
+        const dim3 grid(E, (H + 255) / 256);
+        if (x_dtype == MVLLM_DTYPE_F32)
+            MVB_TRY(launch_serial(route_dw_kernel<float>, grid, dim3(256), 0, st, a,
+                                  static_cast<const float *>(x), ldx, nr, xoff, rows, drouter));
+        else
+            MVB_TRY(launch_serial(route_dw_kernel<bf>, grid, dim3(256), 0, st, a,
+                                  static_cast<const bf *>(x), ldx, nr, xoff, rows, drouter));
+    }
+    return MVLLM_OK;
+}
+
+} // extern "C"

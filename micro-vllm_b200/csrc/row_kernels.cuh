@@ -1,0 +1,262 @@
+// row_kernels.cuh -- token rows to the expert-sorted order and back, each
+// with its gradient, as steps of their own (the fused layer does them inside
+// its staging and combine kernels).
+//
+// With p(t, j) = tok_pos[t, j] >= 0 the sorted position of token t's slot j,
+// as the permutation writes it:
+//   dispatch            xs[p] = x[t]
+//   dispatch gradient   dx[t] = sum_j dxs[p]
+//   combine             out[t] = sum_j rw[p] y[p]
+//   combine gradient    dy[p] = rw[p] dout[t],  drw[p] = <dout[t], y[p]>
+// The first and third are each other's adjoint up to the weights, so there
+// are three kernels: one copies a token's row to its positions, one adds up
+// its positions' rows (weights optional), one does both for the combine's
+// gradient.  All are bound by memory: every byte is moved once.
+#pragma once
+
+#include "common.cuh"
+
+namespace mvb {
+
+constexpr int kMaxSlots = 64; // slots of a token: two per lane of a warp
+
+// N elements of a row as f32; the address is a multiple of min(16, N * size).
+template <int N> __device__ __forceinline__ void load_row(const float *p, float (&v)[N]) {
+    if constexpr (N == 1) {
+        v[0] = *p;
+    } else if constexpr (N == 2) {
+        const float2 a = *reinterpret_cast<const float2 *>(p);
+        v[0] = a.x, v[1] = a.y;
+    } else {
+#pragma unroll
+        for (int q = 0; q < N; q += 4) {
+            const float4 a = *reinterpret_cast<const float4 *>(p + q);
+            v[q] = a.x, v[q + 1] = a.y, v[q + 2] = a.z, v[q + 3] = a.w;
+        }
+    }
+}
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+template <int N> __device__ __forceinline__ void load_row(const __nv_bfloat16 *p, float (&v)[N]) {
+    if constexpr (N == 1) {
+        v[0] = __bfloat162float(*p);
+    } else if constexpr (N == 2) {
+        const uint32_t a = *reinterpret_cast<const uint32_t *>(p);
+        v[0] = bf16_lo(a), v[1] = bf16_hi(a);
+    } else if constexpr (N == 4) {
+        const uint2 a = *reinterpret_cast<const uint2 *>(p);
+        v[0] = bf16_lo(a.x), v[1] = bf16_hi(a.x), v[2] = bf16_lo(a.y), v[3] = bf16_hi(a.y);
+    } else {
+        static_assert(N == 8, "row vector");
+        const uint4 a = *reinterpret_cast<const uint4 *>(p);
+        v[0] = bf16_lo(a.x), v[1] = bf16_hi(a.x), v[2] = bf16_lo(a.y), v[3] = bf16_hi(a.y);
+        v[4] = bf16_lo(a.z), v[5] = bf16_hi(a.z), v[6] = bf16_lo(a.w), v[7] = bf16_hi(a.w);
+    }
+}
+
+// The same way out; bf16 rounds once, to nearest even.
+template <int N> __device__ __forceinline__ void store_row(float *p, const float (&v)[N]) {
+    if constexpr (N == 1) {
+        *p = v[0];
+    } else if constexpr (N == 2) {
+        *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
+    } else {
+#pragma unroll
+        for (int q = 0; q < N; q += 4)
+            *reinterpret_cast<float4 *>(p + q) =
+                make_float4(v[q], v[q + 1], v[q + 2], v[q + 3]);
+    }
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <int N> __device__ __forceinline__ void store_row(__nv_bfloat16 *p, const float (&v)[N]) {
+    if constexpr (N == 1) {
+        *p = __float2bfloat16_rn(v[0]);
+    } else if constexpr (N == 2) {
+        *reinterpret_cast<uint32_t *>(p) = pack_bf16(v[0], v[1]);
+    } else if constexpr (N == 4) {
+        *reinterpret_cast<uint2 *>(p) =
+            make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    } else {
+        static_assert(N == 8, "row vector");
+        *reinterpret_cast<uint4 *>(p) =
+            make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]),
+                       pack_bf16(v[6], v[7]));
+    }
+}
+
+// A token's slots, KK <= kMaxSlots, held by one warp: lane l keeps slots l
+// and l + 32.  A slot counts when its position lies in [0, cap).
+struct WarpSlots {
+    int p0, p1; // positions, -1 = none
+    __device__ __forceinline__ void load(const int *__restrict__ tok_pos, size_t t, int KK,
+                                         int cap) {
+        const int lane = threadIdx.x & 31;
+        const int *row = tok_pos + t * KK;
+        p0 = lane < KK ? row[lane] : -1;
+        p1 = lane + 32 < KK ? row[lane + 32] : -1;
+        if (p0 >= cap)
+            p0 = -1;
+        if (p1 >= cap)
+            p1 = -1;
+    }
+    // Sorts the positions ascending over (lane, half) and returns their
+    // number: each value goes to the place its rank names.
+    __device__ __forceinline__ int sort(int KK, int *smem) {
+        int r0 = 0, r1 = 0;
+        for (int u = 0; u < KK; ++u) {
+            const int q = __shfl_sync(0xffffffffu, u < 32 ? p0 : p1, u & 31);
+            r0 += (q >= 0 && q < p0) ? 1 : 0;
+            r1 += (q >= 0 && q < p1) ? 1 : 0;
+        }
+        const int n = __popc(__ballot_sync(0xffffffffu, p0 >= 0)) +
+                      __popc(__ballot_sync(0xffffffffu, p1 >= 0));
+        __syncwarp(); // the readers of the last token are done with smem
+        if (p0 >= 0)
+            smem[r0] = p0;
+        if (p1 >= 0)
+            smem[r1] = p1;
+        __syncwarp();
+        return n;
+    }
+};
+
+// dispatch: a warp takes (token, segment of the row), loads 32 words at a time
+// and stores them at each of the token's positions: a copy of the bits, so W
+// is only the widest word (16, 4 or 2 bytes) that rows, pitches and addresses
+// are multiples of.  ldx, ldxs, seg and D count words.
+template <typename W>
+__global__ void __launch_bounds__(256)
+    dispatch_rows_kernel(const W *__restrict__ x, int64_t ldx, const int *__restrict__ tok_pos,
+                         int64_t units, int nseg, int seg, int KK, int D, W *__restrict__ xs,
+                         int64_t ldxs, int cap) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t unit = blockIdx.x * int64_t(blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (unit >= units)
+        return;
+    const int64_t t = unit / nseg;
+    const int s0 = static_cast<int>(unit - t * nseg) * seg, s1 = min(D, s0 + seg);
+    WarpSlots sl;
+    sl.load(tok_pos, t, KK, cap);
+    const uint32_t m0 = __ballot_sync(0xffffffffu, sl.p0 >= 0);
+    const uint32_t m1 = __ballot_sync(0xffffffffu, sl.p1 >= 0);
+    if (!(m0 | m1))
+        return;
+    for (int col = s0; col < s1; col += 32) {
+        const int c = col + lane;
+        W v{};
+        if (c < s1)
+            v = x[t * ldx + c];
+        for (uint32_t m = m0; m; m &= m - 1) {
+            const int64_t p = __shfl_sync(0xffffffffu, sl.p0, __ffs(m) - 1);
+            if (c < s1)
+                xs[p * ldxs + c] = v;
+        }
+        for (uint32_t m = m1; m; m &= m - 1) {
+            const int64_t p = __shfl_sync(0xffffffffu, sl.p1, __ffs(m) - 1);
+            if (c < s1)
+                xs[p * ldxs + c] = v;
+        }
+    }
+}
+
+// combine and the dispatch gradient: out[t] = (out[t] +) sum of rw[p] y[p]
+// over the token's positions in ascending order (ascending expert id), f32
+// fused multiply-adds, one rounding at the end.  rw == nullptr: weight 1.
+template <typename TY, typename TO, int N>
+__global__ void __launch_bounds__(256)
+    combine_rows_kernel(const TY *__restrict__ y, int64_t ldy, int cap,
+                        const float *__restrict__ rw, const int *__restrict__ tok_pos,
+                        int64_t units, int nseg, int seg, int KK, int D, TO *__restrict__ out,
+                        int64_t ldo, int accumulate) {
+    pdl_wait();
+    __shared__ int spos[8][kMaxSlots];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t unit = blockIdx.x * int64_t(blockDim.x >> 5) + warp;
+    if (unit >= units)
+        return;
+    const int64_t t = unit / nseg;
+    const int s0 = static_cast<int>(unit - t * nseg) * seg, s1 = min(D, s0 + seg);
+    WarpSlots sl;
+    sl.load(tok_pos, t, KK, cap);
+    const int n = sl.sort(KK, spos[warp]);
+    for (int c = s0 + lane * N; c < s1; c += 32 * N) {
+        float acc[N];
+        if (accumulate)
+            load_row<N>(out + t * ldo + c, acc);
+        else
+#pragma unroll
+            for (int q = 0; q < N; ++q)
+                acc[q] = 0.f;
+        for (int j = 0; j < n; ++j) {
+            const int64_t p = spos[warp][j];
+            const float w = rw ? rw[p] : 1.f;
+            float v[N];
+            load_row<N>(y + p * ldy + c, v);
+#pragma unroll
+            for (int q = 0; q < N; ++q)
+                acc[q] = fmaf(w, v[q], acc[q]);
+        }
+        store_row<N>(out + t * ldo + c, acc);
+    }
+}
+
+// The combine's gradient, a CTA per token: dy[p] = rw[p] dout[t] and
+// drw[p] = <dout[t], y[p]> (f32, warps' partial sums added in warp order),
+// then dwt[t, k] = drw of the position that token t has for expert idx[t, k]
+// (a repeated id shares the position of its first slot), 0 where it has none.
+template <typename TD, typename TY, int N>
+__global__ void __launch_bounds__(256)
+    combine_grad_kernel(const TD *__restrict__ dout, int64_t lddo, const TY *__restrict__ y,
+                        int64_t ldy, int cap, const float *__restrict__ rw,
+                        const int *__restrict__ tok_pos, const int *__restrict__ idx, int K,
+                        int KK, int D, TY *__restrict__ dy, int64_t lddy,
+                        float *__restrict__ dwt) {
+    pdl_wait();
+    __shared__ float part[8][kMaxSlots];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int64_t t = blockIdx.x;
+    for (int j = 0; j < KK; ++j) {
+        const int64_t p = tok_pos[t * KK + j];
+        float dot = 0.f;
+        if (p >= 0 && p < cap) {
+            const float w = rw[p];
+            for (int c = threadIdx.x * N; c < D; c += blockDim.x * N) {
+                float g[N], v[N], o[N];
+                load_row<N>(dout + t * lddo + c, g);
+                load_row<N>(y + p * ldy + c, v);
+#pragma unroll
+                for (int q = 0; q < N; ++q) {
+                    dot = fmaf(g[q], v[q], dot);
+                    o[q] = w * g[q];
+                }
+                store_row<N>(dy + p * lddy + c, o);
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if (lane == 0)
+            part[warp][j] = dot;
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < K; k += blockDim.x) {
+        const int e = idx[t * K + k];
+        float d = 0.f;
+        for (int j = 0; j <= k; ++j) {
+            if (idx[t * K + j] == e) { // the id's first slot
+                const int p = tok_pos[t * KK + j];
+                if (p >= 0 && p < cap)
+                    for (int w = 0; w < warps; ++w)
+                        d += part[w][j];
+                break;
+            }
+        }
+        dwt[t * K + k] = d;
+    }
+}
+
+} // namespace mvb

@@ -53,7 +53,10 @@ C_SYMBOLS = (
     "mvllm_moe_set_exact", "mvllm_moe_get_exact", "mvllm_moe_layer_error",
     "mvllm_moe_peer_alloc", "mvllm_moe_peer_open", "mvllm_moe_peer_close", "mvllm_moe_peer_free",
     "mvllm_moe_ep_window_layout", "mvllm_moe_ep_dispatch_peer_dev",
-    "mvllm_moe_layer_partial_peer_dev",
+    "mvllm_moe_layer_partial_peer_dev", "mvllm_moe_dispatch_dev", "mvllm_moe_dispatch_grad_dev",
+    "mvllm_moe_combine_dev", "mvllm_moe_combine_grad_dev", "mvllm_moe_route_grad_workspace",
+    "mvllm_moe_route_grad_dev", "mvllm_matvec_q4_dev", "mvllm_matvec_q4_grad_dev",
+    "mvllm_moe_matvec_q4_dev", "mvllm_moe_matvec_q4_grad_dev",
 )
 PHASES = ("permute", "gather", "plan", "expert_phase1", "expert_phase2", "combine")
 
@@ -74,7 +77,7 @@ def lib():
         if not os.path.exists(LIB_PATH):
             raise ImportError(f"{LIB_PATH} is missing: run micro-vllm_b200/build.py")
         L = C.CDLL(LIB_PATH)
-        vp, i, f, sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+        vp, i, f, sz, ld = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_int64
         sig = {
             "mvllm_moe_init": (i, [i]),
             "mvllm_moe_shutdown": (None, []),
@@ -143,6 +146,20 @@ def lib():
                                                  [i, f, f, vp, sz]),
             "mvllm_moe_dense_ffn_dev": (i, [vp, i, i, i, i] + [vp] * 7 + [i, f, f, vp, i, vp,
                                                                          sz]),
+            "mvllm_moe_dispatch_dev": (i, [vp, vp, i, ld, vp, i, i, i, vp, ld, i]),
+            "mvllm_moe_dispatch_grad_dev": (i, [vp, vp, i, ld, i, vp, i, i, i, vp, i, ld, i]),
+            "mvllm_moe_combine_dev": (i, [vp, vp, i, ld, i, vp, vp, i, i, i, vp, i, ld, i]),
+            "mvllm_moe_combine_grad_dev": (i, [vp, vp, i, ld, vp, i, ld, i, vp, vp, vp, i, i, i, i,
+                                               vp, ld, vp]),
+            "mvllm_moe_route_grad_workspace": (sz, [i] * 4),
+            "mvllm_moe_route_grad_dev": (i, [vp, vp, i, ld, i, i, vp, i, i, vp, vp, vp, i, f, vp,
+                                             vp, vp, vp, i, vp, i, ld, vp, i, vp, sz]),
+            "mvllm_matvec_q4_dev": (i, [vp, i, vp, i, ld, vp, vp, i, i, i, vp, i, ld]),
+            "mvllm_matvec_q4_grad_dev": (i, [vp, i, vp, i, ld, vp, vp, i, i, i, vp, i, ld]),
+            "mvllm_moe_matvec_q4_dev": (i, [vp, i, i, vp, i, ld, i, vp, vp, vp, vp, i, i, vp, i,
+                                            ld]),
+            "mvllm_moe_matvec_q4_grad_dev": (i, [vp, i, i, vp, i, ld, i, vp, vp, vp, vp, i, i, vp,
+                                                 i, ld]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)
@@ -161,12 +178,19 @@ def _check(rc):
         raise MoeError(rc, last_error())
 
 
+_device = None  # the device init() named
+
+
 def init(device: int = 0) -> None:
+    global _device
     _check(lib().mvllm_moe_init(device))
+    _device = device
 
 
 def shutdown() -> None:
+    global _device
     lib().mvllm_moe_shutdown()
+    _device = None
 
 
 def set_prefill_mode(mode) -> None:
@@ -641,3 +665,211 @@ def route_dev(x, router, bias, K, idx, wt, scores, choice, stream=None):
     _check(lib().mvllm_moe_route_dev(_stream(stream), _dp(x), x_dtype, T, H, _dp(router),
                                      _dp(bias), E, K, _dp(idx), _dp(wt), _dp(scores),
                                      _dp(choice)))
+
+
+# ------------------------------------- the routed layer's steps, with gradients --
+def _on(t, name):
+    """A device tensor of the library's device."""
+    if t is None or not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor is needed")
+    if _device is not None and t.device.index != _device:
+        raise ValueError(f"{name}: on {t.device}, the library runs on cuda:{_device}")
+
+
+def _rows(t, name, shape, out=False):
+    """Pointer, dtype code and row pitch of a row matrix: f32 or bf16, its
+    elements side by side within a row; an output's rows may not overlap."""
+    _on(t, name)
+    code = _ROW_DTYPES.get(str(t.dtype))
+    if code is None:
+        raise ValueError(f"{name}: {t.dtype}, torch.float32 or torch.bfloat16 is needed")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, {shape} is needed")
+    rows, cols = shape
+    pitch = t.stride(0)
+    if cols > 1 and t.stride(1) != 1 and rows:
+        raise ValueError(f"{name}: the elements of a row must be contiguous")
+    if rows <= 1:
+        pitch = cols
+    if out and pitch < cols:
+        raise ValueError(f"{name}: its rows overlap")
+    return C.c_void_p(t.data_ptr()), code, pitch
+
+
+_ROW_DTYPES = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16}
+
+
+def _flat(t, name, dtype, count):
+    """Pointer of a contiguous device tensor of `count` elements or more."""
+    _on(t, name)
+    if str(t.dtype) != dtype or not t.is_contiguous() or t.numel() < count:
+        raise ValueError(f"{name}: a contiguous {dtype} tensor of at least {count} is needed, "
+                         f"got {t.dtype} {tuple(t.shape)}")
+    return C.c_void_p(t.data_ptr())
+
+
+def _slots(tok_pos):
+    if tok_pos.dim() != 2:
+        raise ValueError(f"tok_pos: shape {tuple(tok_pos.shape)}, [T, K + n_shared] is needed")
+    T, KK = tok_pos.shape
+    return T, KK, _flat(tok_pos, "tok_pos", "torch.int32", T * KK)
+
+
+def _matrix(t, name):
+    if t is None or t.dim() != 2:
+        raise ValueError(f"{name}: a 2-D tensor is needed")
+    return tuple(t.shape)
+
+
+def _stream_at(stream, t):
+    """The given stream, or the current one of the tensor's device."""
+    if stream is None:
+        import torch
+        stream = torch.cuda.current_stream(t.device)
+    return C.c_void_p(stream.cuda_stream)
+
+
+def dispatch_dev(x, tok_pos, xs, stream=None):
+    """xs[tok_pos[t, j]] = x[t] for token rows x [T, D] (f32 or bf16) and the
+    slot positions permute_dev wrote; the other rows of xs [cap, D] are left
+    as they were."""
+    T, KK, pos = _slots(tok_pos)
+    cap, D = _matrix(xs, "xs")
+    px, tx, ldx = _rows(x, "x", (T, D))
+    po, to, ldo = _rows(xs, "xs", (cap, D), out=True)
+    if tx != to:
+        raise ValueError("xs: the dtype of x is needed")
+    _check(lib().mvllm_moe_dispatch_dev(_stream_at(stream, x), px, tx, ldx, pos, T, KK, D, po, ldo,
+                                        cap))
+
+
+def dispatch_grad_dev(dxs, tok_pos, dx, accumulate=False, stream=None):
+    """dx[t] (+)= sum_j dxs[tok_pos[t, j]], the gradient of dispatch_dev."""
+    T, KK, pos = _slots(tok_pos)
+    cap, D = _matrix(dxs, "dxs")
+    pi, ti, ldi = _rows(dxs, "dxs", (cap, D))
+    po, to, ldo = _rows(dx, "dx", (T, D), out=True)
+    _check(lib().mvllm_moe_dispatch_grad_dev(_stream_at(stream, dx), pi, ti, ldi, cap, pos, T, KK,
+                                             D, po, to, ldo, int(bool(accumulate))))
+
+
+def combine_dev(y, rw, tok_pos, out, accumulate=False, stream=None):
+    """out[t] (+)= sum_j rw[p] y[p], p = tok_pos[t, j] ascending: expert rows
+    y [cap, D] back to token rows out [T, D] with the weights rw permute_dev
+    wrote."""
+    T, KK, pos = _slots(tok_pos)
+    cap, D = _matrix(y, "y")
+    pi, ti, ldi = _rows(y, "y", (cap, D))
+    po, to, ldo = _rows(out, "out", (T, D), out=True)
+    _check(lib().mvllm_moe_combine_dev(
+        _stream_at(stream, out), pi, ti, ldi, cap, _flat(rw, "rw", "torch.float32",
+                                                         min(cap, T * KK)),
+        pos, T, KK, D, po, to, ldo, int(bool(accumulate))))
+
+
+def combine_grad_dev(dout, y, rw, tok_pos, idx, dy, dwt, stream=None):
+    """The gradients of combine_dev: dy[p] = rw[p] dout[t] (rows no position
+    names are left as they were) and dwt[t, k] = <dout[t], y[p]> for the
+    position p of expert idx[t, k] (0 where the token has none)."""
+    T, KK, pos = _slots(tok_pos)
+    K = _matrix(idx, "idx")[1]
+    cap, D = _matrix(y, "y")
+    pd, td, ldd = _rows(dout, "dout", (T, D))
+    pi, ti, ldi = _rows(y, "y", (cap, D))
+    po, to, ldo = _rows(dy, "dy", (cap, D), out=True)
+    if to != ti:
+        raise ValueError("dy: the dtype of y is needed")
+    _check(lib().mvllm_moe_combine_grad_dev(
+        _stream_at(stream, dout), pd, td, ldd, pi, ti, ldi, cap,
+        _flat(rw, "rw", "torch.float32", min(cap, T * KK)), pos,
+        _flat(idx, "idx", "torch.int32", T * K), T, K, KK, D, po, ldo,
+        _flat(dwt, "dwt", "torch.float32", T * K)))
+
+
+def route_grad_workspace_bytes(T, H, E, K) -> int:
+    return lib().mvllm_moe_route_grad_workspace(T, H, E, K)
+
+
+def route_grad_dev(x, router, idx, scores, dwt, nr, xoff, rows, tok_pos, dx, drouter,
+                   workspace=None, score_fn=SCORE_SIGMOID, routed_scale=1.0, accumulate=False,
+                   stream=None):
+    """The gradients of route_ex_dev's weights: dx [T, H] of the token rows and
+    drouter [E, H] of the router (either may be None), from dwt [T, K].
+    idx, scores: route_ex_dev's; nr, xoff, rows, tok_pos: permute_dev's for
+    them; score_fn and routed_scale as given to route_ex_dev."""
+    import torch
+    T, KK, pos = _slots(tok_pos)
+    E, H = _matrix(router, "router")
+    K = _matrix(idx, "idx")[1]
+    px, tx, ldx = _rows(x, "x", (T, H))
+    pd, td, ldd = (None, DTYPE_F32, 0) if dx is None else _rows(dx, "dx", (T, H), out=True)
+    if workspace is None:
+        workspace = torch.empty(route_grad_workspace_bytes(T, H, E, K), dtype=torch.uint8,
+                                device=x.device)
+    f32, i32 = "torch.float32", "torch.int32"
+    _check(lib().mvllm_moe_route_grad_dev(
+        _stream_at(stream, x), px, tx, ldx, T, H, _flat(router, "router", f32, E * H), E, K,
+        _flat(idx, "idx", i32, T * K), _flat(scores, "scores", f32, T * E),
+        _flat(dwt, "dwt", f32, T * K), score_fn, routed_scale, _flat(nr, "nr", i32, E),
+        _flat(xoff, "xoff", i32, E), _flat(rows, "rows", i32, T * K), pos, KK, pd, td, ldd,
+        None if drouter is None else _flat(drouter, "drouter", f32, E * H),
+        int(bool(accumulate)), _dp(workspace), workspace.numel() * workspace.element_size()))
+
+
+def _q4(fmt, w, scales, I, O):
+    """Pointers of one packed matrix [O, I]."""
+    if fmt not in (FMT_INT4_G64, FMT_MXFP4):
+        raise ValueError(f"fmt {fmt}: FMT_INT4_G64 or FMT_MXFP4 is needed")
+    kind, groups = (("torch.float32", (I + 63) // 64) if fmt == FMT_INT4_G64
+                    else ("torch.uint8", (I + 31) // 32))
+    return (_flat(w, "w", "torch.uint8", O * ((I + 1) // 2)),
+            _flat(scales, "scales", kind, O * groups))
+
+
+def _matvec(entry, fmt, x, w, scales, y, I, O, stream):
+    pw, ps = _q4(fmt, w, scales, I, O)
+    S = x.shape[0]
+    px, tx, ldx = _rows(x, "the input rows", tuple(x.shape))
+    py, ty, ldy = _rows(y, "the output rows", (S, y.shape[1]), out=True)
+    _check(entry(_stream_at(stream, x), fmt, px, tx, ldx, pw, ps, S, I, O, py, ty, ldy))
+
+
+def matvec_q4_dev(fmt, x, w, scales, y, stream=None):
+    """y [S, O] = x [S, I] . W^T for few rows and packed 4-bit W [O, I]
+    (FMT_INT4_G64 or FMT_MXFP4) in tolerance mode; rows f32 or bf16."""
+    _matvec(lib().mvllm_matvec_q4_dev, fmt, x, w, scales, y, _matrix(x, "x")[1],
+            _matrix(y, "y")[1], stream)
+
+
+def matvec_q4_grad_dev(fmt, dy, w, scales, dx, stream=None):
+    """dx [S, I] = dy [S, O] . W, the gradient of matvec_q4_dev's rows."""
+    _matvec(lib().mvllm_matvec_q4_grad_dev, fmt, dy, w, scales, dx, _matrix(dx, "dx")[1],
+            _matrix(dy, "dy")[1], stream)
+
+
+def _expert_matvec(entry, fmt, x, w, scales, nr, xoff, y, I, O, stream):
+    if fmt not in (FMT_INT4_G64, FMT_MXFP4):
+        raise ValueError(f"fmt {fmt}: FMT_INT4_G64 or FMT_MXFP4 is needed")
+    nb, cap = nr.numel(), x.shape[0]
+    px, tx, ldx = _rows(x, "the input rows", tuple(x.shape))
+    py, ty, ldy = _rows(y, "the output rows", (cap, y.shape[1]), out=True)
+    _check(entry(_stream_at(stream, x), fmt, nb, px, tx, ldx, cap,
+                 _flat(nr, "nr", "torch.int32", nb), _flat(xoff, "xoff", "torch.int32", nb),
+                 _flat(w, "w", "torch.int64", nb), _flat(scales, "scales", "torch.int64", nb),
+                 I, O, py, ty, ldy))
+
+
+def expert_matvec_q4_dev(fmt, x, w, scales, nr, xoff, y, stream=None):
+    """matvec_q4_dev for expert-sorted rows: row r of segment e (xoff[e],
+    nr[e]) of x [cap, I] times expert e's matrix into y [cap, O]; w, scales:
+    int64 CUDA tensors of the experts' addresses.  Rows outside every segment
+    are left as they were."""
+    _expert_matvec(lib().mvllm_moe_matvec_q4_dev, fmt, x, w, scales, nr, xoff, y,
+                   _matrix(x, "x")[1], _matrix(y, "y")[1], stream)
+
+
+def expert_matvec_q4_grad_dev(fmt, dy, w, scales, nr, xoff, dx, stream=None):
+    """dx [cap, I] = dy [cap, O] through each row's expert, the gradient of
+    expert_matvec_q4_dev's rows."""
+    _expert_matvec(lib().mvllm_moe_matvec_q4_grad_dev, fmt, dy, w, scales, nr, xoff, dx,
+                   _matrix(dx, "dx")[1], _matrix(dy, "dy")[1], stream)
