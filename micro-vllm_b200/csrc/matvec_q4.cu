@@ -2,26 +2,171 @@
 #include "host.hpp"
 #include "matvec_q4.cuh"
 
+#include <algorithm>
+#include <cmath>
+#include <map>
+#include <mutex>
+#include <tuple>
+
 using namespace mvb;
 
 namespace {
 
 using bf = __nv_bfloat16;
 
-template <typename TX, typename TY>
-int matvec_launch(cudaStream_t st, bool grad, int nb, const MatvecArgs &a, const TX *x,
-                  int64_t ldx, TY *y, int64_t ldy) {
-    if (grad)
-        MVB_TRY(launch_serial(matvec_grad_simple_kernel<TX, TY>, dim3((a.I + 255) / 256, nb),
-                              dim3(256), 0, st, a, x, ldx, y, ldy));
-    else
-        MVB_TRY(launch_serial(matvec_simple_kernel<TX, TY>, dim3((a.O + 7) / 8, nb), dim3(256), 0,
-                              st, a, x, ldx, y, ldy));
+// Clusters of `ranks` CTAs that fit the device at once (one CTA per SM),
+// asked once per kernel and shared-memory size.
+int max_clusters(const void *kern, int ranks, int smem, int sms, int *out) {
+    if (ranks == 1) {
+        *out = sms;
+        return MVLLM_OK;
+    }
+    static std::mutex mu;
+    static std::map<std::tuple<const void *, int, int>, int> seen;
+    std::lock_guard<std::mutex> lk(mu);
+    auto key = std::make_tuple(kern, ranks, smem);
+    auto it = seen.find(key);
+    if (it == seen.end()) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(ranks);
+        cfg.blockDim = dim3(kMvThreads);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = ranks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        int n = 0;
+        MVB_TRY(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+        it = seen.emplace(key, std::max(n, 1)).first;
+    }
+    *out = it->second;
     return MVLLM_OK;
 }
 
-int matvec_any(const char *who, void *stream, bool grad, int nb, const MatvecArgs &a,
-               const void *x, int x_dtype, int64_t ldx, void *y, int y_dtype, int64_t ldy) {
+template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
+    using F = MvFormat<FMT>;
+    static constexpr int T = MvTerms<FMT, TX, GRAD>::T, RP = 8 * NT / T;
+    static constexpr int TILE = GRAD ? kMvCols : kMvRows, STEP = GRAD ? kMvRows : kMvCols;
+    static constexpr int RING = kMvWarps * mv_ring<NT>() * F::STAGE;
+    static constexpr int RED = kMvWarps * mv_red_size<FMT, TX, NT, GRAD>() * 4;
+    static constexpr int XROWS = GRAD && FMT == MVLLM_FMT_INT4_G64 ? RP : 8 * NT;
+
+    // Shared memory for `chunk` staged stages; fills the plan's offsets.
+    static int layout(MatvecPlan &p, int chunk, int nb) {
+        const int cols = chunk * STEP;
+        int at = mv_alias<NT, GRAD>() ? std::max(RING, RED) : RING;
+        p.off_red = 0;
+        if (!mv_alias<NT, GRAD>())
+            p.off_red = at, at += RED;
+        at = (at + 127) & ~127;
+        p.off_x = at, at += XROWS * mv_x_pitch<FMT, TX, GRAD>(cols);
+        p.off_ex = at, at += GRAD ? 0 : cols / F::G * RP * 4;
+        p.off_list = at, at += (nb + 1) * 4;
+        p.chunk = chunk;
+        return at;
+    }
+
+    // How the work is cut.  The candidates are clusters of 1, 2, 4 or 8 CTAs
+    // along the reduction and 1 to 16 warps along the outputs; the rule
+    // estimates each one's time from the bytes a CTA streams (the device's
+    // rate shared by the CTAs in flight, at most 70 B/ns for one), the stages
+    // a warp takes one after another, the rows it stages and a fixed cost per
+    // unit, times the rounds that the units need.
+    static int plan(const void *kern, MatvecPlan &p, int items, int nb, int sms, int *ranks,
+                    int *grid) {
+        const int tiles = (p.N + TILE - 1) / TILE, steps = (p.K + STEP - 1) / STEP;
+        double best = 1e30;
+        MatvecPlan q = p;
+        for (int c = 1; c <= 8; c *= 2) {
+            const int slice = (steps + c - 1) / c;
+            if (c > 1 && slice * (c - 1) >= steps)
+                break;
+            int chunk = slice;
+            while (chunk > 1 && layout(q, chunk, nb) > kMvSmem)
+                chunk = chunk > 8 ? chunk * 7 / 8 : chunk - 1;
+            int nc = 0;
+            if (int rc = max_clusters(kern, c, layout(q, chunk, nb), sms, &nc))
+                return rc;
+            for (int wo = 1; wo <= kMvWarps; ++wo) {
+                const int wk = std::min(kMvWarps / wo, slice);
+                const int nr = (tiles + wo - 1) / wo;
+                const double units = double(items) * nr, busy = std::min<double>(units, nc);
+                const double rounds = std::ceil(units / nc);
+                const double bytes = double(std::min(wo, tiles)) * slice * F::STAGE;
+                const double rate = std::min(70.0, 6000.0 / (busy * c));
+                const double serial = 250.0 * ((slice + wk - 1) / wk);
+                const double rows = double(RP) * slice * STEP * sizeof(TX) / 60.0;
+                const double t = rounds * (std::max(bytes / rate, serial) + rows + 1500.0 +
+                                           (c > 1 ? 300.0 : 0.0));
+                if (t < best) {
+                    best = t;
+                    p.range = wo * TILE, p.nranges = nr, p.wo = wo, p.wk = wk, p.slice = slice;
+                    p.chunk = chunk;
+                    *ranks = c;
+                    *grid = int(std::min<double>(units, nc)) * c;
+                }
+            }
+        }
+        return MVLLM_OK;
+    }
+
+    static int launch(cudaStream_t st, MatvecArgs a, MatvecPlan p, int items, int sms,
+                      const void *x, int64_t ldx, void *y, int64_t ldy) {
+        auto kern = matvec_q4_kernel<FMT, TX, NT, GRAD>;
+        int ranks = 1, grid = 1;
+        MVB_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMvSmem));
+        if (int rc = plan(reinterpret_cast<const void *>(kern), p, items, a.nb, sms, &ranks, &grid))
+            return rc;
+        const int smem = layout(p, p.chunk, a.nb);
+        if (smem > kMvSmem)
+            return host_fail(MVLLM_ERR_UNSUPPORTED, "matvec_q4: %d bytes of shared memory", smem);
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(grid);
+        cfg.blockDim = dim3(kMvThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute at[2];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        at[1].id = cudaLaunchAttributeClusterDimension;
+        at[1].val.clusterDim.x = ranks, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 2;
+        MVB_TRY(cudaLaunchKernelEx(&cfg, kern, a, p, static_cast<const TX *>(x), ldx, y, ldy));
+        return MVLLM_OK;
+    }
+};
+
+// Rows of a matrix that a launch takes at a time: enough operand columns for
+// the average expert (all rows of a single matrix), at most 32 (gradient: 16).
+template <int FMT, typename TX, bool GRAD>
+int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, int sms, const void *x,
+                int64_t ldx, void *y, int64_t ldy) {
+    constexpr int T = MvTerms<FMT, TX, GRAD>::T;
+    const int avg = (a.rows + a.nb - 1) / a.nb;
+    auto items = [&](int rp) {
+        return a.nb == 1 ? (a.rows + rp - 1) / rp
+                         : std::min(a.rows, a.nb * ((avg + rp - 1) / rp));
+    };
+    const int want = a.nb == 1 ? avg : avg + avg / 2;
+    if (want <= 8 / T)
+        return MvHost<FMT, TX, 1, GRAD>::launch(st, a, p, items(8 / T), sms, x, ldx, y, ldy);
+    if (GRAD || want <= 16 / T)
+        return MvHost<FMT, TX, 2, GRAD>::launch(st, a, p, items(16 / T), sms, x, ldx, y, ldy);
+    if constexpr (!GRAD)
+        return MvHost<FMT, TX, 4, false>::launch(st, a, p, items(32 / T), sms, x, ldx, y, ldy);
+    return MVLLM_OK;
+}
+
+template <int FMT, typename TX>
+int matvec_way(cudaStream_t st, bool grad, const MatvecArgs &a, const MatvecPlan &p, int sms,
+               const void *x, int64_t ldx, void *y, int64_t ldy) {
+    return grad ? matvec_rows<FMT, TX, true>(st, a, p, sms, x, ldx, y, ldy)
+                : matvec_rows<FMT, TX, false>(st, a, p, sms, x, ldx, y, ldy);
+}
+
+int matvec_any(const char *who, void *stream, bool grad, const MatvecArgs &a, const void *x, int x_dtype, int64_t ldx, void *y, int y_dtype, int64_t ldy) {
     const int out = grad ? a.I : a.O;
     if ((a.fmt != MVLLM_FMT_INT4_G64 && a.fmt != MVLLM_FMT_MXFP4) ||
         (a.rows > 0 && (!x || !y)) || a.I < 1 ||
@@ -35,18 +180,16 @@ int matvec_any(const char *who, void *stream, bool grad, int nb, const MatvecArg
     if (a.rows == 0)
         return MVLLM_OK;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool fx = x_dtype == MVLLM_DTYPE_F32, fy = y_dtype == MVLLM_DTYPE_F32;
-    if (fx && fy)
-        return matvec_launch(st, grad, nb, a, static_cast<const float *>(x), ldx,
-                             static_cast<float *>(y), ldy);
-    if (fx)
-        return matvec_launch(st, grad, nb, a, static_cast<const float *>(x), ldx,
-                             static_cast<bf *>(y), ldy);
-    if (fy)
-        return matvec_launch(st, grad, nb, a, static_cast<const bf *>(x), ldx,
-                             static_cast<float *>(y), ldy);
-    return matvec_launch(st, grad, nb, a, static_cast<const bf *>(x), ldx, static_cast<bf *>(y),
-                         ldy);
+    MatvecPlan p{};
+    p.N = out, p.K = grad ? a.O : a.I;
+    p.y_f32 = y_dtype == MVLLM_DTYPE_F32;
+    const bool fx = x_dtype == MVLLM_DTYPE_F32, i4 = a.fmt == MVLLM_FMT_INT4_G64;
+    p.x_vec = ((reinterpret_cast<uintptr_t>(x) | uint64_t(ldx) * (fx ? 4 : 2)) & 15u) == 0;
+    if (i4)
+        return fx ? matvec_way<MVLLM_FMT_INT4_G64, float>(st, grad, a, p, dev.sms, x, ldx, y, ldy)
+                  : matvec_way<MVLLM_FMT_INT4_G64, bf>(st, grad, a, p, dev.sms, x, ldx, y, ldy);
+    return fx ? matvec_way<MVLLM_FMT_MXFP4, float>(st, grad, a, p, dev.sms, x, ldx, y, ldy)
+              : matvec_way<MVLLM_FMT_MXFP4, bf>(st, grad, a, p, dev.sms, x, ldx, y, ldy);
 }
 
 int matvec_one(const char *who, void *stream, bool grad, int fmt, const void *x, int x_dtype,
@@ -55,8 +198,8 @@ int matvec_one(const char *who, void *stream, bool grad, int fmt, const void *x,
     if (!w || !s || (fmt == MVLLM_FMT_INT4_G64 && (reinterpret_cast<uintptr_t>(s) & 3u)))
         return host_fail(MVLLM_ERR_INVALID, "%s: invalid arguments", who);
     MatvecArgs a{};
-    a.fmt = fmt, a.I = I, a.O = O, a.w = w, a.s = s, a.rows = S;
-    return matvec_any(who, stream, grad, 1, a, x, x_dtype, ldx, y, y_dtype, ldy);
+    a.fmt = fmt, a.I = I, a.O = O, a.w = w, a.s = s, a.rows = S, a.nb = 1;
+    return matvec_any(who, stream, grad, a, x, x_dtype, ldx, y, y_dtype, ldy);
 }
 
 int matvec_experts(const char *who, void *stream, bool grad, int fmt, int nb, const void *x,
@@ -67,8 +210,8 @@ int matvec_experts(const char *who, void *stream, bool grad, int fmt, int nb, co
         return host_fail(MVLLM_ERR_INVALID, "%s: invalid arguments", who);
     MatvecArgs a{};
     a.fmt = fmt, a.I = I, a.O = O, a.wt = wt, a.st = st, a.nr = nr, a.xoff = xoff;
-    a.rows = rows_cap;
-    return matvec_any(who, stream, grad, nb, a, x, x_dtype, ldx, y, y_dtype, ldy);
+    a.rows = rows_cap, a.nb = nb;
+    return matvec_any(who, stream, grad, a, x, x_dtype, ldx, y, y_dtype, ldy);
 }
 
 } // namespace
