@@ -16,11 +16,7 @@ using bf = __nv_bfloat16;
 
 // Clusters of `ranks` CTAs that fit the device at once (one CTA per SM),
 // asked once per kernel and shared-memory size.
-int max_clusters(const void *kern, int ranks, int smem, int sms, int *out) {
-    if (ranks == 1) {
-        *out = sms;
-        return MVLLM_OK;
-    }
+int max_clusters(const void *kern, int threads, int ranks, int smem, int *out) {
     static std::mutex mu;
     static std::map<std::tuple<const void *, int, int>, int> seen;
     std::lock_guard<std::mutex> lk(mu);
@@ -29,7 +25,7 @@ int max_clusters(const void *kern, int ranks, int smem, int sms, int *out) {
     if (it == seen.end()) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(ranks);
-        cfg.blockDim = dim3(kMvThreads);
+        cfg.blockDim = dim3(threads);
         cfg.dynamicSmemBytes = smem;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeClusterDimension;
@@ -48,63 +44,85 @@ template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
     using F = MvFormat<FMT>;
     static constexpr int T = MvTerms<FMT, TX, GRAD>::T, RP = 8 * NT / T;
     static constexpr int TILE = GRAD ? kMvCols : kMvRows, STEP = GRAD ? kMvRows : kMvCols;
-    static constexpr int RING = kMvWarps * mv_ring<NT>() * F::STAGE;
-    static constexpr int RED = kMvWarps * mv_red_size<FMT, TX, NT, GRAD>() * 4;
-    static constexpr int XROWS = GRAD && FMT == MVLLM_FMT_INT4_G64 ? RP : 8 * NT;
+    static constexpr int WARPS = mv_warps<NT, GRAD>(), THREADS = 32 * WARPS;
+    static constexpr int RING = WARPS * mv_ring<NT, GRAD>() * F::STAGE;
+    static constexpr int RED = mv_red_size<FMT, TX, NT, GRAD>() * 4; // bytes of a task's sums
 
     // Shared memory for `chunk` staged stages; fills the plan's offsets.
-    static int layout(MatvecPlan &p, int chunk, int nb) {
-        const int cols = chunk * STEP;
-        int at = mv_alias<NT, GRAD>() ? std::max(RING, RED) : RING;
+    static int layout(MatvecPlan &p, int chunk, int ranks, int nb) {
+        const int cols = chunk * STEP, n = std::min(RP, p.rows_most), red = p.wo * p.wk * RED;
+        int at = mv_alias<GRAD>() ? std::max(RING, red) : RING;
         p.off_red = 0;
-        if (!mv_alias<NT, GRAD>())
-            p.off_red = at, at += RED;
+        if (!mv_alias<GRAD>())
+            p.off_red = at, at += red;
         at = (at + 127) & ~127;
-        p.off_x = at, at += XROWS * mv_x_pitch<FMT, TX, GRAD>(cols);
+        p.off_x = at;
+        at += (GRAD && FMT == MVLLM_FMT_INT4_G64 ? n : n * T) * mv_x_pitch<FMT, TX, GRAD>(cols);
         p.off_ex = at, at += GRAD ? 0 : cols / F::G * RP * 4;
+        p.off_mail = at; // two buffers
+        if (ranks > 1)
+            at += 2 * ((p.wo * TILE / 32 * RP + ranks - 1) / ranks) * ranks * 128;
         p.off_list = at, at += (nb + 1) * 4;
         p.chunk = chunk;
         return at;
     }
 
     // How the work is cut.  The candidates are clusters of 1, 2, 4 or 8 CTAs
-    // along the reduction and 1 to 16 warps along the outputs; the rule
-    // estimates each one's time from the bytes a CTA streams (the device's
-    // rate shared by the CTAs in flight, at most 70 B/ns for one), the stages
-    // a warp takes one after another, the rows it stages and a fixed cost per
-    // unit, times the rounds that the units need.
-    static int plan(const void *kern, MatvecPlan &p, int items, int nb, int sms, int *ranks,
-                    int *grid) {
+    // along the reduction, ranges of wo tiles and wk parts of each; the rule
+    // estimates each one's time: the stages that a CTA's warps take one after
+    // another at the rate of its share of the memory or of what its warps
+    // dequantise, a fixed cost per unit, the rounds that the units need, and
+    // the rows it stages.
+    static int plan(const void *kern, MatvecPlan &p, int rows_each, int items, int nb, int sms,
+                    int *ranks, int *grid) {
         const int tiles = (p.N + TILE - 1) / TILE, steps = (p.K + STEP - 1) / STEP;
+        const double compute = (GRAD ? 26.0 : 40.0) / (1.0 + 0.25 * (NT - 1)); // B/ns of a CTA
+        const int most = GRAD ? WARPS : 64;
         double best = 1e30;
         MatvecPlan q = p;
         for (int c = 1; c <= 8; c *= 2) {
             const int slice = (steps + c - 1) / c;
             if (c > 1 && slice * (c - 1) >= steps)
                 break;
-            int chunk = slice;
-            while (chunk > 1 && layout(q, chunk, nb) > kMvSmem)
-                chunk = chunk > 8 ? chunk * 7 / 8 : chunk - 1;
-            int nc = 0;
-            if (int rc = max_clusters(kern, c, layout(q, chunk, nb), sms, &nc))
-                return rc;
-            for (int wo = 1; wo <= kMvWarps; ++wo) {
-                const int wk = std::min(kMvWarps / wo, slice);
-                const int nr = (tiles + wo - 1) / wo;
-                const double units = double(items) * nr, busy = std::min<double>(units, nc);
-                const double rounds = std::ceil(units / nc);
-                const double bytes = double(std::min(wo, tiles)) * slice * F::STAGE;
-                const double rate = std::min(70.0, 6000.0 / (busy * c));
-                const double serial = 250.0 * ((slice + wk - 1) / wk);
-                const double rows = double(RP) * slice * STEP * sizeof(TX) / 60.0;
-                const double t = rounds * (std::max(bytes / rate, serial) + rows + 1500.0 +
-                                           (c > 1 ? 300.0 : 0.0));
-                if (t < best) {
-                    best = t;
-                    p.range = wo * TILE, p.nranges = nr, p.wo = wo, p.wk = wk, p.slice = slice;
-                    p.chunk = chunk;
-                    *ranks = c;
-                    *grid = int(std::min<double>(units, nc)) * c;
+            int nc = sms;
+            if (c > 1)
+                if (int rc = max_clusters(kern, THREADS, c, kMvSmem, &nc))
+                    return rc;
+            for (int wo = 1; wo <= std::min(most, tiles); ++wo) {
+                for (int wk = 1; wo * wk <= most && wk <= slice && wk <= WARPS; ++wk) {
+                    q.wo = wo, q.wk = wk;
+                    int chunk = slice;
+                    while (chunk > 1 && layout(q, chunk, c, nb) > kMvSmem)
+                        chunk = chunk > 8 ? chunk * 7 / 8 : chunk - 1;
+                    if (layout(q, chunk, c, nb) > kMvSmem)
+                        continue;
+                    const int tasks = wo * wk, active = std::min(tasks, WARPS);
+                    const int serial = (tasks + WARPS - 1) / WARPS * ((slice + wk - 1) / wk);
+                    const int nr = (tiles + wo - 1) / wo;
+                    const double units = double(items) * nr, busy = std::min<double>(units, nc);
+                    const double rounds = std::ceil(units / nc);
+                    const double chunks = (slice + chunk - 1) / chunk;
+                    // fewer warps than three quarters: the CTA is slower itself
+                    const double rate = std::min(compute * std::min(1.0, active / (0.75 * WARPS)),
+                                                 6000.0 / (busy * c));
+                    const double stage = std::max(active * F::STAGE / rate, 400.0);
+                    // rows are staged once per matrix, or, in chunks, for every
+                    // unit with nothing else under way
+                    const double rows = std::min<double>(RP, rows_each) * slice * STEP / 20.0;
+                    const double stagings = chunks > 1 ? rounds : std::ceil(items / double(nc));
+                    const double t = rounds * (serial * stage + 1500.0 + 5000.0 * (chunks - 1) +
+                                               (c > 1 ? 500.0 : 0.0)) +
+                                     stagings * (rows + 500.0);
+                    if (t < best) {
+                        best = t;
+                        p.wo = wo, p.wk = wk, p.range = wo * TILE, p.nranges = nr;
+                        p.slice = slice, p.chunk = chunk;
+                        // the survey of the rows costs about as much as it
+                        // saves a warp in four stages
+                        p.try_common = chunks == 1 && (nb > 1 ? 1 : rounds) * serial > 4;
+                        *ranks = c;
+                        *grid = int(busy) * c;
+                    }
                 }
             }
         }
@@ -116,14 +134,15 @@ template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
         auto kern = matvec_q4_kernel<FMT, TX, NT, GRAD>;
         int ranks = 1, grid = 1;
         MVB_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMvSmem));
-        if (int rc = plan(reinterpret_cast<const void *>(kern), p, items, a.nb, sms, &ranks, &grid))
+        if (int rc = plan(reinterpret_cast<const void *>(kern), p, (a.rows + a.nb - 1) / a.nb, items, a.nb,
+                          sms, &ranks, &grid))
             return rc;
-        const int smem = layout(p, p.chunk, a.nb);
+        const int smem = layout(p, p.chunk, ranks, a.nb);
         if (smem > kMvSmem)
             return host_fail(MVLLM_ERR_UNSUPPORTED, "matvec_q4: %d bytes of shared memory", smem);
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(grid);
-        cfg.blockDim = dim3(kMvThreads);
+        cfg.blockDim = dim3(THREADS);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = st;
         cudaLaunchAttribute at[2];
@@ -149,7 +168,7 @@ int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, int s
         return a.nb == 1 ? (a.rows + rp - 1) / rp
                          : std::min(a.rows, a.nb * ((avg + rp - 1) / rp));
     };
-    const int want = a.nb == 1 ? avg : avg + avg / 2;
+    const int want = a.nb == 1 ? avg : avg + 1;
     if (want <= 8 / T)
         return MvHost<FMT, TX, 1, GRAD>::launch(st, a, p, items(8 / T), sms, x, ldx, y, ldy);
     if (GRAD || want <= 16 / T)
@@ -183,6 +202,7 @@ int matvec_any(const char *who, void *stream, bool grad, const MatvecArgs &a, co
     MatvecPlan p{};
     p.N = out, p.K = grad ? a.O : a.I;
     p.y_f32 = y_dtype == MVLLM_DTYPE_F32;
+    p.rows_most = a.rows;
     const bool fx = x_dtype == MVLLM_DTYPE_F32, i4 = a.fmt == MVLLM_FMT_INT4_G64;
     p.x_vec = ((reinterpret_cast<uintptr_t>(x) | uint64_t(ldx) * (fx ? 4 : 2)) & 15u) == 0;
     if (i4)

@@ -40,28 +40,37 @@ __device__ __forceinline__ bool matvec_expert(const MatvecArgs &a, int e, const 
     return r0 < r1;
 }
 
-constexpr int kMvWarps = 16, kMvThreads = 32 * kMvWarps;
-constexpr int kMvRows = 32, kMvCols = 128; // weights of a warp's stage
-constexpr int kMvMaxExperts = 1024;
+// Warps of a CTA (one CTA per SM) and stages of a warp's ring.  The forward
+// product is bound by the instructions of the dequantisation and wants as many
+// warps to interleave as registers and the staged rows leave room for; the
+// gradient holds 64 or 128 sums per lane.
+template <int NT, bool GRAD> constexpr int mv_warps() {
+    return GRAD || NT == 4 ? 8 : NT == 2 ? 12 : 16;
+}
+template <int NT, bool GRAD> constexpr int mv_ring() { return GRAD ? 4 : 2; }
 constexpr int kMvSmem = 226 * 1024; // dynamic part of the 227 KB
+constexpr int kMvRows = 32, kMvCols = 256; // weights of a warp's stage
+constexpr int kMvMaxExperts = 1024;
 
 // How a launch cuts its work, filled by the host (matvec_plan).
 struct MatvecPlan {
     int N, K;      // outputs and reduction length: (O, I) forward, (I, O) gradient
     int range;     // outputs of a unit
     int nranges;   // units that cover N
-    int wo, wk;    // warps along the outputs and along the reduction
+    int wo, wk;    // tiles of a range, parts of each along the reduction
     int slice;     // stages of the reduction per CTA of the cluster
     int chunk;     // stages whose rows are staged in shared memory at a time
     int x_vec;     // rows of x start on 16-byte boundaries
+    int rows_most; // rows that one matrix can have
     int y_f32;
-    int off_x, off_ex, off_red, off_list; // shared memory (ring at 0)
+    int try_common; // a main loop long enough to pay for the survey of the rows
+    int off_x, off_ex, off_red, off_mail, off_list; // shared memory (ring at 0)
 };
 
 // Per-format geometry of a stage.
 template <int FMT> struct MvFormat {
     static constexpr int G = FMT == MVLLM_FMT_INT4_G64 ? 64 : 32; // columns of a scale
-    static constexpr int SB = FMT == MVLLM_FMT_INT4_G64 ? 8 : 4;  // scale bytes of a stage row
+    static constexpr int SB = FMT == MVLLM_FMT_INT4_G64 ? 16 : 8; // scale bytes of a stage row
     static constexpr int STAGE = kMvRows * (kMvCols / 2 + SB);
 };
 
@@ -78,6 +87,9 @@ template <int FMT, typename TX, bool GRAD> struct MvTerms {
 __device__ __forceinline__ void cp_async16_part(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                  : "memory");
+}
+__device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async4_part(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
@@ -120,113 +132,217 @@ __device__ __forceinline__ uint32_t mv_cluster_addr(uint32_t addr, int rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
-// A stage in shared memory: 32 weight rows of 64 bytes, 16-byte chunk c of
-// row r at chunk c ^ f(r), then the rows' scales.  f gives the 8 rows (4 rows
-// by 32 bytes) that the forward (gradient) lanes read together 8 different
-// bank groups.
+// A stage in shared memory: 32 weight rows of 128 bytes, 16-byte chunk c of
+// row r at chunk c ^ f(r), then the rows' scales.  f gives the 8 rows x 16
+// bytes (4 rows x 32 bytes) that the forward (gradient) lanes read together 8
+// different bank groups.
 __device__ __forceinline__ uint32_t mv_chunk(int row, int c) {
-    const int f = (row & 2) | ((row >> 2) & 1);
-    return row * 64 + ((c ^ f) << 4);
+    const int f = ((row & 3) << 1) | ((row >> 2) & 1);
+    return row * 128 + ((c ^ f) << 4);
 }
 
-// Fills a stage with rows row0.. of a matrix [rows, I] and columns
-// 128 * cs...  Bytes past the matrix's rows or columns become 0, their scales
-// too.  Aligned matrices are copied asynchronously, others through registers
-// byte by byte where their addresses ask for it.
-template <int FMT>
-__device__ __forceinline__ void mv_fill(uint32_t st, const uint8_t *w, const uint8_t *s, int rows,
-                                        int I, int row0, int cs, bool w_al, bool s_al) {
+__device__ __forceinline__ void cp_async8_part(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                 : "memory");
+}
+
+// A warp's walk over a matrix [rows, I] in stages of 32 rows x 256 columns,
+// along the columns (forward) or down the rows (gradient): 128 contiguous
+// bytes of a row at a time.  (With 64, at the same bytes in flight, the
+// stream ran at 3 TB/s.)  A lane copies 16 bytes of rows lane / 8 + 0, 4, ..
+// 28 and the scales of row `lane`.  Bytes past the matrix's rows or columns
+// become 0, their scales too.  Aligned matrices are copied asynchronously,
+// others through registers, byte by byte where their addresses ask for it.
+template <int FMT, bool GRAD> struct MvWalk {
     using F = MvFormat<FMT>;
-    const int lane = threadIdx.x & 31;
-    const int rb = (I + 1) >> 1;
+    static constexpr int SW = FMT == MVLLM_FMT_INT4_G64 ? 4 : 1; // bytes of a scale
+    const uint8_t *w, *s; // this lane's first weight chunk and scale of step 0
+    int rb, ng;           // bytes and scale groups of a row
+    int row, col;         // first row and column-step of step 0
+    int rows;
+    bool w_al;
+    int s_al; // bytes that the scales can be copied by (0: one by one)
+
+    __device__ __forceinline__ void start(const uint8_t *w0, const uint8_t *s0, int rows_, int I,
+                                          int row_, int col_) {
+        const int lane = threadIdx.x & 31;
+        rb = (I + 1) >> 1, ng = (I + F::G - 1) / F::G;
+        row = row_, col = col_, rows = rows_;
+        w_al = ((reinterpret_cast<uintptr_t>(w0) | unsigned(rb)) & 15u) == 0;
+        const unsigned sa = unsigned(reinterpret_cast<uintptr_t>(s0)) | unsigned(ng * SW);
+        s_al = (sa & (F::SB - 1)) == 0 ? F::SB : (sa & 3) == 0 ? 4 : 0;
+        w = w0 + int64_t(row + (lane >> 3)) * rb + int64_t(col) * (kMvCols / 2) + (lane & 7) * 16;
+        s = s0 + (int64_t(row + lane) * ng + int64_t(col) * (kMvCols / F::G)) * SW;
+    }
+    // Copies stage `step` (steps of 256 columns or of 32 rows from the start).
+    __device__ __forceinline__ void fill(uint32_t st, int step) const {
+        const int lane = threadIdx.x & 31;
+        const int r0 = GRAD ? row + step * kMvRows : row;
+        const int cs = GRAD ? col : col + step;
+        const uint8_t *wp =
+            w + (GRAD ? int64_t(step) * kMvRows * rb : int64_t(step) * (kMvCols / 2));
+        const uint8_t *sp = s + (GRAD ? int64_t(step) * kMvRows * ng * SW : int64_t(step) * F::SB);
+        const int at = cs * (kMvCols / 2) + (lane & 7) * 16;
+        const int left_rows = rows - r0 - (lane >> 3);
+        const bool inside = rows - r0 >= kMvRows && (cs + 1) * (kMvCols / 2) <= rb;
+        if (w_al && inside) { // uniform over the warp
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int id = lane + 32 * q, r = id >> 2, c = id & 3;
-        const int at = cs * 64 + c * 16;
-        const uint8_t *src = w + int64_t(row0 + r) * rb + at;
-        const bool in = row0 + r < rows;
-        const uint32_t dst = st + mv_chunk(r, c);
-        if (w_al) {
-            const bool ok = in && at < rb;
-            cp_async16_part(dst, ok ? src : w, ok ? 16 : 0);
+            for (int q = 0; q < 8; ++q)
+                cp_async16_at(st + mv_chunk((lane >> 3) + 4 * q, lane & 7),
+                              wp + uint64_t(uint32_t(4 * rb)) * q);
+        } else if (w_al) {
+            const bool ok = at < rb;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const bool in = ok && 4 * q < left_rows;
+                cp_async16_part(st + mv_chunk((lane >> 3) + 4 * q, lane & 7),
+                                in ? wp + int64_t(4 * q) * rb : w, in ? 16 : 0);
+            }
+        } else {
+            for (int q = 0; q < 8; ++q)
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t v = 0;
+                    if (4 * q < left_rows) {
+                        const uint8_t *p = wp + int64_t(4 * q) * rb + 4 * k;
+                        const int left = rb - at - 4 * k;
+                        if (left >= 4 && (reinterpret_cast<uintptr_t>(p) & 3u) == 0)
+                            v = *reinterpret_cast<const uint32_t *>(p);
+                        else
+                            for (int b = 0; b < 4 && b < left; ++b)
+                                v |= uint32_t(p[b]) << (8 * b);
+                    }
+                    sts32(st + mv_chunk((lane >> 3) + 4 * q, lane & 7) + 4 * k, v);
+                }
+        }
+        const uint32_t sd = st + kMvRows * 128 + lane * F::SB;
+        const int g0 = cs * (kMvCols / F::G);
+        const int left = r0 + lane < rows ? min(ng - g0, kMvCols / F::G) * SW : 0; // bytes
+        if (s_al == F::SB) { // whole stages: rows of a multiple of SB bytes
+            if constexpr (F::SB == 16)
+                cp_async16_part(sd, left > 0 ? sp : s, left > 0 ? 16 : 0);
+            else
+                cp_async8_part(sd, left > 0 ? sp : s, left > 0 ? 8 : 0);
+        } else if (s_al == 4) {
+#pragma unroll
+            for (int k = 0; k < F::SB / 4; ++k)
+                cp_async4_part(sd + 4 * k, left > 4 * k ? sp + 4 * k : s, left > 4 * k ? 4 : 0);
         } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < F::SB / 4; ++k) {
                 uint32_t v = 0;
-                if (in) {
-                    const uint8_t *p = src + 4 * k;
-                    const int left = rb - at - 4 * k;
-                    if (left >= 4 && (reinterpret_cast<uintptr_t>(p) & 3u) == 0)
-                        v = *reinterpret_cast<const uint32_t *>(p);
-                    else
-                        for (int b = 0; b < 4 && b < left; ++b)
-                            v |= uint32_t(p[b]) << (8 * b);
-                }
-                sts32(dst + 4 * k, v);
-            }
-        }
-    }
-    // Scales: lane = row.
-    const uint32_t sd = st + kMvRows * 64 + lane * F::SB;
-    const int ng = (I + F::G - 1) / F::G;
-    const bool in = row0 + lane < rows;
-    if constexpr (FMT == MVLLM_FMT_INT4_G64) {
-        const int g0 = cs * 2;
-        const uint8_t *src = s + (int64_t(row0 + lane) * ng + g0) * 4;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const bool ok = in && g0 + k < ng;
-            if (s_al) {
-                cp_async4_part(sd + 4 * k, ok ? src + 4 * k : s, ok ? 4 : 0);
-            } else {
-                uint32_t v = 0;
-                if (ok)
-                    for (int b = 0; b < 4; ++b)
-                        v |= uint32_t(src[4 * k + b]) << (8 * b);
+                for (int b = 0; b < 4; ++b)
+                    if (4 * k + b < left)
+                        v |= uint32_t(sp[4 * k + b]) << (8 * b);
                 sts32(sd + 4 * k, v);
             }
         }
-    } else {
-        const int g0 = cs * 4;
-        const uint8_t *src = s + int64_t(row0 + lane) * ng + g0;
-        if (s_al) {
-            const bool ok = in && g0 < ng;
-            cp_async4_part(sd, ok ? src : s, ok ? 4 : 0);
-        } else {
-            uint32_t v = 0;
-            for (int b = 0; b < 4; ++b)
-                if (in && g0 + b < ng)
-                    v |= uint32_t(src[b]) << (8 * b);
-            sts32(sd, v);
-        }
     }
-}
+};
 
-// 8 elements of a row from column c, 0 past K.
-template <typename TX>
-__device__ __forceinline__ void mv_load8(const TX *row, int c, int K, bool vec, float (&v)[8]) {
-    if (vec && c + 8 <= K) {
-        if constexpr (sizeof(TX) == 4) {
-            load_row<8>(row + c, v);
-        } else {
-            load_row<8>(row + c, v);
-        }
-    } else {
+// 8 elements of a row, as loaded; 0 past K.
+template <typename TX> struct MvRaw {
+    uint4 u[sizeof(TX) / 2];
+    __device__ __forceinline__ void load(const TX *row, int c, int K, bool vec) {
+        if (vec && c + 8 <= K) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            float e[1] = {0.f};
-            if (c + q < K)
-                load_row<1>(row + c + q, e);
-            v[q] = e[0];
+            for (int q = 0; q < int(sizeof(TX)) / 2; ++q) // stays where it is written
+                asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(u[q].x), "=r"(u[q].y), "=r"(u[q].z), "=r"(u[q].w)
+                             : "l"(reinterpret_cast<const uint4 *>(row + c) + q)
+                             : "memory");
+        } else {
+            uint32_t w[sizeof(TX) * 2];
+#pragma unroll
+            for (int q = 0; q < int(sizeof(TX)) * 2; ++q) {
+                w[q] = 0;
+                if constexpr (sizeof(TX) == 4) {
+                    if (c + q < K)
+                        w[q] = __float_as_uint(row[c + q]);
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+                        if (c + 2 * q + b < K)
+                            w[q] |= uint32_t(__bfloat16_as_ushort(row[c + 2 * q + b])) << (16 * b);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < int(sizeof(TX)) / 2; ++q)
+                u[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
         }
     }
-}
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint4 a = u[0];
+        if constexpr (sizeof(TX) == 4) {
+            const uint4 b = u[1];
+            v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y);
+            v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
+            v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y);
+            v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
+        } else {
+            v[0] = bf16_lo(a.x), v[1] = bf16_hi(a.x), v[2] = bf16_lo(a.y), v[3] = bf16_hi(a.y);
+            v[4] = bf16_lo(a.z), v[5] = bf16_hi(a.z), v[6] = bf16_lo(a.w), v[7] = bf16_hi(a.w);
+        }
+    }
+};
+
+// Walks the groups of 8 elements of the rows to stage: group `tid` first, then
+// every THREADS-th, as (row, group of the row).
+template <int THREADS> struct MvGroups {
+    int r, q, per;
+    __device__ __forceinline__ explicit MvGroups(int per_) : r(0), q(threadIdx.x), per(per_) {
+        settle();
+    }
+    __device__ __forceinline__ void settle() {
+        while (q >= per)
+            q -= per, ++r;
+    }
+    __device__ __forceinline__ void next() {
+        q += THREADS;
+        settle();
+    }
+};
+
+// The gradient's rows: a thread's first HOLD groups, loaded before the weights'
+// copies are issued; behind them in the memory system the rows would arrive
+// some microseconds later, and the main loop waits for them.
+template <typename TX, int NT> struct MvHeld {
+    static constexpr int THREADS = 32 * mv_warps<NT, true>();
+    static constexpr int HOLD = sizeof(TX) == 4 ? 4 : 8;
+    MvRaw<TX> raw[HOLD];
+    __device__ __forceinline__ void load(const TX *x, int64_t ldx, int r0, int n, int c0, int cols,
+                                         int K, bool vec) {
+        MvGroups<THREADS> at(cols / 8);
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h, at.next())
+            if (at.r < n)
+                raw[h].load(x + int64_t(r0 + at.r) * ldx, c0 + at.q * 8, K, vec);
+    }
+    // f(raw, r, q) for every group of the n rows, the held ones from registers.
+    template <typename F>
+    __device__ __forceinline__ void each(const TX *x, int64_t ldx, int r0, int n, int c0, int cols,
+                                         int K, bool vec, bool have, F f) const {
+        MvGroups<THREADS> at(cols / 8);
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h, at.next()) {
+            if (at.r < n) {
+                MvRaw<TX> now = raw[h];
+                if (!have)
+                    now.load(x + int64_t(r0 + at.r) * ldx, c0 + at.q * 8, K, vec);
+                f(now, at.r, at.q);
+            }
+        }
+        for (; at.r < n; at.next()) {
+            MvRaw<TX> now;
+            now.load(x + int64_t(r0 + at.r) * ldx, c0 + at.q * 8, K, vec);
+            f(now, at.r, at.q);
+        }
+    }
+};
+
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -249,93 +365,204 @@ template <int T> __device__ __forceinline__ float mv_term(float v, int term) {
     return term == 0 ? h : term == 1 ? m : r - m;
 }
 
-// Stages rows [r0, r0 + n) of x, columns c0 .. c0 + cols, as the B operand.
-// Forward: f16 parts of x * 2^e with e per row and scale group such that the
-// group's largest finite value lies in [2^14, 2^15): parts [8 NT][cols]
-// (8-column chunks; int4 in its nibble pair order) and 2^-e as ex[group][row].
-// A value 2^-24 of its group's largest keeps all the bits that matter next to
-// it.  Gradient: bf16 parts (MXFP4) or plain f32 (int4), 16 rows of the
-// matrix in the order lane t's four rows t, t + 4, t + 8, t + 12.
-template <int FMT, typename TX, int NT, bool GRAD>
-__device__ __forceinline__ void mv_stage_x(uint8_t *xs, float *ex, int pitch, const TX *x,
-                                           int64_t ldx, int r0, int n, int c0, int cols, int K,
-                                           bool vec) {
-    constexpr int T = MvTerms<FMT, TX, GRAD>::T, RP = 8 * NT / T;
-    if constexpr (!GRAD) {
-        constexpr int GL = MvFormat<FMT>::G / 8; // lanes of a group
-        const int per = cols / 8, tasks = per * RP;
-        for (int b = (threadIdx.x & ~31); b < tasks; b += kMvThreads) {
-            const int id = b + (threadIdx.x & 31);
-            const int r = id / per, q = id - r * per;
-            float v[8] = {};
-            if (id < tasks && r < n)
-                mv_load8(x + int64_t(r0 + r) * ldx, c0 + q * 8, K, vec, v);
-            float m = 0.f;
+__device__ __forceinline__ float finite_max(const float (&v)[8]) {
+    float m = 0.f;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float a = fabsf(v[k]);
-                m = a <= 3.402823466e38f ? fmaxf(m, a) : m;
-            }
+    for (int k = 0; k < 8; ++k)
+        m = fmaxf(m, fabsf(v[k])); // passes NaN over
+    if (m > 3.402823466e38f) {
+        m = 0.f;
 #pragma unroll
-            for (int o = 1; o < GL; o <<= 1)
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            // 2^(14 - floor(log2 m)) and its reciprocal, both normal f32.
-            const int e = m > 0.f ? max(14 - (int(__float_as_uint(m) >> 23) - 127), -113) : 0;
-            const int sh = min(e, 126);
-            const float sc = __uint_as_float(uint32_t(127 + sh) << 23);
-            if (id >= tasks)
-                continue;
-            float h[8], l[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float a = v[k] * sc;
-                h[k] = a;
-                l[k] = fabsf(a) <= 3.402823466e38f ? a - __half2float(__float2half_rn(a)) : 0.f;
-            }
-            const bool i4 = FMT == MVLLM_FMT_INT4_G64;
-#pragma unroll
-            for (int term = 0; term < T; ++term) {
-                const float(&p)[8] = term ? l : h;
-                const uint4 w = i4 ? make_uint4(pack_f16(p[0], p[4]), pack_f16(p[1], p[5]),
-                                                pack_f16(p[2], p[6]), pack_f16(p[3], p[7]))
-                                   : make_uint4(pack_f16(p[0], p[1]), pack_f16(p[2], p[3]),
-                                                pack_f16(p[4], p[5]), pack_f16(p[6], p[7]));
-                *reinterpret_cast<uint4 *>(xs + (r * T + term) * pitch + q * 16) = w;
-            }
-            if ((q & (GL - 1)) == 0)
-                ex[(q / GL) * RP + r] = __uint_as_float(uint32_t(127 - sh) << 23);
+        for (int k = 0; k < 8; ++k) {
+            const float a = fabsf(v[k]);
+            m = a <= 3.402823466e38f ? fmaxf(m, a) : m;
         }
-    } else {
-        constexpr bool I4 = FMT == MVLLM_FMT_INT4_G64;
-        constexpr int R = I4 ? RP : (8 * NT + T - 1) / T; // the last may be partial
-        for (int id = threadIdx.x; id < cols * R; id += kMvThreads) {
-            const int r = id / cols, o = id - r * cols;
-            float v[1] = {0.f};
-            if (r < n && c0 + o < K)
-                load_row<1>(x + int64_t(r0 + r) * ldx + c0 + o, v);
-            if (v[0] != v[0])
-                v[0] = __uint_as_float(0x7fc00000u);
-            const int at = (o & ~15) + (o & 3) * 4 + ((o >> 2) & 3);
-            if constexpr (I4) {
-                *reinterpret_cast<float *>(xs + r * pitch + at * 4) = v[0];
-            } else {
+    }
+    return m;
+}
+// The power of two that brings m into [2^14, 2^15) (m = 0: 1), clamped so
+// that it and its reciprocal are normal f32: its exponent.
+__device__ __forceinline__ int mv_shift(float m) {
+    const int e = int(__float_as_uint(m) >> 23) - 127;
+    return m > 0.f ? min(14 - e, 126) : 0;
+}
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }
+
+// Stages rows [r0, r0 + n) of x, columns c0 .. c0 + cols, as the forward
+// product's B operand: f16 parts of x * 2^e, [n T][cols] in 8-column chunks
+// (int4: in its nibble pair order), and 2^-e in ex.  f16's 30 binades hold a
+// row of activations with one e for all its columns; that is checked: where
+// every scale group's largest finite value (or zero) lies within 2^-12 of its
+// row's, `common` is returned and ex[row] = 2^-e, else e goes by group,
+// ex[group][row].  Either way a group's largest scaled value is at least 4,
+// and what the parts leave of an element is at most 2^-22 of it (nothing, for
+// bf16) or 2^-25, f16's last step: below 2^-26 of the group's largest.
+//
+// The elements come first, as they are, to the places of their parts, which
+// take as many bytes (mv_fetch_rows, asynchronous where rows are aligned);
+// mv_stage_forward then replaces them.
+template <int FMT, typename TX, int NT>
+__device__ __forceinline__ void mv_fetch_rows(uint8_t *xs, int pitch, const TX *x, int64_t ldx,
+                                              int r0, int n, int c0, int cols, int K, bool vec) {
+    constexpr int T = MvTerms<FMT, TX, false>::T;
+    static_assert(sizeof(TX) == 2 * T, "raw elements fit their parts' places");
+    for (MvGroups<32 * mv_warps<NT, false>()> at(cols / 8); at.r < n; at.next()) {
+        const TX *row = x + int64_t(r0 + at.r) * ldx;
+        const int c = c0 + at.q * 8;
+        uint8_t *to = xs + at.r * T * pitch + at.q * 16;
+        if (vec && c + 8 <= K) {
 #pragma unroll
-                for (int term = 0; term < T; ++term)
-                    if (r * T + term < 8 * NT)
-                        *reinterpret_cast<__nv_bfloat16 *>(xs + (r * T + term) * pitch + at * 2) =
-                            __float2bfloat16_rn(mv_term<T>(v[0], term));
-            }
+            for (int term = 0; term < T; ++term)
+                cp_async16_at(smem_u32(to + term * pitch),
+                              reinterpret_cast<const uint4 *>(row + c) + term);
+        } else {
+            MvRaw<TX> raw;
+            raw.load(row, c, K, vec);
+#pragma unroll
+            for (int term = 0; term < T; ++term)
+                *reinterpret_cast<uint4 *>(to + term * pitch) = raw.u[term];
         }
     }
 }
+template <int FMT, typename TX, int NT>
+__device__ __forceinline__ bool mv_stage_forward(uint8_t *xs, float *ex, int pitch, int n, int cols,
+                                                 bool try_common, uint32_t *row_max) {
+    constexpr int T = MvTerms<FMT, TX, false>::T, RP = 8 * NT / T;
+    constexpr int GL = MvFormat<FMT>::G / 8; // lanes of a group
+    using Groups = MvGroups<32 * mv_warps<NT, false>()>;
+    const int lane = threadIdx.x & 31;
+    auto read = [&](const Groups &at, float(&v)[8]) {
+        MvRaw<TX> raw;
+#pragma unroll
+        for (int term = 0; term < T; ++term)
+            raw.u[term] =
+                *reinterpret_cast<const uint4 *>(xs + (at.r * T + term) * pitch + at.q * 16);
+        raw.get(v);
+    };
+    // row_max[r]: bits of the row's largest finite value; [RP + r]: of its
+    // smallest nonzero group maximum.
+    bool common = false;
+    if (try_common) {
+        for (Groups at(cols / 8); at.r < n; at.next()) {
+            float v[8];
+            read(at, v);
+            float m = finite_max(v);
+#pragma unroll
+            for (int o = 1; o < GL; o <<= 1)
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            // cols / 8 is a multiple of 32: a warp has one row; positive f32
+            // order as their bits
+            const uint32_t hi = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+            const uint32_t lo =
+                __reduce_min_sync(0xffffffffu, m > 0.f ? __float_as_uint(m) : 0x7f800000u);
+            if (lane == 0) {
+                atomicMax(&row_max[at.r], hi);
+                atomicMin(&row_max[RP + at.r], lo);
+            }
+        }
+        __syncthreads();
+        bool fits = true;
+        if (int(threadIdx.x) < n) {
+            const float m = __uint_as_float(row_max[threadIdx.x]);
+            fits = __uint_as_float(row_max[RP + threadIdx.x]) >= m * 0x1p-12f;
+            ex[threadIdx.x] = exp2_int(-mv_shift(m));
+        }
+        common = __syncthreads_and(fits);
+    }
+    for (Groups at(cols / 8); at.r < n; at.next()) {
+        float v[8];
+        read(at, v);
+        int sh;
+        if (common) {
+            sh = mv_shift(__uint_as_float(row_max[at.r]));
+        } else {
+            float m = finite_max(v);
+#pragma unroll
+            for (int o = 1; o < GL; o <<= 1)
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            sh = mv_shift(m);
+            if ((at.q & (GL - 1)) == 0)
+                ex[(at.q / GL) * RP + at.r] = exp2_int(-sh);
+        }
+        const float sc = exp2_int(sh);
+        float l[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            v[k] *= sc;
+            l[k] = fabsf(v[k]) <= 3.402823466e38f ? v[k] - __half2float(__float2half_rn(v[k]))
+                                                   : 0.f;
+        }
+#pragma unroll
+        for (int term = 0; term < T; ++term) {
+            const float(&p)[8] = term ? l : v;
+            const uint4 w = FMT == MVLLM_FMT_INT4_G64
+                                ? make_uint4(pack_f16(p[0], p[4]), pack_f16(p[1], p[5]),
+                                             pack_f16(p[2], p[6]), pack_f16(p[3], p[7]))
+                                : make_uint4(pack_f16(p[0], p[1]), pack_f16(p[2], p[3]),
+                                             pack_f16(p[4], p[5]), pack_f16(p[6], p[7]));
+            *reinterpret_cast<uint4 *>(xs + (at.r * T + term) * pitch + at.q * 16) = w;
+        }
+    }
+    return common;
+}
 
-// Forward product of one stage: 32 weight rows x 128 columns on the staged
+// The gradient's B operand: rows of dy as bf16 parts (MXFP4) or as they are
+// (int4, whose scales multiply them first), the 16 rows of a matrix block in
+// the order of lane t's four rows t, t + 4, t + 8, t + 12.
+template <int FMT, typename TX, int NT>
+__device__ __forceinline__ void mv_stage_gradient(uint8_t *xs, int pitch, const TX *x, int64_t ldx,
+                                                  int r0, int n, int c0, int cols, int K, bool vec,
+                                                  bool have, const MvHeld<TX, NT> &held) {
+    constexpr int T = MvTerms<FMT, TX, true>::T;
+    constexpr bool I4 = FMT == MVLLM_FMT_INT4_G64;
+    held.each(x, ldx, r0, n, c0, cols, K, vec, have, [&](const MvRaw<TX> &raw, int r, int q) {
+        float v[8];
+        raw.get(v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (v[k] != v[k])
+                v[k] = __uint_as_float(0x7fc00000u);
+        // elements k and k + 4 lie side by side at place 4 k (+ 2 in the
+        // block's upper half)
+        const int at = (q >> 1) * 16 + (q & 1) * 2;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (I4) {
+                *reinterpret_cast<float2 *>(xs + r * pitch + (at + 4 * k) * 4) =
+                    make_float2(v[k], v[k + 4]);
+            } else {
+#pragma unroll
+                for (int term = 0; term < T; ++term)
+                    *reinterpret_cast<uint32_t *>(xs + (r * T + term) * pitch + (at + 4 * k) * 2) =
+                        pack_bf16(mv_term<T>(v[k], term), mv_term<T>(v[k + 4], term));
+            }
+        }
+    });
+}
+
+// int4x8_to_f16x8 with one shift for eight codes: a nibble in bits 4..7 of a
+// halfword reads as 1024 + 16 n, which one multiply-add turns into n - 8.
+__device__ __forceinline__ void mv_int4x8(uint32_t w, uint32_t (&h)[4]) {
+    const uint32_t u = w >> 8, m0 = 0x000f000fu, m1 = 0x00f000f0u, one = 0x64006400u;
+    uint32_t a, b, c, d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(a) : "r"(w), "r"(m0), "r"(one));
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(b) : "r"(w), "r"(m1), "r"(one));
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(c) : "r"(u), "r"(m0), "r"(one));
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(u), "r"(m1), "r"(one));
+    const uint32_t bias = 0x64086408u, sixteenth = 0x2c002c00u, off = 0xd480d480u; // 1032, 1/16, -72
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(h[0]) : "r"(a), "r"(bias));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(h[1]) : "r"(b), "r"(sixteenth), "r"(off));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(h[2]) : "r"(c), "r"(bias));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(h[3]) : "r"(d), "r"(sixteenth), "r"(off));
+}
+
+// Forward product of one stage: 32 weight rows x 256 columns on the staged
 // columns from xc on.  A lane holds rows g and g + 8 of two 16-row tiles and,
 // of every 32 columns, its own 8: their order along the MMA's K is the same
 // for both operands, so no nibble moves between lanes.  Each scale group's
 // sum starts from zero and is scaled into the f32 accumulator.
-template <int FMT, typename TX, int NT>
-__device__ __forceinline__ void mv_forward(uint32_t st, uint32_t xs, const float *ex, int pitch,
+template <int FMT, typename TX, int NT, bool COMMON>
+__device__ __forceinline__ void mv_forward(uint32_t st, const uint32_t (&xs)[NT], const float *ex,
                                            float (&acc)[2][NT][4]) {
     using F = MvFormat<FMT>;
     constexpr int T = MvTerms<FMT, TX, false>::T, RP = 8 * NT / T;
@@ -346,27 +573,24 @@ __device__ __forceinline__ void mv_forward(uint32_t st, uint32_t xs, const float
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t at = st + kMvRows * 64 + (mt * 16 + h * 8 + g) * F::SB;
+            const uint32_t at = st + kMvRows * 128 + (mt * 16 + h * 8 + g) * F::SB;
             if constexpr (FMT == MVLLM_FMT_INT4_G64) {
-                const uint2 v = lds64(at);
+                const uint4 v = lds128(at);
                 sc[mt][h][0] = __uint_as_float(v.x), sc[mt][h][1] = __uint_as_float(v.y);
+                sc[mt][h][2] = __uint_as_float(v.z), sc[mt][h][3] = __uint_as_float(v.w);
             } else {
-                const uint32_t v = lds32(at);
+                const uint2 v = lds64(at);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    sc[mt][h][k] = ue8m0_byte(v, k);
+                for (int k = 0; k < 4; ++k) {
+                    sc[mt][h][k] = ue8m0_byte(v.x, k);
+                    sc[mt][h][4 + k] = ue8m0_byte(v.y, k);
+                }
             }
         }
 #pragma unroll
     for (int gr = 0; gr < kMvCols / F::G; ++gr) {
         float d[2][NT][4];
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    d[mt][nt][q] = 0.f;
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int bb = 0; bb < BPG; ++bb) {
             const int b = gr * BPG + bb;
@@ -377,17 +601,21 @@ __device__ __forceinline__ void mv_forward(uint32_t st, uint32_t xs, const float
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t w = lds32(st + mv_chunk(mt * 16 + h * 8 + g, b) + t * 4);
                     if constexpr (FMT == MVLLM_FMT_INT4_G64)
-                        int4x8_to_f16x8(w, a[mt][h][0], a[mt][h][1], a[mt][h][2], a[mt][h][3]);
+                        mv_int4x8(w, a[mt][h]);
                     else
                         e2m1x8_to_f16x8(w, a[mt][h][0], a[mt][h][1], a[mt][h][2], a[mt][h][3]);
                 }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const uint4 v = lds128(xs + (nt * 8 + g) * pitch + b * 64 + t * 16);
+                const uint4 v = lds128(xs[nt] + b * 64);
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
-                    mma_f16_16816(d[mt][nt], a[mt][0][0], a[mt][1][0], a[mt][0][1], a[mt][1][1],
-                                  v.x, v.y, d[mt][nt]);
+                    if (bb == 0)
+                        mma_f16_16816(d[mt][nt], a[mt][0][0], a[mt][1][0], a[mt][0][1],
+                                      a[mt][1][1], v.x, v.y, zero);
+                    else
+                        mma_f16_16816(d[mt][nt], a[mt][0][0], a[mt][1][0], a[mt][0][1],
+                                      a[mt][1][1], v.x, v.y, d[mt][nt]);
                     mma_f16_16816(d[mt][nt], a[mt][0][2], a[mt][1][2], a[mt][0][3], a[mt][1][3],
                                   v.z, v.w, d[mt][nt]);
                 }
@@ -395,7 +623,15 @@ __device__ __forceinline__ void mv_forward(uint32_t st, uint32_t xs, const float
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            if constexpr (T == 1) {
+            if constexpr (COMMON) { // the columns' factors follow at the end
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt) {
+                    ffma2(acc[mt][nt][0], acc[mt][nt][1], d[mt][nt][0], d[mt][nt][1],
+                          sc[mt][0][gr]);
+                    ffma2(acc[mt][nt][2], acc[mt][nt][3], d[mt][nt][2], d[mt][nt][3],
+                          sc[mt][1][gr]);
+                }
+            } else if constexpr (T == 1) {
                 const float2 e = *reinterpret_cast<const float2 *>(ex + gr * RP + nt * 8 + 2 * t);
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
@@ -418,30 +654,31 @@ __device__ __forceinline__ void mv_forward(uint32_t st, uint32_t xs, const float
     }
 }
 
-// Gradient product of one stage: W^T, 128 columns x 32 rows.  A lane loads 8
+// Gradient product of one stage: W^T, 256 columns x 32 rows.  A lane loads 8
 // columns (4 bytes) of rows t, t + 4, t + 8, t + 12 of each 16 and pairs two
 // rows' halfwords, after which the nibble extraction yields (row, row + 4)
 // pairs of one column: the transposition costs 4 byte permutes per 32
 // weights.  MXFP4's scale multiplies the bf16 weight, exact as a power of
 // two; int4's f32 scale multiplies the row's value, before it is split.
 template <int FMT, typename TX, int NT>
-__device__ __forceinline__ void mv_gradient(uint32_t st, uint32_t xs, int pitch,
-                                            float (&acc)[2][4][NT][4]) {
+__device__ __forceinline__ void mv_gradient(uint32_t st, const uint32_t (&xs)[NT],
+                                            float (&acc)[4][4][NT][4]) {
     using F = MvFormat<FMT>;
     constexpr bool I4 = FMT == MVLLM_FMT_INT4_G64;
-    constexpr int T = MvTerms<FMT, TX, true>::T, RP = 8 * NT / T;
+    constexpr int T = MvTerms<FMT, TX, true>::T;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-        uint32_t sw[4][I4 ? 2 : 1];
+        uint32_t sw[4][I4 ? 4 : 2];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t at = st + kMvRows * 64 + (kb * 16 + t + 4 * j) * F::SB;
+            const uint32_t at = st + kMvRows * 128 + (kb * 16 + t + 4 * j) * F::SB;
             if constexpr (I4) {
+                const uint4 v = lds128(at);
+                sw[j][0] = v.x, sw[j][1] = v.y, sw[j][2] = v.z, sw[j][3] = v.w;
+            } else {
                 const uint2 v = lds64(at);
                 sw[j][0] = v.x, sw[j][1] = v.y;
-            } else {
-                sw[j][0] = lds32(at);
             }
         }
         uint32_t bx[NT][2]; // MXFP4: the same for every column
@@ -449,20 +686,16 @@ __device__ __forceinline__ void mv_gradient(uint32_t st, uint32_t xs, int pitch,
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             if constexpr (I4) {
-                const int r = (nt * 8 + g) / T;
-                bv[nt] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < RP) {
-                    const uint4 v = lds128(xs + r * pitch + kb * 64 + t * 16);
-                    bv[nt] = make_float4(__uint_as_float(v.x), __uint_as_float(v.y),
-                                         __uint_as_float(v.z), __uint_as_float(v.w));
-                }
+                const uint4 v = lds128(xs[nt] + kb * 64);
+                bv[nt] = make_float4(__uint_as_float(v.x), __uint_as_float(v.y),
+                                     __uint_as_float(v.z), __uint_as_float(v.w));
             } else {
-                const uint2 v = lds64(xs + (nt * 8 + g) * pitch + kb * 32 + t * 8);
+                const uint2 v = lds64(xs[nt] + kb * 32);
                 bx[nt][0] = v.x, bx[nt][1] = v.y;
             }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 4; ++h) {
             uint32_t r[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -492,10 +725,10 @@ __device__ __forceinline__ void mv_gradient(uint32_t st, uint32_t xs, int pitch,
                 // weight's bits being 2^-126 of its value; codes above 128
                 // take 2^126 and then the scale.
                 uint32_t c[4];
-                const int k = h * 2 + (g >> 2);
+                const int k = (h & 1) * 2 + (g >> 2);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    c[j] = (sw[j][0] >> (8 * k)) & 255u;
+                    c[j] = (sw[j][h >> 1] >> (8 * k)) & 255u;
                     high |= c[j] > 128u;
                 }
                 high = __any_sync(0xffffffffu, high);
@@ -542,14 +775,12 @@ __device__ __forceinline__ void mv_gradient(uint32_t st, uint32_t xs, int pitch,
     }
 }
 
-// Ring stages of a warp.
-template <int NT> constexpr int mv_ring() { return NT == 4 ? 3 : 4; }
-// The partial sums share the ring's memory (no copy of the next unit is in
-// flight over the reduction) where both would not fit.
-template <int NT, bool GRAD> constexpr bool mv_alias() { return GRAD || NT == 4; }
-// f32 elements of one warp's partial sums.
+// The gradient's partial sums share the ring's memory (no copy of the next unit
+// is in flight over the reduction): both would not fit.
+template <bool GRAD> constexpr bool mv_alias() { return GRAD; }
+// f32 elements of one task's partial sums.
 template <int FMT, typename TX, int NT, bool GRAD> constexpr int mv_red_pitch() {
-    return GRAD ? 129 : 36;
+    return GRAD ? kMvCols + 1 : 36;
 }
 template <int FMT, typename TX, int NT, bool GRAD> constexpr int mv_red_size() {
     return (GRAD ? 8 * NT : 8 * NT / MvTerms<FMT, TX, GRAD>::T) *
@@ -565,29 +796,90 @@ template <int FMT, typename TX, bool GRAD> __host__ __device__ constexpr int mv_
     return (cols * 2 + 127) / 128 * 128 + 32;
 }
 
+__device__ __forceinline__ void mv_store(void *y, int f32, int64_t at, float v) {
+    if (f32)
+        static_cast<float *>(y)[at] = v;
+    else
+        static_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(v);
+}
+
+// A task's partial sums to shared memory, [row of x][output] (f32 rows: their
+// two parts added), times the rows' factors where those were left out; on top
+// of what an earlier chunk left there when `add`.
+template <int T, int RPITCH, int NT>
+__device__ __forceinline__ void mv_put(float *to, const float (&acc)[2][NT][4], const float *ex,
+                                       bool add) {
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float d[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                d[q] = acc[mt][nt][q];
+            if (T == 1) {
+                if (ex) {
+                    const float2 e = *reinterpret_cast<const float2 *>(ex + nt * 8 + 2 * t);
+                    d[0] *= e.x, d[1] *= e.y, d[2] *= e.x, d[3] *= e.y;
+                }
+                float *at = to + (nt * 8 + 2 * t) * RPITCH + mt * 16 + g;
+                at[0] = add ? at[0] + d[0] : d[0];
+                at[8] = add ? at[8] + d[2] : d[2];
+                at[RPITCH] = add ? at[RPITCH] + d[1] : d[1];
+                at[RPITCH + 8] = add ? at[RPITCH + 8] + d[3] : d[3];
+            } else {
+                if (ex) {
+                    const float e = ex[nt * 4 + t];
+                    d[0] = (d[0] + d[1]) * e, d[2] = (d[2] + d[3]) * e;
+                }
+                float *at = to + (nt * 4 + t) * RPITCH + mt * 16 + g;
+                at[0] = add ? at[0] + d[0] : d[0];
+                at[8] = add ? at[8] + d[2] : d[2];
+            }
+        }
+}
+// The gradient's: [part of a row][output].
+template <int RPITCH, int NT>
+__device__ __forceinline__ void mv_put_gradient(float *to, const float (&acc)[4][4][NT][4]) {
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float(&d)[4] = acc[h][q][nt];
+                float *at = to + (nt * 8 + 2 * t) * RPITCH + h * 64 + 8 * g + q;
+                at[0] = d[0], at[RPITCH] = d[1];
+                at[4] = d[2], at[RPITCH + 4] = d[3];
+            }
+}
+
 struct MvUnit {
     const uint8_t *w, *s;
     int item, r0, n, out0;
-    bool w_al, s_al;
 };
 
 // One CTA of a cluster.  A unit is (rows of one matrix, at most RP of them) x
-// (a range of outputs); the cluster's CTAs split the reduction, each CTA's
-// warps split the range (wo) and the CTA's part of the reduction (wk).  Every
-// warp streams its own tiles through its own ring, so the main loop has no
-// barrier; the partial sums of a unit's wk x cluster parts meet in (distributed)
-// shared memory and are added in a fixed order.
+// (a range of outputs); the cluster's CTAs split the reduction.  A CTA's tasks
+// are the range's tiles x wk parts of its slice of the reduction; its warps
+// take them in turn, each streaming its tasks' stages through its own ring, so
+// the main loop has no barrier.  The wk x cluster partial sums of an output
+// meet in (distributed) shared memory and are added in a fixed order.
 template <int FMT, typename TX, int NT, bool GRAD>
-__global__ void __launch_bounds__(kMvThreads, 1)
+__global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
     matvec_q4_kernel(const MatvecArgs a, const MatvecPlan pl, const TX *__restrict__ x,
                      int64_t ldx, void *__restrict__ y, int64_t ldy) {
     using F = MvFormat<FMT>;
-    constexpr int T = MvTerms<FMT, TX, GRAD>::T, RP = 8 * NT / T, ST = mv_ring<NT>();
+    constexpr int T = MvTerms<FMT, TX, GRAD>::T, RP = 8 * NT / T, ST = mv_ring<NT, GRAD>();
+    constexpr int kMvWarps = mv_warps<NT, GRAD>(), kMvThreads = 32 * kMvWarps;
     constexpr int TILE = GRAD ? kMvCols : kMvRows, STEP = GRAD ? kMvRows : kMvCols;
     constexpr int RPITCH = mv_red_pitch<FMT, TX, NT, GRAD>();
     constexpr int RSIZE = mv_red_size<FMT, TX, NT, GRAD>();
     extern __shared__ __align__(128) uint8_t mv_smem[];
     pdl_wait();
+    pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int rank, ranks, cluster, clusters;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -599,16 +891,18 @@ __global__ void __launch_bounds__(kMvThreads, 1)
     int *list = reinterpret_cast<int *>(mv_smem + pl.off_list); // passes before each expert
     int items;
     if (a.wt) {
-        int n[2];
+        constexpr int PER = (kMvMaxExperts + kMvThreads - 1) / kMvThreads;
         __shared__ int wsum[kMvWarps];
+        int n[PER], v = 0;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int e = 2 * int(threadIdx.x) + k;
+        for (int k = 0; k < PER; ++k) {
+            const int e = PER * int(threadIdx.x) + k;
             const uint8_t *w, *s;
             int r0 = 0, r1 = 0;
             n[k] = e < a.nb && matvec_expert(a, e, w, s, r0, r1) ? (r1 - r0 + RP - 1) / RP : 0;
+            v += n[k];
         }
-        int v = n[0] + n[1];
+        int first = -v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -617,16 +911,18 @@ __global__ void __launch_bounds__(kMvThreads, 1)
         if (lane == 31)
             wsum[warp] = v;
         __syncthreads();
-        int before = 0;
-        for (int k = 0; k < kMvWarps; ++k)
-            before += k < warp ? wsum[k] : 0;
-        const int first = before + v - n[0] - n[1];
-        if (2 * int(threadIdx.x) <= a.nb)
-            list[2 * threadIdx.x] = first;
-        if (2 * int(threadIdx.x) + 1 <= a.nb)
-            list[2 * threadIdx.x + 1] = first + n[0];
-        if (threadIdx.x == kMvThreads - 1 && a.nb == kMvMaxExperts)
-            list[kMvMaxExperts] = first + n[0] + n[1];
+        first += v;
+        for (int k = 0; k < warp; ++k)
+            first += wsum[k];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int e = PER * int(threadIdx.x) + k;
+            if (e < a.nb)
+                list[e] = first;
+            first += n[k];
+            if (e == a.nb - 1)
+                list[a.nb] = first;
+        }
         __syncthreads();
         items = list[a.nb];
     } else {
@@ -656,152 +952,226 @@ __global__ void __launch_bounds__(kMvThreads, 1)
         }
         q.r0 = r0 + pass * RP;
         q.n = min(RP, r1 - q.r0);
-        q.w_al = (reinterpret_cast<uintptr_t>(q.w) & 15u) == 0 && (a.I & 31) == 0;
-        q.s_al = (reinterpret_cast<uintptr_t>(q.s) & 3u) == 0 &&
-                 (FMT == MVLLM_FMT_INT4_G64 || (a.I & 127) == 0);
         return q;
     };
-    // This warp's part of a unit: a tile of outputs and every wk-th stage of
-    // the CTA's slice.
-    const int wo = warp / pl.wk, wk = warp - wo * pl.wk;
     const int steps = (pl.K + STEP - 1) / STEP;
     const int k0 = min(rank * pl.slice, steps), nk = min(pl.slice, steps - k0);
-    auto mine = [&](const MvUnit &q) {
-        const int out = q.out0 + wo * TILE;
-        const int end = min(pl.N, q.out0 + pl.range);
-        return wo < pl.wo && out < end && q.w && nk > wk ? (nk - wk + pl.wk - 1) / pl.wk : 0;
-    };
     const uint32_t ring = smem_u32(mv_smem) + warp * ST * F::STAGE;
-    int head = 0; // ring slot of this warp's next stage to compute
-    auto issue = [&](const MvUnit &q, int i, int n) {
-        if (i < n) {
-            const int step = k0 + wk + i * pl.wk, out = q.out0 + wo * TILE;
-            int slot = head + i;
-            slot %= ST;
-            mv_fill<FMT>(ring + slot * F::STAGE, q.w, q.s, rows_w, a.I,
-                         GRAD ? step * STEP : out, GRAD ? out / kMvCols : step, q.w_al, q.s_al);
+    // Tasks of a unit, and the stages of chunk c0 that part kk of one takes.
+    auto tasks_of = [&](const MvUnit &q) {
+        return q.w ? (min(pl.range, pl.N - q.out0) + TILE - 1) / TILE * pl.wk : 0;
+    };
+    auto stages_of = [&](int c0, int kk) {
+        const int len = min(pl.chunk, nk - c0);
+        return len > kk ? (len - kk + pl.wk - 1) / pl.wk : 0;
+    };
+    // The copies run ahead of the products through the same order: chunks,
+    // this warp's tasks, the task's stages.
+    MvWalk<FMT, GRAD> walk;
+    int w_c0 = 0, w_task = 0, w_i = 0, w_n = 0, w_tasks = 0, filled = 0, used = 0;
+    const uint8_t *w_w = nullptr, *w_s = nullptr;
+    int w_out = 0;
+    auto enter = [&] { // the walk's current task
+        const int kk = w_task % pl.wk;
+        w_i = 0, w_n = stages_of(w_c0, kk);
+        const int out = w_out + w_task / pl.wk * TILE, at = k0 + w_c0 + kk;
+        walk.start(w_w, w_s, rows_w, a.I, GRAD ? at * STEP : out, GRAD ? out / kMvCols : at);
+    };
+    auto issue = [&] {
+        while (w_i >= w_n && w_c0 < nk) { // the next task that has a stage
+            w_task += kMvWarps;
+            if (w_task >= w_tasks) {
+                w_task = warp;
+                w_c0 += pl.chunk;
+                if (w_c0 >= nk)
+                    break;
+            }
+            enter();
         }
+        if (w_i < w_n)
+            walk.fill(ring + (filled % ST) * F::STAGE, w_i++ * pl.wk);
+        ++filled;
         mv_commit();
     };
     auto prologue = [&](const MvUnit &q) {
-        const int n = mine(q);
-        for (int i = 0; i < ST - 1; ++i)
-            issue(q, i, n);
+        w_w = q.w, w_s = q.s, w_out = q.out0, w_tasks = tasks_of(q);
+        w_c0 = 0, w_task = warp, w_i = w_n = 0;
+        filled = used;
+        if (warp < w_tasks)
+            enter();
+        else
+            w_c0 = nk; // nothing to copy
+        issue();
     };
 
     const int cols = pl.chunk * STEP, pitch = mv_x_pitch<FMT, TX, GRAD>(cols);
     const uint32_t xs = smem_u32(mv_smem + pl.off_x);
-    int staged = -1; // the item whose only chunk is staged
+    // Where this lane reads its operand columns.  A column without a row reads
+    // the last one's again: its results are not written.
+    constexpr int XB = GRAD ? (FMT == MVLLM_FMT_INT4_G64 ? 4 : 2) : 2; // bytes of an element
+    uint32_t xcol[NT];
+    int staged = -1;     // the item whose only chunk is staged
+    bool common = false; // its rows have one power of two each
+    int turn = 0;        // the mail buffer of this unit
+    __shared__ uint32_t row_max[GRAD ? 1 : 2 * RP];
+    MvHeld<TX, NT> held; // gradient
+    // The first rows of a unit that has to be staged, then its weights.
+    auto begin = [&](const MvUnit &q) {
+        if (q.w && staged != q.item) {
+            if constexpr (GRAD) {
+                held.load(x, ldx, q.r0, q.n, k0 * STEP, cols, pl.K, pl.x_vec);
+            } else {
+                mv_fetch_rows<FMT, TX, NT>(mv_smem + pl.off_x, pitch, x, ldx, q.r0, q.n, k0 * STEP,
+                                           cols, pl.K, pl.x_vec);
+                if (threadIdx.x < RP)
+                    row_max[threadIdx.x] = 0u, row_max[RP + threadIdx.x] = 0x7f800000u;
+            }
+        }
+        mv_commit();
+        prologue(q);
+    };
     MvUnit cur{};
     if (cluster < total) {
         cur = decode(cluster);
-        prologue(cur);
+        begin(cur);
     }
     for (int64_t u = cluster; u < total; u += clusters) {
-        const int n = mine(cur);
-        float accf[GRAD ? 1 : 2][NT][4];
-        float accg[GRAD ? 2 : 1][GRAD ? 4 : 1][NT][4];
-        if constexpr (GRAD) {
+        const int tasks = tasks_of(cur);
 #pragma unroll
-            for (int i = 0; i < 8 * NT * 4; ++i)
-                (&accg[0][0][0][0])[i] = 0.f;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2 * NT * 4; ++i)
-                (&accf[0][0][0])[i] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) {
+            int col = nt * 8 + (lane >> 2);
+            if (GRAD && FMT == MVLLM_FMT_INT4_G64)
+                col = min(col / T, cur.n - 1);
+            else
+                col = min(col, cur.n * T - 1);
+            xcol[nt] = xs + col * pitch + (lane & 3) * (GRAD ? 4 * XB : 16);
         }
-        int i = 0;
+        // The gradient's one task per warp keeps its sums to the end of the
+        // unit; the forward's tasks leave theirs in shared memory one by one.
+        float accg[GRAD ? 4 : 1][GRAD ? 4 : 1][NT][4] = {};
+        bool refilled = false;
         for (int c0 = 0; c0 < nk; c0 += pl.chunk) {
             if (cur.w && staged != cur.item) { // uniform over the CTA
-                __syncthreads(); // the last readers of x are done
-                mv_stage_x<FMT, TX, NT, GRAD>(mv_smem + pl.off_x, ex, pitch, x, ldx, cur.r0,
-                                              cur.n, (k0 + c0) * STEP, cols, pl.K, pl.x_vec);
+                if constexpr (GRAD) {
+                    __syncthreads(); // the last readers of x are done
+                    mv_stage_gradient<FMT, TX, NT>(mv_smem + pl.off_x, pitch, x, ldx, cur.r0, cur.n,
+                                                   (k0 + c0) * STEP, cols, pl.K, pl.x_vec, c0 == 0,
+                                                   held);
+                } else {
+                    if (c0 > 0) {
+                        __syncthreads();
+                        mv_fetch_rows<FMT, TX, NT>(mv_smem + pl.off_x, pitch, x, ldx, cur.r0, cur.n,
+                                                   (k0 + c0) * STEP, cols, pl.K, pl.x_vec);
+                        mv_commit();
+                        mv_wait<0>();
+                    } else {
+                        mv_wait<1>(); // all but the weights' first stage
+                    }
+                    __syncthreads();
+                    common = mv_stage_forward<FMT, TX, NT>(mv_smem + pl.off_x, ex, pitch, cur.n,
+                                                           cols, pl.try_common && nk <= pl.chunk,
+                                                           row_max);
+                }
                 __syncthreads();
                 if (nk <= pl.chunk)
                     staged = cur.item;
             }
-            for (; i < n; ++i) {
-                const int step = wk + i * pl.wk - c0; // within the chunk
-                if (step >= pl.chunk)
-                    break;
-                mv_wait<ST - 2>();
+            // The ring's other stages, now that the rows are staged: the first
+            // kept the memory system busy meanwhile, more would only have
+            // queued in front of them.
+            for (int k = refilled ? ST : 1; k < ST - 1; ++k)
+                issue();
+            refilled = true;
+            for (int task = warp; task < tasks; task += kMvWarps) {
+                const int kk = task % pl.wk, n = stages_of(c0, kk);
+                float accf[GRAD ? 1 : 2][NT][4] = {};
+                for (int i = 0; i < n; ++i) {
+                    mv_wait<ST - 2>();
+                    __syncwarp();
+                    issue(); // into the slot computed last
+                    const uint32_t st = ring + (used++ % ST) * F::STAGE;
+                    const int step = kk + i * pl.wk; // within the chunk
+                    uint32_t xat[NT];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        xat[nt] = xcol[nt] + step * (STEP * XB);
+                    if constexpr (GRAD)
+                        mv_gradient<FMT, TX, NT>(st, xat, accg);
+                    else if (common)
+                        mv_forward<FMT, TX, NT, true>(st, xat, ex, accf);
+                    else
+                        mv_forward<FMT, TX, NT, false>(st, xat, ex + step * (STEP / F::G) * RP,
+                                                       accf);
+                }
                 __syncwarp();
-                issue(cur, i + ST - 1, n); // into the slot computed last
-                const uint32_t st = ring + ((head + i) % ST) * F::STAGE;
-                if constexpr (GRAD)
-                    mv_gradient<FMT, TX, NT>(
-                        st, xs + step * STEP * (FMT == MVLLM_FMT_INT4_G64 ? 4 : 2), pitch, accg);
-                else
-                    mv_forward<FMT, TX, NT>(st, xs + step * STEP * 2,
-                                            ex + step * (STEP / F::G) * RP, pitch, accf);
+                if constexpr (!GRAD)
+                    mv_put<T, RPITCH>(red + task * RSIZE, accf, common ? ex : nullptr, c0 > 0);
             }
         }
-        head = (head + n) % ST;
-        __syncwarp();
         MvUnit next{};
         if (u + clusters < total)
             next = decode(u + clusters);
-        if constexpr (!mv_alias<NT, GRAD>()) {
-            if (u + clusters < total)
-                prologue(next);
-        } else {
+        if constexpr (mv_alias<GRAD>()) {
             mv_wait<0>();
             __syncthreads(); // the ring is done with before the sums overlay it
+            if (warp < tasks)
+                mv_put_gradient<RPITCH>(red + warp * RSIZE, accg);
         }
-        // Partial sums [column][output] of this warp.
-        float *mr = red + warp * RSIZE;
-        const int g = lane >> 2, t = lane & 3;
-        if constexpr (GRAD) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const float(&d)[4] = accg[h][q][nt];
-                        float *at = mr + (nt * 8 + 2 * t) * RPITCH + h * 64 + 8 * g + q;
-                        at[0] = d[0], at[RPITCH] = d[1];
-                        at[4] = d[2], at[RPITCH + 4] = d[3];
-                    }
-        } else {
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const float(&d)[4] = accf[mt][nt];
-                    float *at = mr + (T == 1 ? nt * 8 + 2 * t : nt * 4 + t) * RPITCH + mt * 16 + g;
-                    at[0] = d[0], at[8] = d[2];
-                    if (T == 1)
-                        at[RPITCH] = d[1], at[RPITCH + 8] = d[3];
-                }
+        __syncthreads();
+        if constexpr (!mv_alias<GRAD>()) { // the rows' places are free now
+            if (u + clusters < total)
+                begin(next);
         }
-        mv_cluster_sync();
-        // Each CTA adds up and writes its share of the unit's outputs.
-        const int outs = min(pl.range, pl.N - cur.out0);
-        for (int id = rank * kMvThreads + threadIdx.x; id < outs * cur.n;
-             id += ranks * kMvThreads) {
-            const int r = id / outs, o = id - r * outs;
-            const int w0 = (o / TILE) * pl.wk;
-            const uint32_t at = smem_u32(red + w0 * RSIZE + (GRAD ? r * T : r) * RPITCH + o % TILE);
-            float v = 0.f;
-            for (int c = 0; c < ranks; ++c) {
-                const uint32_t ra = mv_cluster_addr(at, c);
-                for (int k = 0; k < pl.wk; ++k)
+        // The CTA's own wk partial sums (and the gradient's parts) first.  With one CTA per cluster that is the
+        // result; else it goes to the CTA that owns the block, and one cluster
+        // barrier later each CTA adds up what it was sent.  Two buffers take
+        // turns, so that a unit's values cannot meet the next one's.
+        // A warp takes a block of 32 outputs and goes through the rows.
+        const int outs = min(pl.range, pl.N - cur.out0), blocks = (outs + 31) / 32;
+        const int slots = (pl.range / 32 * RP + ranks - 1) / ranks * ranks; // of a mail buffer
+        const uint32_t mail = smem_u32(mv_smem + pl.off_mail) + turn * slots * 128;
+        const int parts = cur.w ? pl.wk : 0, mask = ranks - 1;
+        for (int b = warp; b < blocks; b += kMvWarps) {
+            const int o = b * 32 + lane;
+            const float *at = red + (o / TILE) * pl.wk * RSIZE + o % TILE;
+            // item = (row, block), owned by rank item % ranks there, slot
+            // item / ranks * ranks + sender
+            int item = b;
+#pragma unroll 2
+            for (int r = 0; r < cur.n; ++r, item += blocks, at += (GRAD ? T : 1) * RPITCH) {
+                float v = 0.f;
+                for (int k = 0; k < parts; ++k)
 #pragma unroll
                     for (int q = 0; q < (GRAD ? T : 1); ++q)
-                        v += ld_cluster_f32(ra + 4 * (k * RSIZE + q * RPITCH));
+                        v += at[k * RSIZE + q * RPITCH];
+                if (ranks > 1)
+                    st_cluster_f32(mv_cluster_addr(mail + ((item & ~mask) + rank) * 128 + lane * 4,
+                                                   item & mask),
+                                   v);
+                else if (o < outs)
+                    mv_store(y, pl.y_f32, int64_t(cur.r0 + r) * ldy + cur.out0 + o, v);
             }
-            const int64_t to = int64_t(cur.r0 + r) * ldy + cur.out0 + o;
-            if (pl.y_f32)
-                static_cast<float *>(y)[to] = v;
-            else
-                static_cast<__nv_bfloat16 *>(y)[to] = __float2bfloat16_rn(v);
         }
-        mv_cluster_sync(); // the sums are read before they are overwritten
+        if (ranks > 1) {
+            mv_cluster_sync();
+            for (int item = warp * ranks + rank; item < blocks * cur.n; item += kMvWarps * ranks) {
+                const int r = item / blocks, o = (item - r * blocks) * 32 + lane;
+                const uint32_t at = mail + (item & ~mask) * 128 + lane * 4;
+                float v = 0.f;
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    v += c < ranks ? __uint_as_float(lds32(at + c * 128)) : 0.f;
+                if (o < outs)
+                    mv_store(y, pl.y_f32, int64_t(cur.r0 + r) * ldy + cur.out0 + o, v);
+            }
+            turn ^= 1;
+        } else {
+            __syncthreads();
+        }
         cur = next;
-        if constexpr (mv_alias<NT, GRAD>()) {
+        if constexpr (mv_alias<GRAD>()) {
             if (u + clusters < total)
-                prologue(cur);
+                begin(cur);
         }
     }
 }
