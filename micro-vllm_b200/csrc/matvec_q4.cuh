@@ -71,7 +71,11 @@ struct MatvecPlan {
 template <int FMT> struct MvFormat {
     static constexpr int G = FMT == MVLLM_FMT_INT4_G64 ? 64 : 32; // columns of a scale
     static constexpr int SB = FMT == MVLLM_FMT_INT4_G64 ? 16 : 8; // scale bytes of a stage row
-    static constexpr int STAGE = kMvRows * (kMvCols / 2 + SB);
+    // A row's scales take 16 bytes of a stage: MXFP4's 8 come as the aligned 16
+    // that hold them, at (column-step & 1) * 8.  (Copied by 8 bytes they go
+    // through L1, which had no room for the lines of 512 rows: 3.3 against
+    // 5.5 TB/s on 48 experts of 7168 x 2048.)
+    static constexpr int STAGE = kMvRows * (kMvCols / 2 + 16);
 };
 
 // Parts an x element is split into, and rows that 8 * NT operand columns hold.
@@ -84,16 +88,11 @@ template <int FMT, typename TX, bool GRAD> struct MvTerms {
     static constexpr int T = GRAD ? (F32 ? 3 : FMT == MVLLM_FMT_INT4_G64 ? 2 : 1) : (F32 ? 2 : 1);
 };
 
-__device__ __forceinline__ void cp_async16_part(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-                 : "memory");
-}
 __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async4_part(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-                 : "memory");
+__device__ __forceinline__ void cp_async4_at(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void mv_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void mv_wait() {
@@ -145,9 +144,8 @@ __device__ __forceinline__ uint32_t mv_chunk(int row, int c) {
     return row * 128 + ((c ^ f) << 4);
 }
 
-__device__ __forceinline__ void cp_async8_part(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-                 : "memory");
+__device__ __forceinline__ void cp_async8_at(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 
 // A warp's walk over a matrix [rows, I] in stages of 32 rows x 256 columns,
@@ -160,54 +158,86 @@ __device__ __forceinline__ void cp_async8_part(uint32_t dst, const void *src, in
 template <int FMT, bool GRAD> struct MvWalk {
     using F = MvFormat<FMT>;
     static constexpr int SW = FMT == MVLLM_FMT_INT4_G64 ? 4 : 1; // bytes of a scale
-    const uint8_t *w, *s; // this lane's first weight chunk and scale of step 0
+    const uint8_t *w, *s; // this lane's weight chunk and scale of the next stage
+    int64_t dw;           // bytes from one stage's weights to the next one's
+    int ds;               // and scales (times 32 rows: below 2^31)
     int rb, ng;           // bytes and scale groups of a row
-    int row, col;         // first row and column-step of step 0
-    int rows;
-    bool w_al;
-    int s_al; // bytes that the scales can be copied by (0: one by one)
+    int row, col;         // first row and column-step of the next stage
+    int rows, every;      // rows of the matrix; steps from a stage to the next
+    int inside;           // stages ahead that lie in the matrix as a whole
+    int s_al;             // 16, 8 or 4: scales can be copied by so many bytes; 0: one by one
 
+    // From row `row_` and column-step `col_` on, every `every_`-th step.
     __device__ __forceinline__ void start(const uint8_t *w0, const uint8_t *s0, int rows_, int I,
-                                          int row_, int col_) {
+                                          int row_, int col_, int every_) {
         const int lane = threadIdx.x & 31;
         rb = (I + 1) >> 1, ng = (I + F::G - 1) / F::G;
-        row = row_, col = col_, rows = rows_;
-        w_al = ((reinterpret_cast<uintptr_t>(w0) | unsigned(rb)) & 15u) == 0;
+        row = row_, col = col_, rows = rows_, every = every_;
+        const bool w_al = ((reinterpret_cast<uintptr_t>(w0) | unsigned(rb)) & 15u) == 0;
         const unsigned sa = unsigned(reinterpret_cast<uintptr_t>(s0)) | unsigned(ng * SW);
-        s_al = (sa & (F::SB - 1)) == 0 ? F::SB : (sa & 3) == 0 ? 4 : 0;
+        s_al = (sa & 15) == 0 ? 16 : (sa & 7) == 0 ? 8 : (sa & 3) == 0 ? 4 : 0;
         w = w0 + int64_t(row + (lane >> 3)) * rb + int64_t(col) * (kMvCols / 2) + (lane & 7) * 16;
         s = s0 + (int64_t(row + lane) * ng + int64_t(col) * (kMvCols / F::G)) * SW;
+        dw = GRAD ? int64_t(every) * kMvRows * rb : int64_t(every) * (kMvCols / 2);
+        ds = GRAD ? every * kMvRows : every; // row or group steps
+        const int full_rows = rows - row, full_cols = rb / (kMvCols / 2) - col;
+        if (GRAD)
+            inside = full_cols >= 1 ? (full_rows / kMvRows + every - 1) / every : 0;
+        else
+            inside = full_rows >= kMvRows ? (full_cols + every - 1) / every : 0;
+        inside = !w_al ? -1 : max(inside, 0); // -1: not asynchronously either
     }
-    // Copies stage `step` (steps of 256 columns or of 32 rows from the start).
-    __device__ __forceinline__ void fill(uint32_t st, int step) const {
+    // Copies the next stage.
+    __device__ __forceinline__ void fill(uint32_t st) {
         const int lane = threadIdx.x & 31;
-        const int r0 = GRAD ? row + step * kMvRows : row;
-        const int cs = GRAD ? col : col + step;
-        const uint8_t *wp =
-            w + (GRAD ? int64_t(step) * kMvRows * rb : int64_t(step) * (kMvCols / 2));
-        const uint8_t *sp = s + (GRAD ? int64_t(step) * kMvRows * ng * SW : int64_t(step) * F::SB);
-        const int at = cs * (kMvCols / 2) + (lane & 7) * 16;
-        const int left_rows = rows - r0 - (lane >> 3);
-        const bool inside = rows - r0 >= kMvRows && (cs + 1) * (kMvCols / 2) <= rb;
-        if (w_al && inside) { // uniform over the warp
+        const int half = F::SB == 8 ? (col & 1) * 8 : 0;
+        const uint32_t sd = st + kMvRows * 128 + lane * 16;
+        if (inside > 0) { // uniform over the warp
+            const uint32_t d0 = st + mv_chunk(lane >> 3, lane & 7);
+            const uint32_t d1 = st + mv_chunk((lane >> 3) + 4, lane & 7) - 512;
 #pragma unroll
             for (int q = 0; q < 8; ++q)
-                cp_async16_at(st + mv_chunk((lane >> 3) + 4 * q, lane & 7),
-                              wp + uint64_t(uint32_t(4 * rb)) * q);
-        } else if (w_al) {
-            const bool ok = at < rb;
-#pragma unroll
+                cp_async16_at((q & 1 ? d1 : d0) + 512 * q, w + uint64_t(uint32_t(4 * rb)) * q);
+            if (s_al == 16)
+                cp_async16_at(sd, s - half);
+            else if (F::SB == 8 && s_al == 8)
+                cp_async8_at(sd + half, s);
+            else
+                edge_scales(sd + half, s, ng, row, col, rows, s_al != 0);
+            --inside;
+        } else {
+            edge_weights(st, w, rb, row, col, rows, inside == 0);
+            edge_scales(sd + half, s, ng, row, col, rows, s_al != 0);
+        }
+        w += dw;
+        s += int64_t(ds) * (GRAD ? ng * SW : F::SB);
+        if (GRAD)
+            row += every * kMvRows;
+        else
+            col += every;
+    }
+    // A stage at the matrix's edges, or of a matrix that cannot be copied by 16
+    // bytes (`async` false).
+    static __device__ __noinline__ void edge_weights(uint32_t st, const uint8_t *w, int rb,
+                                                     int row, int col, int rows, bool async) {
+        const int lane = threadIdx.x & 31;
+        const int at = col * (kMvCols / 2) + (lane & 7) * 16;
+        const int left_rows = rows - row - (lane >> 3);
+        if (async) {
             for (int q = 0; q < 8; ++q) {
-                const bool in = ok && 4 * q < left_rows;
-                cp_async16_part(st + mv_chunk((lane >> 3) + 4 * q, lane & 7),
-                                in ? wp + int64_t(4 * q) * rb : w, in ? 16 : 0);
+                const uint32_t to = st + mv_chunk((lane >> 3) + 4 * q, lane & 7);
+                if (at < rb && 4 * q < left_rows)
+                    cp_async16_at(to, w + int64_t(4 * q) * rb);
+                else
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(to), "r"(0)
+                                 : "memory");
             }
         } else {
             for (int q = 0; q < 8; ++q)
                 for (int k = 0; k < 4; ++k) {
                     uint32_t v = 0;
                     if (4 * q < left_rows) {
-                        const uint8_t *p = wp + int64_t(4 * q) * rb + 4 * k;
+                        const uint8_t *p = w + int64_t(4 * q) * rb + 4 * k;
                         const int left = rb - at - 4 * k;
                         if (left >= 4 && (reinterpret_cast<uintptr_t>(p) & 3u) == 0)
                             v = *reinterpret_cast<const uint32_t *>(p);
@@ -218,25 +248,20 @@ template <int FMT, bool GRAD> struct MvWalk {
                     sts32(st + mv_chunk((lane >> 3) + 4 * q, lane & 7) + 4 * k, v);
                 }
         }
-        const uint32_t sd = st + kMvRows * 128 + lane * F::SB;
-        const int g0 = cs * (kMvCols / F::G);
-        const int left = r0 + lane < rows ? min(ng - g0, kMvCols / F::G) * SW : 0; // bytes
-        if (s_al == F::SB) { // whole stages: rows of a multiple of SB bytes
-            if constexpr (F::SB == 16)
-                cp_async16_part(sd, left > 0 ? sp : s, left > 0 ? 16 : 0);
-            else
-                cp_async8_part(sd, left > 0 ? sp : s, left > 0 ? 8 : 0);
-        } else if (s_al == 4) {
-#pragma unroll
-            for (int k = 0; k < F::SB / 4; ++k)
-                cp_async4_part(sd + 4 * k, left > 4 * k ? sp + 4 * k : s, left > 4 * k ? 4 : 0);
-        } else {
-#pragma unroll
-            for (int k = 0; k < F::SB / 4; ++k) {
+    }
+    static __device__ __noinline__ void edge_scales(uint32_t sd, const uint8_t *s, int ng, int row,
+                                                    int col, int rows, bool async) {
+        const int lane = threadIdx.x & 31;
+        const int g0 = col * (kMvCols / F::G);
+        const int left = row + lane < rows ? min(ng - g0, kMvCols / F::G) * SW : 0; // bytes
+        for (int k = 0; k < F::SB / 4; ++k) {
+            if (async && left >= 4 * k + 4) { // whole words
+                cp_async4_at(sd + 4 * k, s + 4 * k);
+            } else {
                 uint32_t v = 0;
                 for (int b = 0; b < 4; ++b)
                     if (4 * k + b < left)
-                        v |= uint32_t(sp[4 * k + b]) << (8 * b);
+                        v |= uint32_t(s[4 * k + b]) << (8 * b);
                 sts32(sd + 4 * k, v);
             }
         }
@@ -562,7 +587,8 @@ __device__ __forceinline__ void mv_int4x8(uint32_t w, uint32_t (&h)[4]) {
 // for both operands, so no nibble moves between lanes.  Each scale group's
 // sum starts from zero and is scaled into the f32 accumulator.
 template <int FMT, typename TX, int NT, bool COMMON>
-__device__ __forceinline__ void mv_forward(uint32_t st, const uint32_t (&xs)[NT], const float *ex,
+__device__ __forceinline__ void mv_forward(uint32_t st, int half, const uint32_t (&xs)[NT],
+                                           const float *ex,
                                            float (&acc)[2][NT][4]) {
     using F = MvFormat<FMT>;
     constexpr int T = MvTerms<FMT, TX, false>::T, RP = 8 * NT / T;
@@ -573,7 +599,7 @@ __device__ __forceinline__ void mv_forward(uint32_t st, const uint32_t (&xs)[NT]
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t at = st + kMvRows * 128 + (mt * 16 + h * 8 + g) * F::SB;
+            const uint32_t at = st + kMvRows * 128 + (mt * 16 + h * 8 + g) * 16 + half;
             if constexpr (FMT == MVLLM_FMT_INT4_G64) {
                 const uint4 v = lds128(at);
                 sc[mt][h][0] = __uint_as_float(v.x), sc[mt][h][1] = __uint_as_float(v.y);
@@ -661,7 +687,7 @@ __device__ __forceinline__ void mv_forward(uint32_t st, const uint32_t (&xs)[NT]
 // weights.  MXFP4's scale multiplies the bf16 weight, exact as a power of
 // two; int4's f32 scale multiplies the row's value, before it is split.
 template <int FMT, typename TX, int NT>
-__device__ __forceinline__ void mv_gradient(uint32_t st, const uint32_t (&xs)[NT],
+__device__ __forceinline__ void mv_gradient(uint32_t st, int half, const uint32_t (&xs)[NT],
                                             float (&acc)[4][4][NT][4]) {
     using F = MvFormat<FMT>;
     constexpr bool I4 = FMT == MVLLM_FMT_INT4_G64;
@@ -672,7 +698,7 @@ __device__ __forceinline__ void mv_gradient(uint32_t st, const uint32_t (&xs)[NT
         uint32_t sw[4][I4 ? 4 : 2];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t at = st + kMvRows * 128 + (kb * 16 + t + 4 * j) * F::SB;
+            const uint32_t at = st + kMvRows * 128 + (kb * 16 + t + 4 * j) * 16 + half;
             if constexpr (I4) {
                 const uint4 v = lds128(at);
                 sw[j][0] = v.x, sw[j][1] = v.y, sw[j][2] = v.z, sw[j][3] = v.w;
@@ -975,7 +1001,8 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
         const int kk = w_task % pl.wk;
         w_i = 0, w_n = stages_of(w_c0, kk);
         const int out = w_out + w_task / pl.wk * TILE, at = k0 + w_c0 + kk;
-        walk.start(w_w, w_s, rows_w, a.I, GRAD ? at * STEP : out, GRAD ? out / kMvCols : at);
+        walk.start(w_w, w_s, rows_w, a.I, GRAD ? at * STEP : out, GRAD ? out / kMvCols : at,
+                   pl.wk);
     };
     auto issue = [&] {
         while (w_i >= w_n && w_c0 < nk) { // the next task that has a stage
@@ -988,8 +1015,10 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
             }
             enter();
         }
-        if (w_i < w_n)
-            walk.fill(ring + (filled % ST) * F::STAGE, w_i++ * pl.wk);
+        if (w_i < w_n) {
+            walk.fill(ring + (filled % ST) * F::STAGE);
+            ++w_i;
+        }
         ++filled;
         mv_commit();
     };
@@ -1091,17 +1120,20 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
                     issue(); // into the slot computed last
                     const uint32_t st = ring + (used++ % ST) * F::STAGE;
                     const int step = kk + i * pl.wk; // within the chunk
+                    const int colstep = GRAD ? (cur.out0 + task / pl.wk * TILE) / kMvCols
+                                             : k0 + c0 + step;
+                    const int half = F::SB == 8 ? (colstep & 1) * 8 : 0;
                     uint32_t xat[NT];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
                         xat[nt] = xcol[nt] + step * (STEP * XB);
                     if constexpr (GRAD)
-                        mv_gradient<FMT, TX, NT>(st, xat, accg);
+                        mv_gradient<FMT, TX, NT>(st, half, xat, accg);
                     else if (common)
-                        mv_forward<FMT, TX, NT, true>(st, xat, ex, accf);
+                        mv_forward<FMT, TX, NT, true>(st, half, xat, ex, accf);
                     else
-                        mv_forward<FMT, TX, NT, false>(st, xat, ex + step * (STEP / F::G) * RP,
-                                                       accf);
+                        mv_forward<FMT, TX, NT, false>(
+                            st, half, xat, ex + step * (STEP / F::G) * RP, accf);
                 }
                 __syncwarp();
                 if constexpr (!GRAD)
