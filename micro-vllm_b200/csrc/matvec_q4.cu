@@ -168,7 +168,7 @@ int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, int s
         return a.nb == 1 ? (a.rows + rp - 1) / rp
                          : std::min(a.rows, a.nb * ((avg + rp - 1) / rp));
     };
-    const int want = a.nb == 1 ? avg : avg + 1;
+    const int want = a.nb == 1 || GRAD ? avg : avg + 1;
     if (want <= 8 / T)
         return MvHost<FMT, TX, 1, GRAD>::launch(st, a, p, items(8 / T), sms, x, ldx, y, ldy);
     if (GRAD || want <= 16 / T)

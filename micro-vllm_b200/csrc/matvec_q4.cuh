@@ -686,13 +686,28 @@ __device__ __forceinline__ void mv_forward(uint32_t st, int half, const uint32_t
 // pairs of one column: the transposition costs 4 byte permutes per 32
 // weights.  MXFP4's scale multiplies the bf16 weight, exact as a power of
 // two; int4's f32 scale multiplies the row's value, before it is split.
-template <int FMT, typename TX, int NT>
+//
+// int4's parts (`col` = this lane's operand column): its own part of a
+// product p is picked without a branch, hi = p's upper 16 bits, r = p - hi:
+// one of 1 * hi, 1 * r, ... by factors 0 and 1, exact.  A product that is not
+// finite comes out as NaN that way; the caller notices the NaN in its sums and
+// repeats the unit with CAREFUL, which keeps such a product whole in its first
+// part.  For MXFP4 CAREFUL stands for scale codes 0 and above 127, which the
+// short form of the scale's bits does not cover.
+template <int FMT, typename TX, int NT, bool CAREFUL>
 __device__ __forceinline__ void mv_gradient(uint32_t st, int half, const uint32_t (&xs)[NT],
                                             float (&acc)[4][4][NT][4]) {
-    using F = MvFormat<FMT>;
     constexpr bool I4 = FMT == MVLLM_FMT_INT4_G64;
     constexpr int T = MvTerms<FMT, TX, true>::T;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float pick[NT][3]; // int4: factors of hi, r (T = 2) or hi, r, mid (T = 3)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int term = (nt * 8 + g) % T;
+        pick[nt][0] = term == 0 ? 1.f : 0.f;
+        pick[nt][1] = term == T - 1 ? 1.f : 0.f;
+        pick[nt][2] = term == 1 ? 1.f : term == 2 ? -1.f : 0.f;
+    }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
         uint32_t sw[4][I4 ? 4 : 2];
@@ -731,7 +746,6 @@ __device__ __forceinline__ void mv_gradient(uint32_t st, int half, const uint32_
             const uint32_t p[4] = {mv_prmt(r[0], r[1], 0x5410u), mv_prmt(r[0], r[1], 0x7632u),
                                    mv_prmt(r[2], r[3], 0x5410u), mv_prmt(r[2], r[3], 0x7632u)};
             uint32_t m[2] = {}, m2[2] = {};
-            bool high = false;
             uint32_t b[NT][2];
             if constexpr (I4) {
                 float s[4];
@@ -740,31 +754,42 @@ __device__ __forceinline__ void mv_gradient(uint32_t st, int half, const uint32_
                     s[j] = __uint_as_float(sw[j][h]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const int term = (nt * 8 + g) % T;
-                    b[nt][0] = pack_bf16(mv_term<T>(bv[nt].x * s[0], term),
-                                         mv_term<T>(bv[nt].y * s[1], term));
-                    b[nt][1] = pack_bf16(mv_term<T>(bv[nt].z * s[2], term),
-                                         mv_term<T>(bv[nt].w * s[3], term));
+                    const float v[4] = {bv[nt].x * s[0], bv[nt].y * s[1], bv[nt].z * s[2],
+                                        bv[nt].w * s[3]};
+                    float o[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if constexpr (CAREFUL) {
+                            o[j] = mv_term<T>(v[j], (nt * 8 + g) % T);
+                        } else {
+                            const float hi = trunc_bf16(v[j]), lo = v[j] - hi;
+                            o[j] = lo * pick[nt][1];
+                            if (T == 3)
+                                o[j] = fmaf(trunc_bf16(lo), pick[nt][2], o[j]);
+                            o[j] = fmaf(hi, pick[nt][0], o[j]);
+                        }
+                    }
+                    b[nt][0] = pack_bf16(o[0], o[1]);
+                    b[nt][1] = pack_bf16(o[2], o[3]);
                 }
             } else {
-                // 2^(code - 1) = 2^126 * scale as bf16 (code 0: 0), the
-                // weight's bits being 2^-126 of its value; codes above 128
-                // take 2^126 and then the scale.
-                uint32_t c[4];
-                const int k = (h & 1) * 2 + (g >> 2);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    c[j] = (sw[j][h >> 1] >> (8 * k)) & 255u;
-                    high |= c[j] > 128u;
-                }
-                high = __any_sync(0xffffffffu, high);
+                // 2^(code - 1) = 2^126 * scale as bf16, the weight's bits being
+                // 2^-126 of its value: the code's exponent field plus 126.
+                // Codes above 128 take 2^126 and then the scale, 0 is 0.
+                const uint32_t sel = ((h & 1) * 2 + (g >> 2)) * 0x11u;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const uint32_t lo = c[2 * j], hi = c[2 * j + 1];
-                    const uint32_t a0 = high ? 253u : lo ? lo + 126u : 0u;
-                    const uint32_t a1 = high ? 253u : hi ? hi + 126u : 0u;
-                    m[j] = (a0 << 7) | (a1 << 23);
-                    m2[j] = (lo << 7) | (hi << 23);
+                    // byte k of the two rows' codes in the two halfwords
+                    const uint32_t c = mv_prmt(sw[2 * j][h >> 1], sw[2 * j + 1][h >> 1],
+                                               sel | ((sel | 0x44u) << 8)) &
+                                       0x00ff00ffu;
+                    if constexpr (CAREFUL) {
+                        const uint32_t lo = c & 255u, hi = c >> 16;
+                        m[j] = (lo ? 253u << 7 : 0u) | (hi ? 253u << 23 : 0u);
+                        m2[j] = (lo << 7) | (hi << 23);
+                    } else {
+                        m[j] = c * 128u + ((126u << 7) | (126u << 23));
+                    }
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -786,12 +811,9 @@ __device__ __forceinline__ void mv_gradient(uint32_t st, int half, const uint32_
                         const uint32_t v = (mag & 0x01c001c0u) |
                                            ((p[j] << (12 - 4 * q)) & 0x80008000u);
                         a[j] = mul_bf16x2(v, m[j >> 1]);
+                        if constexpr (CAREFUL)
+                            a[j] = mul_bf16x2(a[j], m2[j >> 1]);
                     }
-                }
-                if (!I4 && high) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        a[j] = mul_bf16x2(a[j], m2[j >> 1]);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -799,6 +821,13 @@ __device__ __forceinline__ void mv_gradient(uint32_t st, int half, const uint32_
             }
         }
     }
+}
+
+// Whether a stage of MXFP4 has a scale code of 0 or above 127 (lane = row).
+__device__ __forceinline__ bool mv_odd_codes(uint32_t st, int half) {
+    const uint2 v = lds64(st + kMvRows * 128 + (threadIdx.x & 31) * 16 + half);
+    const uint32_t odd = v.x | v.y | ((v.x - 0x01010101u) & ~v.x) | ((v.y - 0x01010101u) & ~v.y);
+    return __any_sync(0xffffffffu, (odd & 0x80808080u) != 0);
 }
 
 // The gradient's partial sums share the ring's memory (no copy of the next unit
@@ -1044,8 +1073,8 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
     int turn = 0;        // the mail buffer of this unit
     __shared__ uint32_t row_max[GRAD ? 1 : 2 * RP];
     MvHeld<TX, NT> held; // gradient
-    // The first rows of a unit that has to be staged, then its weights.
-    auto begin = [&](const MvUnit &q) {
+    // The first rows of a unit that has to be staged.
+    auto fetch = [&](const MvUnit &q) {
         if (q.w && staged != q.item) {
             if constexpr (GRAD) {
                 held.load(x, ldx, q.r0, q.n, k0 * STEP, cols, pl.K, pl.x_vec);
@@ -1057,12 +1086,12 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
             }
         }
         mv_commit();
-        prologue(q);
     };
     MvUnit cur{};
     if (cluster < total) {
         cur = decode(cluster);
-        begin(cur);
+        fetch(cur);
+        prologue(cur);
     }
     for (int64_t u = cluster; u < total; u += clusters) {
         const int tasks = tasks_of(cur);
@@ -1077,82 +1106,111 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
         }
         // The gradient's one task per warp keeps its sums to the end of the
         // unit; the forward's tasks leave theirs in shared memory one by one.
-        float accg[GRAD ? 4 : 1][GRAD ? 4 : 1][NT][4] = {};
-        bool refilled = false;
-        for (int c0 = 0; c0 < nk; c0 += pl.chunk) {
-            if (cur.w && staged != cur.item) { // uniform over the CTA
-                if constexpr (GRAD) {
-                    __syncthreads(); // the last readers of x are done
-                    mv_stage_gradient<FMT, TX, NT>(mv_smem + pl.off_x, pitch, x, ldx, cur.r0, cur.n,
-                                                   (k0 + c0) * STEP, cols, pl.K, pl.x_vec, c0 == 0,
-                                                   held);
-                } else {
-                    if (c0 > 0) {
-                        __syncthreads();
-                        mv_fetch_rows<FMT, TX, NT>(mv_smem + pl.off_x, pitch, x, ldx, cur.r0, cur.n,
-                                                   (k0 + c0) * STEP, cols, pl.K, pl.x_vec);
-                        mv_commit();
-                        mv_wait<0>();
+        float accg[GRAD ? 4 : 1][GRAD ? 4 : 1][NT][4];
+        for (bool careful = false;; careful = true) {
+            bool refilled = false;
+            if constexpr (GRAD) {
+#pragma unroll
+                for (int i = 0; i < 16 * NT * 4; ++i)
+                    (&accg[0][0][0][0])[i] = 0.f;
+            }
+            for (int c0 = 0; c0 < nk; c0 += pl.chunk) {
+                if (cur.w && staged != cur.item) { // uniform over the CTA
+                    if constexpr (GRAD) {
+                        __syncthreads(); // the last readers of x are done
+                        mv_stage_gradient<FMT, TX, NT>(mv_smem + pl.off_x, pitch, x, ldx, cur.r0, cur.n,
+                                                       (k0 + c0) * STEP, cols, pl.K, pl.x_vec, c0 == 0,
+                                                       held);
                     } else {
-                        mv_wait<1>(); // all but the weights' first stage
+                        if (c0 > 0) {
+                            __syncthreads();
+                            mv_fetch_rows<FMT, TX, NT>(mv_smem + pl.off_x, pitch, x, ldx, cur.r0, cur.n,
+                                                       (k0 + c0) * STEP, cols, pl.K, pl.x_vec);
+                            mv_commit();
+                            mv_wait<0>();
+                        } else {
+                            // the first unit's rows were asked for before its
+                            // weights, the others' after
+                            if (u == cluster)
+                                mv_wait<1>();
+                            else
+                                mv_wait<0>();
+                        }
+                        __syncthreads();
+                        common = mv_stage_forward<FMT, TX, NT>(mv_smem + pl.off_x, ex, pitch, cur.n,
+                                                               cols, pl.try_common && nk <= pl.chunk,
+                                                               row_max);
                     }
                     __syncthreads();
-                    common = mv_stage_forward<FMT, TX, NT>(mv_smem + pl.off_x, ex, pitch, cur.n,
-                                                           cols, pl.try_common && nk <= pl.chunk,
-                                                           row_max);
+                    if (nk <= pl.chunk)
+                        staged = cur.item;
                 }
-                __syncthreads();
-                if (nk <= pl.chunk)
-                    staged = cur.item;
-            }
-            // The ring's other stages, now that the rows are staged: the first
-            // kept the memory system busy meanwhile, more would only have
-            // queued in front of them.
-            for (int k = refilled ? ST : 1; k < ST - 1; ++k)
-                issue();
-            refilled = true;
-            for (int task = warp; task < tasks; task += kMvWarps) {
-                const int kk = task % pl.wk, n = stages_of(c0, kk);
-                float accf[GRAD ? 1 : 2][NT][4] = {};
-                for (int i = 0; i < n; ++i) {
-                    mv_wait<ST - 2>();
-                    __syncwarp();
-                    issue(); // into the slot computed last
-                    const uint32_t st = ring + (used++ % ST) * F::STAGE;
-                    const int step = kk + i * pl.wk; // within the chunk
-                    const int colstep = GRAD ? (cur.out0 + task / pl.wk * TILE) / kMvCols
-                                             : k0 + c0 + step;
-                    const int half = F::SB == 8 ? (colstep & 1) * 8 : 0;
-                    uint32_t xat[NT];
+                // The ring's other stages, now that the rows are staged: the first
+                // kept the memory system busy meanwhile, more would only have
+                // queued in front of them.
+                for (int k = refilled ? ST : 1; k < ST - 1; ++k)
+                    issue();
+                refilled = true;
+                for (int task = warp; task < tasks; task += kMvWarps) {
+                    const int kk = task % pl.wk, n = stages_of(c0, kk);
+                    float accf[GRAD ? 1 : 2][NT][4] = {};
+                    for (int i = 0; i < n; ++i) {
+                        mv_wait<ST - 2>();
+                        __syncwarp();
+                        issue(); // into the slot computed last
+                        const uint32_t st = ring + (used++ % ST) * F::STAGE;
+                        const int step = kk + i * pl.wk; // within the chunk
+                        const int colstep = GRAD ? (cur.out0 + task / pl.wk * TILE) / kMvCols
+                                                 : k0 + c0 + step;
+                        const int half = F::SB == 8 ? (colstep & 1) * 8 : 0;
+                        uint32_t xat[NT];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        xat[nt] = xcol[nt] + step * (STEP * XB);
-                    if constexpr (GRAD)
-                        mv_gradient<FMT, TX, NT>(st, half, xat, accg);
-                    else if (common)
-                        mv_forward<FMT, TX, NT, true>(st, half, xat, ex, accf);
-                    else
-                        mv_forward<FMT, TX, NT, false>(
-                            st, half, xat, ex + step * (STEP / F::G) * RP, accf);
+                        for (int nt = 0; nt < NT; ++nt)
+                            xat[nt] = xcol[nt] + step * (STEP * XB);
+                        if constexpr (GRAD)
+                            if (careful || (FMT == MVLLM_FMT_MXFP4 && mv_odd_codes(st, half)))
+                                mv_gradient<FMT, TX, NT, true>(st, half, xat, accg);
+                            else
+                                mv_gradient<FMT, TX, NT, false>(st, half, xat, accg);
+                        else if (common)
+                            mv_forward<FMT, TX, NT, true>(st, half, xat, ex, accf);
+                        else
+                            mv_forward<FMT, TX, NT, false>(
+                                st, half, xat, ex + step * (STEP / F::G) * RP, accf);
+                    }
+                    __syncwarp();
+                    if constexpr (!GRAD)
+                        mv_put<T, RPITCH>(red + task * RSIZE, accf, common ? ex : nullptr, c0 > 0);
                 }
-                __syncwarp();
-                if constexpr (!GRAD)
-                    mv_put<T, RPITCH>(red + task * RSIZE, accf, common ? ex : nullptr, c0 > 0);
             }
+            if (!GRAD || FMT != MVLLM_FMT_INT4_G64 || careful)
+                break;
+            float nan = 0.f; // NaN where a sum is, or where infinities meet
+#pragma unroll
+            for (int i = 0; i < (GRAD ? 16 * NT * 4 : 0); ++i)
+                nan += (&accg[0][0][0][0])[i];
+            if (!__syncthreads_or(nan != nan))
+                break;
+            prologue(cur);
         }
         MvUnit next{};
         if (u + clusters < total)
             next = decode(u + clusters);
-        if constexpr (mv_alias<GRAD>()) {
+        if constexpr (GRAD) {
             mv_wait<0>();
             __syncthreads(); // the ring is done with before the sums overlay it
             if (warp < tasks)
                 mv_put_gradient<RPITCH>(red + warp * RSIZE, accg);
-        }
-        __syncthreads();
-        if constexpr (!mv_alias<GRAD>()) { // the rows' places are free now
+            __syncthreads();
+        } else {
+            // A warp that is done goes on to the next unit's weights; its rows
+            // wait until their places are free.
+            __syncwarp();
             if (u + clusters < total)
-                begin(next);
+                prologue(next);
+            __syncthreads();
+            if (u + clusters < total)
+                fetch(next);
         }
         // The CTA's own wk partial sums (and the gradient's parts) first.  With one CTA per cluster that is the
         // result; else it goes to the CTA that owns the block, and one cluster
@@ -1201,9 +1259,9 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
             __syncthreads();
         }
         cur = next;
-        if constexpr (mv_alias<GRAD>()) {
-            if (u + clusters < total)
-                begin(cur);
+        if (GRAD && u + clusters < total) {
+            fetch(cur);
+            prologue(cur);
         }
     }
 }
