@@ -27,8 +27,15 @@ struct RouteGradArgs {
     const float *router; // [E, H]
     int T, K, KK, E, H, cap, score_fn, accumulate;
     float scale;
-    float *dzp; // [cap] dz of each sorted position
+    float *dz;      // [T, K] the slots' dz
+    float *dzp;     // [cap] the sorted positions' dz
+    int *arrived;   // [E, column blocks] partial sums of an expert that are done
+    float *partial; // [row blocks][H]
 };
+
+constexpr int kRgCols = 256; // columns of a drouter item
+constexpr int kRgRows = 512; // sorted rows of a drouter item
+constexpr int kRgSmem = 200 * 1024;
 
 // dz of lane k's slot (K <= 32, one warp a token); 0 for lanes past K and ids
 // outside [0, E).
@@ -56,11 +63,15 @@ __device__ __forceinline__ float route_slot_grad(const RouteGradArgs &a, int64_t
     return dm * slope;
 }
 
-// A warp per token: dz, and its value at the sorted position of each slot
-// (slots that repeat an id add to the first one's).
-__global__ void __launch_bounds__(256) route_dz_kernel(const RouteGradArgs a) {
+// A warp per token: the slots' dz, and at the sorted position of each id their
+// sum (slots that repeat an id add to the first one's).  Clears the drouter
+// kernel's counters.
+__global__ void __launch_bounds__(256) route_dz_kernel(const RouteGradArgs a, int counters) {
     pdl_wait();
+    pdl_trigger();
     const int lane = threadIdx.x & 31;
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < counters; i += gridDim.x * blockDim.x)
+        a.arrived[i] = 0;
     const int64_t t = blockIdx.x * int64_t(blockDim.x >> 5) + (threadIdx.x >> 5);
     if (t >= a.T)
         return;
@@ -73,62 +84,295 @@ __global__ void __launch_bounds__(256) route_dz_kernel(const RouteGradArgs a) {
             sum += dk;
     }
     if (lane < a.K) {
+        a.dz[t * a.K + lane] = dz;
         const int p = a.tok_pos[t * a.KK + lane];
         if (p >= 0 && p < a.cap)
             a.dzp[p] = sum;
     }
 }
 
-// dx[t] = sum_k dz_k router[idx_k], a CTA per token.
-template <typename TO>
+// dx[t] = sum_k dz_k router[idx_k], each router row gathered from L2: a CTA
+// per token, for calls of fewer slots than experts.
+template <typename TO, int N>
 __global__ void __launch_bounds__(256)
-    route_dx_kernel(const RouteGradArgs a, TO *__restrict__ dx, int64_t lddx) {
+    route_dx_gather_kernel(const RouteGradArgs a, TO *__restrict__ dx, int64_t lddx) {
     pdl_wait();
+    pdl_trigger();
     __shared__ float sdz[32];
     __shared__ int se[32];
     const int64_t t = blockIdx.x;
     if (threadIdx.x < 32) {
-        int e;
-        sdz[threadIdx.x] = route_slot_grad(a, t, e);
-        se[threadIdx.x] = e;
+        int e = -1;
+        if (int(threadIdx.x) < a.K)
+            e = a.idx[t * a.K + threadIdx.x];
+        sdz[threadIdx.x] = e >= 0 && e < a.E ? a.dz[t * a.K + threadIdx.x] : 0.f;
+        se[threadIdx.x] = e >= a.E ? -1 : e;
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < a.H; c += blockDim.x) {
-        float acc[1] = {0.f};
+    for (int c = threadIdx.x * N; c < a.H; c += blockDim.x * N) {
+        float acc[N] = {};
         if (a.accumulate)
-            load_row<1>(dx + t * lddx + c, acc);
-        for (int k = 0; k < a.K; ++k)
-            if (se[k] >= 0)
-                acc[0] = fmaf(sdz[k], a.router[int64_t(se[k]) * a.H + c], acc[0]);
-        store_row<1>(dx + t * lddx + c, acc);
+            load_row<N>(dx + t * lddx + c, acc);
+#pragma unroll 4
+        for (int k = 0; k < a.K; ++k) {
+            if (se[k] >= 0) {
+                float v[N];
+                load_row<N>(a.router + int64_t(se[k]) * a.H + c, v);
+#pragma unroll
+                for (int q = 0; q < N; ++q)
+                    acc[q] = fmaf(sdz[k], v[q], acc[q]);
+            }
+        }
+        store_row<N>(dx + t * lddx + c, acc);
     }
 }
 
-// drouter[e] = sum over e's sorted rows of dz x[rows], a CTA per (expert,
-// columns), rows in ascending order.
-template <typename TX>
+// The same with the router's columns in shared memory.  Gathered from L2 the
+// rows are 4 T K H bytes (1.9 GB for 8192 tokens of 8 out of 384 experts, H
+// 7168), which L2 serves at about half of what shared memory does; so a CTA
+// keeps LPT * 4 columns of every expert and goes through tokens, LPT lanes
+// each.  The (column block, token) plane is cut evenly over the CTAs, column
+// blocks outermost.
+template <typename TO, int LPT>
+__global__ void __launch_bounds__(512)
+    route_dx_tile_kernel(const RouteGradArgs a, TO *__restrict__ dx, int64_t lddx, int vec) {
+    extern __shared__ __align__(16) float rg_tile[];
+    constexpr int COLS = LPT * 4, TPW = 32 / LPT; // tokens a warp has at a time
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int sub = lane / LPT, col4 = (lane % LPT) * 4;
+    const int blocks = (a.H + COLS - 1) / COLS;
+    const int64_t plane = int64_t(blocks) * a.T;
+    int64_t at = plane * blockIdx.x / gridDim.x;
+    const int64_t end = plane * (blockIdx.x + 1) / gridDim.x;
+    while (at < end) {
+        const int b = int(at / a.T), c0 = b * COLS;
+        const int t0 = int(at - int64_t(b) * a.T);
+        const int t1 = int(min(int64_t(a.T), t0 + end - at));
+        __syncthreads(); // the last block's readers are done
+        for (int i = threadIdx.x; i < a.E * LPT; i += blockDim.x) {
+            const int e = i / LPT, c = (i - e * LPT) * 4;
+            const float *src = a.router + int64_t(e) * a.H + c0 + c;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (vec && c0 + c + 4 <= a.H) {
+                v = *reinterpret_cast<const float4 *>(src);
+            } else {
+                if (c0 + c < a.H)
+                    v.x = src[0];
+                if (c0 + c + 1 < a.H)
+                    v.y = src[1];
+                if (c0 + c + 2 < a.H)
+                    v.z = src[2];
+                if (c0 + c + 3 < a.H)
+                    v.w = src[3];
+            }
+            *reinterpret_cast<float4 *>(rg_tile + e * COLS + c) = v;
+        }
+        __syncthreads();
+        for (int tb = t0 + warp * TPW; tb < t1; tb += 16 * TPW) {
+            // A token's lanes hold LPT of its slots at a time.
+            const int t = tb + sub;
+            const bool live = t < t1;
+            float acc[4] = {};
+            const int c = c0 + col4;
+            const bool whole = vec && c + 4 <= a.H;
+            if (live && a.accumulate) {
+                if (whole) {
+                    load_row<4>(dx + t * lddx + c, acc);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float o[1] = {0.f};
+                        if (c + q < a.H)
+                            load_row<1>(dx + t * lddx + c + q, o);
+                        acc[q] = o[0];
+                    }
+                }
+            }
+            for (int k0 = 0; k0 < a.K; k0 += LPT) {
+                const int k = k0 + lane % LPT;
+                int e = -1;
+                float dz = 0.f;
+                if (live && k < a.K) {
+                    e = a.idx[int64_t(t) * a.K + k];
+                    dz = a.dz[int64_t(t) * a.K + k];
+                    if (e >= a.E)
+                        e = -1;
+                }
+                const int n = min(LPT, a.K - k0);
+#pragma unroll 8
+                for (int j = 0; j < n; ++j) {
+                    const int ej = __shfl_sync(0xffffffffu, e, j, LPT);
+                    const float dj = __shfl_sync(0xffffffffu, dz, j, LPT);
+                    if (ej >= 0) {
+                        const float4 v =
+                            *reinterpret_cast<const float4 *>(rg_tile + ej * COLS + col4);
+                        acc[0] = fmaf(dj, v.x, acc[0]), acc[1] = fmaf(dj, v.y, acc[1]);
+                        acc[2] = fmaf(dj, v.z, acc[2]), acc[3] = fmaf(dj, v.w, acc[3]);
+                    }
+                }
+            }
+            if (live) {
+                if (whole) {
+                    store_row<4>(dx + t * lddx + c, acc);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float o[1] = {acc[q]};
+                        if (c + q < a.H)
+                            store_row<1>(dx + t * lddx + c + q, o);
+                    }
+                }
+            }
+        }
+        at += t1 - t0;
+    }
+}
+
+// drouter[e] = sum over e's sorted rows of dz x[rows].  An item is (kRgCols
+// columns, an expert, kRgRows of its rows): the CTA's warps take its rows in
+// turn, eight loads under way in each, and meet in shared memory.  Items run
+// column block by column block, so the columns of x that all experts gather
+// from (2 T kRgCols bytes) stay in L2.  An expert of several items leaves its
+// partial sums in the workspace, and the item that arrives last adds them in
+// order; one without rows gets zeros.
+template <typename TX, int N>
 __global__ void __launch_bounds__(256)
     route_dw_kernel(const RouteGradArgs a, const TX *__restrict__ x, int64_t ldx,
                     const int *__restrict__ nr, const int *__restrict__ xoff,
                     const int *__restrict__ rows, float *__restrict__ drouter) {
+    constexpr int LANES = kRgCols / N >= 32 ? 32 : kRgCols / N; // lanes of a row
+    constexpr int PIECES = kRgCols / (LANES * N);               // vectors of a lane
+    __shared__ int first[1025]; // row blocks before each expert
+    __shared__ int wsum[8];
+    __shared__ float part[8][kRgCols];
+    __shared__ int last;
     pdl_wait();
-    const int e = blockIdx.x, c = blockIdx.y * blockDim.x + threadIdx.x;
-    if (c >= a.H)
-        return;
-    const int n = nr[e], off = xoff[e];
-    float acc = a.accumulate ? drouter[int64_t(e) * a.H + c] : 0.f;
-    for (int i = 0; i < n; ++i) {
-        const int p = off + i;
-        if (p < 0 || p >= a.cap)
-            break;
-        const int t = rows[p];
-        if (t < 0 || t >= a.T)
-            continue;
-        float v[1];
-        load_row<1>(x + t * ldx + c, v);
-        acc = fmaf(a.dzp[p], v[0], acc);
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // Prefix sums of the experts' row blocks, four experts a thread.
+    int n4[4], v = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int e = 4 * int(threadIdx.x) + k;
+        n4[k] = e < a.E ? max(1, (min(nr[e], a.cap) + kRgRows - 1) / kRgRows) : 0;
+        v += n4[k];
     }
-    drouter[int64_t(e) * a.H + c] = acc;
+    int before = -v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        v += lane >= o ? u : 0;
+    }
+    if (lane == 31)
+        wsum[warp] = v;
+    __syncthreads();
+    before += v;
+    for (int k = 0; k < warp; ++k)
+        before += wsum[k];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int e = 4 * int(threadIdx.x) + k;
+        if (e < a.E)
+            first[e] = before;
+        before += n4[k];
+        if (e == a.E - 1)
+            first[a.E] = before;
+    }
+    __syncthreads();
+    // (No more than the workspace holds, whatever nr says.)
+    const int blocks = min(first[a.E], a.cap / kRgRows + a.E);
+    const int ncol = (a.H + kRgCols - 1) / kRgCols;
+    for (int64_t it = blockIdx.x; it < int64_t(blocks) * ncol; it += gridDim.x) {
+        const int cb = int(it / blocks), slot = int(it - int64_t(cb) * blocks);
+        int lo = 0, hi = a.E; // the last expert with first[e] <= slot
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first[mid] <= slot)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        const int e = lo, rb = slot - first[e], nblk = first[e + 1] - first[e];
+        const int off = xoff[e], n = min(nr[e], a.cap);
+        const int p0 = off + rb * kRgRows, p1 = min(off + n, p0 + kRgRows);
+        const int c0 = cb * kRgCols;
+        float acc[PIECES][N] = {};
+        // A warp's 32 rows at a time: their tokens and dz by lane.
+        for (int pb = p0 + warp * 32; pb < p1; pb += 8 * 32) {
+            const int p = pb + lane;
+            int t = -1;
+            float dz = 0.f;
+            if (p >= 0 && p < p1 && p < a.cap) {
+                t = rows[p];
+                dz = a.dzp[p];
+                if (t < 0 || t >= a.T)
+                    t = -1;
+            }
+            const int cnt = min(32, p1 - pb);
+#pragma unroll 1
+            for (int j0 = 0; j0 < cnt; j0 += 8) {
+                float xv[8][PIECES][N];
+                float dj[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int tj = __shfl_sync(0xffffffffu, t, j0 + j);
+                    dj[j] = __shfl_sync(0xffffffffu, dz, j0 + j);
+#pragma unroll
+                    for (int q = 0; q < PIECES; ++q) {
+                        const int c = c0 + (q * LANES + lane) * N;
+#pragma unroll
+                        for (int s = 0; s < N; ++s)
+                            xv[j][q][s] = 0.f;
+                        if (tj >= 0 && c < a.H)
+                            load_row<N>(x + tj * ldx + c, xv[j][q]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int q = 0; q < PIECES; ++q)
+#pragma unroll
+                        for (int s = 0; s < N; ++s)
+                            acc[q][s] = fmaf(dj[j], xv[j][q][s], acc[q][s]);
+            }
+        }
+        __syncthreads(); // part of the last item is read
+#pragma unroll
+        for (int q = 0; q < PIECES; ++q)
+#pragma unroll
+            for (int s = 0; s < N; ++s)
+                part[warp][(q * LANES + lane) * N + s] = acc[q][s];
+        __syncthreads();
+        const int c = c0 + threadIdx.x; // 256 threads, kRgCols columns
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+            sum += part[w][threadIdx.x];
+        float *out = drouter + int64_t(e) * a.H + c;
+        if (nblk == 1) {
+            if (c < a.H)
+                *out = a.accumulate ? *out + sum : sum;
+            continue;
+        }
+        if (c < a.H)
+            a.partial[int64_t(slot) * a.H + c] = sum;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0)
+            last = atomicAdd(&a.arrived[e * ncol + cb], 1) == nblk - 1;
+        __syncthreads();
+        if (last) {
+            __threadfence();
+            if (c < a.H) {
+                float s = a.accumulate ? *out : 0.f;
+                for (int k = 0; k < nblk; ++k)
+                    s += __ldcg(a.partial + int64_t(first[e] + k) * a.H + c);
+                *out = s;
+            }
+        }
+    }
 }
 
 } // namespace mvb

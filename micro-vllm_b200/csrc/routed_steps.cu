@@ -206,10 +206,78 @@ int mvllm_moe_combine_grad_dev(void *stream, const void *dout, int dout_dtype, i
                                KK, D, static_cast<bf *>(dy), lddy, dwt);
 }
 
+} // extern "C"
+
+namespace {
+
+template <typename TO>
+int route_dx(cudaStream_t st, const RouteGradArgs &a, int sms, TO *dx, int64_t lddx) {
+    const int type = sizeof(TO) == 4 ? MVLLM_DTYPE_F32 : MVLLM_DTYPE_BF16;
+    const bool vec = std::min(row_align(a.router, a.H, a.H, MVLLM_DTYPE_F32), 16u) == 16 &&
+                     row_align(dx, lddx, a.H, type) >= 4 * sizeof(TO);
+    // Fewer slots than experts: loading every expert's columns once costs more
+    // than gathering the slots' rows.
+    if (int64_t(a.T) * a.K < 2 * a.E) {
+        if (vec)
+            MVB_TRY(launch_serial(route_dx_gather_kernel<TO, 4>, dim3(a.T), dim3(256), 0, st, a, dx,
+                                  lddx));
+        else
+            MVB_TRY(launch_serial(route_dx_gather_kernel<TO, 1>, dim3(a.T), dim3(256), 0, st, a, dx,
+                                  lddx));
+        return MVLLM_OK;
+    }
+    // The widest column block whose experts fit shared memory.
+    const int lpt = a.E * 512 <= kRgSmem ? 32 : a.E * 256 <= kRgSmem ? 16 : 8;
+    const int smem = a.E * lpt * 16;
+    const int64_t work = int64_t((a.H + 4 * lpt - 1) / (4 * lpt)) * a.T;
+    const int per_sm = std::max(1, std::min(4, kRgSmem / std::max(smem, 1)));
+    const unsigned grid = unsigned(std::min<int64_t>(int64_t(sms) * per_sm, (work + 15) / 16));
+#define MVB_DX(L)                                                                              \
+    do {                                                                                       \
+        MVB_TRY(cudaFuncSetAttribute(route_dx_tile_kernel<TO, L>,                              \
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, kRgSmem));   \
+        MVB_TRY(launch_serial(route_dx_tile_kernel<TO, L>, dim3(grid), dim3(512), smem, st, a, \
+                              dx, lddx, int(vec)));                                            \
+    } while (0)
+    if (lpt == 32)
+        MVB_DX(32);
+    else if (lpt == 16)
+        MVB_DX(16);
+    else
+        MVB_DX(8);
+#undef MVB_DX
+    return MVLLM_OK;
+}
+
+template <typename TX>
+int route_dw(cudaStream_t st, const RouteGradArgs &a, int sms, const TX *x, int64_t ldx,
+             const int *nr, const int *xoff, const int *rows, float *drouter) {
+    const int type = sizeof(TX) == 4 ? MVLLM_DTYPE_F32 : MVLLM_DTYPE_BF16;
+    const int64_t ncol = (a.H + kRgCols - 1) / kRgCols;
+    const int64_t most = (int64_t(a.cap) / kRgRows + a.E) * ncol;
+    const unsigned grid = unsigned(std::min<int64_t>(int64_t(sms) * 4, most));
+    const unsigned al = row_align(x, ldx, a.H, type);
+#define MVB_DW(N)                                                                              \
+    MVB_TRY(launch_serial(route_dw_kernel<TX, N>, dim3(grid), dim3(256), 0, st, a, x, ldx, nr, \
+                          xoff, rows, drouter))
+    if (al >= 16)
+        MVB_DW(16 / int(sizeof(TX)));
+    else
+        MVB_DW(1);
+#undef MVB_DW
+    return MVLLM_OK;
+}
+
+} // namespace
+
+extern "C" {
+
 size_t mvllm_moe_route_grad_workspace(int T, int H, int E, int K) {
     if (T < 0 || H < 1 || E < 1 || K < 1)
         return 0;
-    return (size_t(T) * K + 64) * sizeof(float) + 256;
+    const size_t slots = size_t(T) * K, ncol = (size_t(H) + kRgCols - 1) / kRgCols;
+    // dz by slot and by position, counters, partial sums of each row block
+    return (2 * slots + E * ncol + (slots / kRgRows + E) * H) * sizeof(float) + 4 * 256;
 }
 
 int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t ldx, int T, int H,
@@ -237,27 +305,37 @@ int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t l
     a.idx = idx, a.scores = scores, a.dwt = dwt, a.tok_pos = tok_pos, a.router = router;
     a.T = T, a.K = K, a.KK = KK, a.E = E, a.H = H, a.cap = T * K;
     a.score_fn = score_fn, a.accumulate = accumulate, a.scale = routed_scale;
-    a.dzp = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(workspace) + 255) &
-                                      ~uintptr_t(255));
-    using bf = __nv_bfloat16;
-    if (T > 0 && drouter)
-        MVB_TRY(launch_serial(route_dz_kernel, dim3((T + 7) / 8), dim3(256), 0, st, a));
+    const size_t slots = size_t(T) * K;
+    const int ncol = (H + kRgCols - 1) / kRgCols;
+    uintptr_t at = reinterpret_cast<uintptr_t>(workspace);
+    auto take = [&](size_t n) {
+        at = (at + 255) & ~uintptr_t(255);
+        float *p = reinterpret_cast<float *>(at);
+        at += n * sizeof(float);
+        return p;
+    };
+    a.dz = take(slots);
+    a.dzp = take(slots);
+    a.arrived = reinterpret_cast<int *>(take(size_t(E) * ncol));
+    a.partial = take((slots / kRgRows + E) * H);
+    const int counters = drouter ? E * ncol : 0;
+    const int warps = std::max(T, (counters + 31) / 32);
+    MVB_TRY(launch_serial(route_dz_kernel, dim3((warps + 7) / 8), dim3(256), 0, st, a, counters));
     if (T > 0 && dx) {
-        if (dx_dtype == MVLLM_DTYPE_F32)
-            MVB_TRY(launch_serial(route_dx_kernel<float>, dim3(T), dim3(256), 0, st, a,
-                                  static_cast<float *>(dx), lddx));
-        else
-            MVB_TRY(launch_serial(route_dx_kernel<bf>, dim3(T), dim3(256), 0, st, a,
-                                  static_cast<bf *>(dx), lddx));
+        const int rc = dx_dtype == MVLLM_DTYPE_F32
+                           ? route_dx(st, a, dev.sms, static_cast<float *>(dx), lddx)
+                           : route_dx(st, a, dev.sms, static_cast<__nv_bfloat16 *>(dx), lddx);
+        if (rc)
+            return rc;
     }
     if (drouter) {
-        const dim3 grid(E, (H + 255) / 256);
-        if (x_dtype == MVLLM_DTYPE_F32)
-            MVB_TRY(launch_serial(route_dw_kernel<float>, grid, dim3(256), 0, st, a,
-                                  static_cast<const float *>(x), ldx, nr, xoff, rows, drouter));
-        else
-            MVB_TRY(launch_serial(route_dw_kernel<bf>, grid, dim3(256), 0, st, a,
-                                  static_cast<const bf *>(x), ldx, nr, xoff, rows, drouter));
+        const int rc =
+            x_dtype == MVLLM_DTYPE_F32
+                ? route_dw(st, a, dev.sms, static_cast<const float *>(x), ldx, nr, xoff, rows, drouter)
+                : route_dw(st, a, dev.sms, static_cast<const __nv_bfloat16 *>(x), ldx, nr, xoff,
+                           rows, drouter);
+        if (rc)
+            return rc;
     }
     return MVLLM_OK;
 }
