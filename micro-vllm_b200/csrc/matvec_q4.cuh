@@ -268,52 +268,6 @@ template <int FMT, bool GRAD> struct MvWalk {
     }
 };
 
-// 8 elements of a row, as loaded; 0 past K.
-template <typename TX> struct MvRaw {
-    uint4 u[sizeof(TX) / 2];
-    __device__ __forceinline__ void load(const TX *row, int c, int K, bool vec) {
-        if (vec && c + 8 <= K) {
-#pragma unroll
-            for (int q = 0; q < int(sizeof(TX)) / 2; ++q) // stays where it is written
-                asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];"
-                             : "=r"(u[q].x), "=r"(u[q].y), "=r"(u[q].z), "=r"(u[q].w)
-                             : "l"(reinterpret_cast<const uint4 *>(row + c) + q)
-                             : "memory");
-        } else {
-            uint32_t w[sizeof(TX) * 2];
-#pragma unroll
-            for (int q = 0; q < int(sizeof(TX)) * 2; ++q) {
-                w[q] = 0;
-                if constexpr (sizeof(TX) == 4) {
-                    if (c + q < K)
-                        w[q] = __float_as_uint(row[c + q]);
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-                        if (c + 2 * q + b < K)
-                            w[q] |= uint32_t(__bfloat16_as_ushort(row[c + 2 * q + b])) << (16 * b);
-                }
-            }
-#pragma unroll
-            for (int q = 0; q < int(sizeof(TX)) / 2; ++q)
-                u[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
-        }
-    }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        const uint4 a = u[0];
-        if constexpr (sizeof(TX) == 4) {
-            const uint4 b = u[1];
-            v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y);
-            v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
-            v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y);
-            v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
-        } else {
-            v[0] = bf16_lo(a.x), v[1] = bf16_hi(a.x), v[2] = bf16_lo(a.y), v[3] = bf16_hi(a.y);
-            v[4] = bf16_lo(a.z), v[5] = bf16_hi(a.z), v[6] = bf16_lo(a.w), v[7] = bf16_hi(a.w);
-        }
-    }
-};
-
 // Walks the groups of 8 elements of the rows to stage: group `tid` first, then
 // every THREADS-th, as (row, group of the row).
 template <int THREADS> struct MvGroups {
@@ -337,7 +291,7 @@ template <int THREADS> struct MvGroups {
 template <typename TX, int NT> struct MvHeld {
     static constexpr int THREADS = 32 * mv_warps<NT, true>();
     static constexpr int HOLD = sizeof(TX) == 4 ? 4 : 8;
-    MvRaw<TX> raw[HOLD];
+    Raw8<TX> raw[HOLD];
     __device__ __forceinline__ void load(const TX *x, int64_t ldx, int r0, int n, int c0, int cols,
                                          int K, bool vec) {
         MvGroups<THREADS> at(cols / 8);
@@ -354,14 +308,14 @@ template <typename TX, int NT> struct MvHeld {
 #pragma unroll
         for (int h = 0; h < HOLD; ++h, at.next()) {
             if (at.r < n) {
-                MvRaw<TX> now = raw[h];
+                Raw8<TX> now = raw[h];
                 if (!have)
                     now.load(x + int64_t(r0 + at.r) * ldx, c0 + at.q * 8, K, vec);
                 f(now, at.r, at.q);
             }
         }
         for (; at.r < n; at.next()) {
-            MvRaw<TX> now;
+            Raw8<TX> now;
             now.load(x + int64_t(r0 + at.r) * ldx, c0 + at.q * 8, K, vec);
             f(now, at.r, at.q);
         }
@@ -441,7 +395,7 @@ __device__ __forceinline__ void mv_fetch_rows(uint8_t *xs, int pitch, const TX *
                 cp_async16_at(smem_u32(to + term * pitch),
                               reinterpret_cast<const uint4 *>(row + c) + term);
         } else {
-            MvRaw<TX> raw;
+            Raw8<TX> raw;
             raw.load(row, c, K, vec);
 #pragma unroll
             for (int term = 0; term < T; ++term)
@@ -457,7 +411,7 @@ __device__ __forceinline__ bool mv_stage_forward(uint8_t *xs, float *ex, int pit
     using Groups = MvGroups<32 * mv_warps<NT, false>()>;
     const int lane = threadIdx.x & 31;
     auto read = [&](const Groups &at, float(&v)[8]) {
-        MvRaw<TX> raw;
+        Raw8<TX> raw;
 #pragma unroll
         for (int term = 0; term < T; ++term)
             raw.u[term] =
@@ -540,7 +494,7 @@ __device__ __forceinline__ void mv_stage_gradient(uint8_t *xs, int pitch, const 
                                                   bool have, const MvHeld<TX, NT> &held) {
     constexpr int T = MvTerms<FMT, TX, true>::T;
     constexpr bool I4 = FMT == MVLLM_FMT_INT4_G64;
-    held.each(x, ldx, r0, n, c0, cols, K, vec, have, [&](const MvRaw<TX> &raw, int r, int q) {
+    held.each(x, ldx, r0, n, c0, cols, K, vec, have, [&](const Raw8<TX> &raw, int r, int q) {
         float v[8];
         raw.get(v);
 #pragma unroll

@@ -34,7 +34,7 @@ struct RouteGradArgs {
 };
 
 constexpr int kRgCols = 256; // columns of a drouter item
-constexpr int kRgRows = 512; // sorted rows of a drouter item
+constexpr int kRgRows = 128; // sorted rows of a drouter item
 constexpr int kRgSmem = 200 * 1024;
 
 // dz of lane k's slot (K <= 32, one warp a token); 0 for lanes past K and ids
@@ -170,58 +170,76 @@ __global__ void __launch_bounds__(512)
             *reinterpret_cast<float4 *>(rg_tile + e * COLS + c) = v;
         }
         __syncthreads();
-        for (int tb = t0 + warp * TPW; tb < t1; tb += 16 * TPW) {
-            // A token's lanes hold LPT of its slots at a time.
-            const int t = tb + sub;
-            const bool live = t < t1;
-            float acc[4] = {};
-            const int c = c0 + col4;
-            const bool whole = vec && c + 4 <= a.H;
-            if (live && a.accumulate) {
-                if (whole) {
-                    load_row<4>(dx + t * lddx + c, acc);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        float o[1] = {0.f};
-                        if (c + q < a.H)
-                            load_row<1>(dx + t * lddx + c + q, o);
-                        acc[q] = o[0];
-                    }
-                }
+        // A group of LPT lanes takes BT tokens at a time, their slots' ids and dz
+        // by lane, the next batch's loaded before this one is worked off.
+        const int bt = max(1, LPT / a.K), lk = lane % LPT;
+        const int stride = 16 * TPW * bt;
+        auto fetch = [&](int t, int k0, int &e, float &dz) { // slots k0.. of tokens t..
+            e = -1, dz = 0.f;
+            const int tt = t + (a.K <= LPT ? lk / a.K : 0), k = a.K <= LPT ? lk % a.K : k0 + lk;
+            if (tt < min(t1, t + bt) && k < a.K) {
+                e = a.idx[int64_t(tt) * a.K + k];
+                dz = a.dz[int64_t(tt) * a.K + k];
+                if (e >= a.E)
+                    e = -1;
             }
-            for (int k0 = 0; k0 < a.K; k0 += LPT) {
-                const int k = k0 + lane % LPT;
-                int e = -1;
-                float dz = 0.f;
-                if (live && k < a.K) {
-                    e = a.idx[int64_t(t) * a.K + k];
-                    dz = a.dz[int64_t(t) * a.K + k];
-                    if (e >= a.E)
-                        e = -1;
-                }
-                const int n = min(LPT, a.K - k0);
+        };
+        const int c = c0 + col4;
+        const bool whole = vec && c + 4 <= a.H;
+        auto old = [&](int64_t t, float (&acc)[4]) {
+            if (whole) {
+                load_row<4>(dx + t * lddx + c, acc);
+                return;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float o[1] = {0.f};
+                if (c + q < a.H)
+                    load_row<1>(dx + t * lddx + c + q, o);
+                acc[q] = o[0];
+            }
+        };
+        int tb = t0 + (warp * TPW + sub) * bt;
+        int e_next;
+        float dz_next;
+        fetch(tb, 0, e_next, dz_next);
+        const int rounds = (t1 - t0 + stride - 1) / stride; // the same for every lane
+        for (int i = 0; i < rounds; ++i, tb += stride) {
+            int e = e_next;
+            float dz = dz_next;
+            fetch(tb + stride, 0, e_next, dz_next);
+            for (int s = 0; s < bt; ++s) {
+                const int t = tb + s;
+                const bool live = t < t1;
+                float acc[4] = {};
+                if (live && a.accumulate)
+                    old(t, acc);
+                for (int k0 = 0; k0 < a.K; k0 += LPT) {
+                    if (k0 > 0) // more slots than lanes: bt is 1
+                        fetch(tb, k0, e, dz);
+                    const int n = min(LPT, a.K - k0);
 #pragma unroll 8
-                for (int j = 0; j < n; ++j) {
-                    const int ej = __shfl_sync(0xffffffffu, e, j, LPT);
-                    const float dj = __shfl_sync(0xffffffffu, dz, j, LPT);
-                    if (ej >= 0) {
-                        const float4 v =
-                            *reinterpret_cast<const float4 *>(rg_tile + ej * COLS + col4);
-                        acc[0] = fmaf(dj, v.x, acc[0]), acc[1] = fmaf(dj, v.y, acc[1]);
-                        acc[2] = fmaf(dj, v.z, acc[2]), acc[3] = fmaf(dj, v.w, acc[3]);
+                    for (int j = 0; j < n; ++j) {
+                        const int ej = __shfl_sync(0xffffffffu, e, s * a.K + j, LPT);
+                        const float dj = __shfl_sync(0xffffffffu, dz, s * a.K + j, LPT);
+                        if (ej >= 0) {
+                            const float4 v =
+                                *reinterpret_cast<const float4 *>(rg_tile + ej * COLS + col4);
+                            acc[0] = fmaf(dj, v.x, acc[0]), acc[1] = fmaf(dj, v.y, acc[1]);
+                            acc[2] = fmaf(dj, v.z, acc[2]), acc[3] = fmaf(dj, v.w, acc[3]);
+                        }
                     }
                 }
-            }
-            if (live) {
-                if (whole) {
-                    store_row<4>(dx + t * lddx + c, acc);
-                } else {
+                if (live) {
+                    if (whole) {
+                        store_row<4>(dx + t * lddx + c, acc);
+                    } else {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float o[1] = {acc[q]};
-                        if (c + q < a.H)
-                            store_row<1>(dx + t * lddx + c + q, o);
+                        for (int q = 0; q < 4; ++q) {
+                            const float o[1] = {acc[q]};
+                            if (c + q < a.H)
+                                store_row<1>(dx + t * lddx + c + q, o);
+                        }
                     }
                 }
             }
@@ -230,24 +248,22 @@ __global__ void __launch_bounds__(512)
     }
 }
 
-// drouter[e] = sum over e's sorted rows of dz x[rows].  An item is (kRgCols
-// columns, an expert, kRgRows of its rows): the CTA's warps take its rows in
-// turn, eight loads under way in each, and meet in shared memory.  Items run
-// column block by column block, so the columns of x that all experts gather
-// from (2 T kRgCols bytes) stay in L2.  An expert of several items leaves its
-// partial sums in the workspace, and the item that arrives last adds them in
-// order; one without rows gets zeros.
-template <typename TX, int N>
+// drouter[e] = sum over e's sorted rows of dz x[rows].  An item is (eight
+// blocks of kRgCols columns, an expert, kRgRows of its rows), a column block
+// for each of the CTA's warps, which go on without meeting; a warp has eight
+// (f32: four) rows' loads under way.  Items run column group by column group,
+// so the columns of x that all experts gather from (16 T kRgCols bytes in
+// bf16) stay in L2.  An expert of several items leaves its partial sums in the
+// workspace, and the warp that arrives last adds them in order; one without
+// rows gets zeros.
+template <typename TX>
 __global__ void __launch_bounds__(256)
-    route_dw_kernel(const RouteGradArgs a, const TX *__restrict__ x, int64_t ldx,
+    route_dw_kernel(const RouteGradArgs a, const TX *__restrict__ x, int64_t ldx, int vec,
                     const int *__restrict__ nr, const int *__restrict__ xoff,
                     const int *__restrict__ rows, float *__restrict__ drouter) {
-    constexpr int LANES = kRgCols / N >= 32 ? 32 : kRgCols / N; // lanes of a row
-    constexpr int PIECES = kRgCols / (LANES * N);               // vectors of a lane
+    constexpr int B = sizeof(TX) == 4 ? 4 : 8;
     __shared__ int first[1025]; // row blocks before each expert
     __shared__ int wsum[8];
-    __shared__ float part[8][kRgCols];
-    __shared__ int last;
     pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -283,9 +299,12 @@ __global__ void __launch_bounds__(256)
     __syncthreads();
     // (No more than the workspace holds, whatever nr says.)
     const int blocks = min(first[a.E], a.cap / kRgRows + a.E);
-    const int ncol = (a.H + kRgCols - 1) / kRgCols;
-    for (int64_t it = blockIdx.x; it < int64_t(blocks) * ncol; it += gridDim.x) {
-        const int cb = int(it / blocks), slot = int(it - int64_t(cb) * blocks);
+    const int ncol = (a.H + kRgCols - 1) / kRgCols, groups = (ncol + 7) / 8;
+    for (int64_t it = blockIdx.x; it < int64_t(blocks) * groups; it += gridDim.x) {
+        const int cg = int(it / blocks), slot = int(it - int64_t(cg) * blocks);
+        const int cb = cg * 8 + warp;
+        if (cb >= ncol)
+            continue; // uniform over the warp; warps do not meet here
         int lo = 0, hi = a.E; // the last expert with first[e] <= slot
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -296,82 +315,98 @@ __global__ void __launch_bounds__(256)
         }
         const int e = lo, rb = slot - first[e], nblk = first[e + 1] - first[e];
         const int off = xoff[e], n = min(nr[e], a.cap);
-        const int p0 = off + rb * kRgRows, p1 = min(off + n, p0 + kRgRows);
-        const int c0 = cb * kRgCols;
-        float acc[PIECES][N] = {};
-        // A warp's 32 rows at a time: their tokens and dz by lane.
-        for (int pb = p0 + warp * 32; pb < p1; pb += 8 * 32) {
+        const int p0 = off + rb * kRgRows, p1 = min(min(off + n, p0 + kRgRows), a.cap);
+        const int c = cb * kRgCols + lane * 8;
+        float acc[8] = {};
+        // 32 rows at a time, their tokens and dz by lane; rows that do not
+        // count are row 0 with dz 0, and not added
+        auto slots = [&](int pb, int &t, float &dz) {
             const int p = pb + lane;
-            int t = -1;
-            float dz = 0.f;
-            if (p >= 0 && p < p1 && p < a.cap) {
+            t = -1, dz = 0.f;
+            if (p >= 0 && p < p1) {
                 t = rows[p];
                 dz = a.dzp[p];
                 if (t < 0 || t >= a.T)
                     t = -1;
             }
+        };
+        int t_next;
+        float dz_next;
+        slots(p0, t_next, dz_next);
+        for (int pb = p0; pb < p1; pb += 32) {
+            const int t = t_next;
+            const float dz = dz_next;
+            slots(pb + 32, t_next, dz_next);
             const int cnt = min(32, p1 - pb);
-#pragma unroll 1
-            for (int j0 = 0; j0 < cnt; j0 += 8) {
-                float xv[8][PIECES][N];
-                float dj[8];
+            for (int j0 = 0; j0 < cnt; j0 += B) {
+                Raw8<TX> xv[B];
+                int tj[B];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int tj = __shfl_sync(0xffffffffu, t, j0 + j);
-                    dj[j] = __shfl_sync(0xffffffffu, dz, j0 + j);
-#pragma unroll
-                    for (int q = 0; q < PIECES; ++q) {
-                        const int c = c0 + (q * LANES + lane) * N;
-#pragma unroll
-                        for (int s = 0; s < N; ++s)
-                            xv[j][q][s] = 0.f;
-                        if (tj >= 0 && c < a.H)
-                            load_row<N>(x + tj * ldx + c, xv[j][q]);
-                    }
+                for (int j = 0; j < B; ++j) {
+                    tj[j] = __shfl_sync(0xffffffffu, t, j0 + j);
+                    if (tj[j] >= 0 && c < a.H)
+                        xv[j].load(x + tj[j] * ldx, c, a.H, vec);
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < B; ++j) {
+                    const float dj = __shfl_sync(0xffffffffu, dz, j0 + j);
+                    if (tj[j] >= 0) {
+                        float f[8];
+                        xv[j].get(f);
 #pragma unroll
-                    for (int q = 0; q < PIECES; ++q)
-#pragma unroll
-                        for (int s = 0; s < N; ++s)
-                            acc[q][s] = fmaf(dj[j], xv[j][q][s], acc[q][s]);
+                        for (int s = 0; s < 8; ++s)
+                            acc[s] = fmaf(dj, f[s], acc[s]);
+                    }
+                }
             }
         }
-        __syncthreads(); // part of the last item is read
-#pragma unroll
-        for (int q = 0; q < PIECES; ++q)
-#pragma unroll
-            for (int s = 0; s < N; ++s)
-                part[warp][(q * LANES + lane) * N + s] = acc[q][s];
-        __syncthreads();
-        const int c = c0 + threadIdx.x; // 256 threads, kRgCols columns
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w)
-            sum += part[w][threadIdx.x];
         float *out = drouter + int64_t(e) * a.H + c;
-        if (nblk == 1) {
-            if (c < a.H)
-                *out = a.accumulate ? *out + sum : sum;
-            continue;
-        }
-        if (c < a.H)
-            a.partial[int64_t(slot) * a.H + c] = sum;
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0)
-            last = atomicAdd(&a.arrived[e * ncol + cb], 1) == nblk - 1;
-        __syncthreads();
-        if (last) {
+        const bool whole = (a.H & 3) == 0 && (reinterpret_cast<uintptr_t>(drouter) & 15u) == 0;
+        auto put = [&](float *to, const float (&f)[8]) {
+            if (whole && c + 8 <= a.H) {
+                store_row<8>(to, f);
+                return;
+            }
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                if (c + s < a.H)
+                    to[s] = f[s];
+        };
+        float base[8] = {};
+        if (nblk > 1) {
+            float *mine = a.partial + int64_t(slot) * a.H + c;
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                if (c + s < a.H)
+                    mine[s] = acc[s];
             __threadfence();
-            if (c < a.H) {
-                float s = a.accumulate ? *out : 0.f;
-                for (int k = 0; k < nblk; ++k)
-                    s += __ldcg(a.partial + int64_t(first[e] + k) * a.H + c);
-                *out = s;
+            __syncwarp();
+            int arrived = 0;
+            if (lane == 0)
+                arrived = atomicAdd(&a.arrived[e * ncol + cb], 1);
+            if (__shfl_sync(0xffffffffu, arrived, 0) != nblk - 1)
+                continue;
+            __threadfence();
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                acc[s] = 0.f;
+            for (int k = 0; k < nblk; ++k) {
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                    if (c + s < a.H)
+                        acc[s] += __ldcg(a.partial + int64_t(first[e] + k) * a.H + c + s);
             }
         }
+        if (a.accumulate) {
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                if (c + s < a.H)
+                    base[s] = out[s];
+        }
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+            acc[s] += base[s];
+        put(out, acc);
     }
 }
 

@@ -28,6 +28,19 @@ int row_vec(unsigned align, size_t bytes) {
 
 constexpr int64_t kMaxGrid = 0x7fffffff;
 
+// Segments of a row of `words` lane-words for T tokens: as few as fill the
+// device with warps (32 per SM), each a multiple of `piece` words.
+struct Segments {
+    int n, words;
+    Segments(int T, int total, int piece, int sms) {
+        const int most = (total + piece - 1) / piece;
+        const int64_t want = (int64_t(sms) * 32 + T - 1) / T;
+        n = int(std::max<int64_t>(1, std::min<int64_t>(most, want)));
+        words = (most + n - 1) / n * piece;
+        n = (total + words - 1) / words;
+    }
+};
+
 } // namespace
 
 extern "C" {
@@ -46,15 +59,15 @@ int mvllm_moe_dispatch_dev(void *stream, const void *x, int dtype, int64_t ldx,
     const unsigned al = std::min(row_align(x, ldx, D, dtype), row_align(xs, ldxs, D, dtype));
     const int64_t b = dtype_bytes(dtype), w = al >= 16 ? 16 : al >= 4 ? 4 : 2;
     const int words = int(D * b / w);
-    const int seg = std::max(32, words), nseg = 1;
-    const int64_t units = int64_t(T) * nseg, grid = (units + 7) / 8;
+    const Segments s(T, words, 32, dev.sms);
+    const int64_t units = int64_t(T) * s.n, grid = (units + 7) / 8;
     if (grid > kMaxGrid)
         return host_fail(MVLLM_ERR_INVALID, "dispatch_dev: T too large");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define MVB_DISPATCH(W)                                                                        \
     MVB_TRY(launch_serial(dispatch_rows_kernel<W>, dim3(unsigned(grid)), dim3(256), 0, st,     \
-                          static_cast<const W *>(x), ldx *b / w, tok_pos, units, nseg, seg,    \
-                          KK, words, static_cast<W *>(xs), ldxs *b / w, rows_cap))
+                          static_cast<const W *>(x), ldx *b / w, tok_pos, units, s.n,          \
+                          s.words, KK, words, static_cast<W *>(xs), ldxs *b / w, rows_cap))
     if (w == 16)
         MVB_DISPATCH(uint4);
     else if (w == 4)
@@ -70,17 +83,17 @@ int mvllm_moe_dispatch_dev(void *stream, const void *x, int dtype, int64_t ldx,
 namespace {
 
 template <typename TY, typename TO>
-int combine_launch(cudaStream_t st, int n, const TY *y, int64_t ldy, int cap, const float *rw,
+int combine_launch(cudaStream_t st, int sms, int n, const TY *y, int64_t ldy, int cap, const float *rw,
                    const int *tok_pos, int T, int KK, int D, TO *out, int64_t ldo,
                    int accumulate) {
-    const int nseg = 1, seg = D;
-    const int64_t units = int64_t(T) * nseg, grid = (units + 7) / 8;
+    const Segments s(T, (D + n - 1) / n, 32, sms);
+    const int64_t units = int64_t(T) * s.n, grid = (units + 7) / 8;
     if (grid > kMaxGrid)
         return host_fail(MVLLM_ERR_INVALID, "combine: T too large");
 #define MVB_COMBINE(N)                                                                         \
     MVB_TRY(launch_serial(combine_rows_kernel<TY, TO, N>, dim3(unsigned(grid)), dim3(256), 0,  \
-                          st, y, ldy, cap, rw, tok_pos, units, nseg, seg, KK, D, out, ldo,     \
-                          accumulate))
+                          st, y, ldy, cap, rw, tok_pos, units, s.n, s.words * N, KK, D, out,   \
+                          ldo, accumulate))
     if (n == 16 / int(sizeof(TY)))
         MVB_COMBINE(16 / int(sizeof(TY)));
     else if (n == 4 / int(sizeof(TY)) && n > 1)
@@ -115,15 +128,15 @@ int combine_any(const char *who, void *stream, const void *y, int y_dtype, int64
     const bool fy = y_dtype == MVLLM_DTYPE_F32, fo = out_dtype == MVLLM_DTYPE_F32;
     using bf = __nv_bfloat16;
     if (fy && fo)
-        return combine_launch(st, n, static_cast<const float *>(y), ldy, cap, rw, tok_pos, T, KK,
+        return combine_launch(st, dev.sms, n, static_cast<const float *>(y), ldy, cap, rw, tok_pos, T, KK,
                               D, static_cast<float *>(out), ldo, accumulate);
     if (fy)
-        return combine_launch(st, n, static_cast<const float *>(y), ldy, cap, rw, tok_pos, T, KK,
+        return combine_launch(st, dev.sms, n, static_cast<const float *>(y), ldy, cap, rw, tok_pos, T, KK,
                               D, static_cast<bf *>(out), ldo, accumulate);
     if (fo)
-        return combine_launch(st, n, static_cast<const bf *>(y), ldy, cap, rw, tok_pos, T, KK, D,
+        return combine_launch(st, dev.sms, n, static_cast<const bf *>(y), ldy, cap, rw, tok_pos, T, KK, D,
                               static_cast<float *>(out), ldo, accumulate);
-    return combine_launch(st, n, static_cast<const bf *>(y), ldy, cap, rw, tok_pos, T, KK, D,
+    return combine_launch(st, dev.sms, n, static_cast<const bf *>(y), ldy, cap, rw, tok_pos, T, KK, D,
                           static_cast<bf *>(out), ldo, accumulate);
 }
 
@@ -252,19 +265,13 @@ int route_dx(cudaStream_t st, const RouteGradArgs &a, int sms, TO *dx, int64_t l
 template <typename TX>
 int route_dw(cudaStream_t st, const RouteGradArgs &a, int sms, const TX *x, int64_t ldx,
              const int *nr, const int *xoff, const int *rows, float *drouter) {
-    const int type = sizeof(TX) == 4 ? MVLLM_DTYPE_F32 : MVLLM_DTYPE_BF16;
-    const int64_t ncol = (a.H + kRgCols - 1) / kRgCols;
-    const int64_t most = (int64_t(a.cap) / kRgRows + a.E) * ncol;
+    const int64_t groups = ((a.H + kRgCols - 1) / kRgCols + 7) / 8;
+    const int64_t most = (int64_t(a.cap) / kRgRows + a.E) * groups;
     const unsigned grid = unsigned(std::min<int64_t>(int64_t(sms) * 4, most));
-    const unsigned al = row_align(x, ldx, a.H, type);
-#define MVB_DW(N)                                                                              \
-    MVB_TRY(launch_serial(route_dw_kernel<TX, N>, dim3(grid), dim3(256), 0, st, a, x, ldx, nr, \
-                          xoff, rows, drouter))
-    if (al >= 16)
-        MVB_DW(16 / int(sizeof(TX)));
-    else
-        MVB_DW(1);
-#undef MVB_DW
+    const unsigned b = sizeof(TX);
+    const int vec = ((reinterpret_cast<uintptr_t>(x) | uint64_t(ldx) * b) & 15u) == 0;
+    MVB_TRY(launch_serial(route_dw_kernel<TX>, dim3(grid), dim3(256), 0, st, a, x, ldx, vec, nr,
+                          xoff, rows, drouter));
     return MVLLM_OK;
 }
 

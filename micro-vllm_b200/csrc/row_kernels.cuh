@@ -54,6 +54,25 @@ template <int N> __device__ __forceinline__ void load_row(const __nv_bfloat16 *p
     }
 }
 
+// N elements as loaded (32, 16, 8, 4 or 2 bytes), to be converted when used.
+template <int BYTES> struct RowWord;
+struct alignas(16) Word32 {
+    uint4 lo, hi;
+};
+template <> struct RowWord<32> { using type = Word32; };
+template <> struct RowWord<16> { using type = uint4; };
+template <> struct RowWord<8> { using type = uint2; };
+template <> struct RowWord<4> { using type = uint32_t; };
+template <> struct RowWord<2> { using type = uint16_t; };
+template <typename T, int N> struct RowVec {
+    using Word = typename RowWord<N * sizeof(T)>::type;
+    Word w;
+    __device__ __forceinline__ void load(const T *p) { w = *reinterpret_cast<const Word *>(p); }
+    __device__ __forceinline__ void get(float (&v)[N]) const {
+        load_row<N>(reinterpret_cast<const T *>(&w), v);
+    }
+};
+
 // The same way out; bf16 rounds once, to nearest even.
 template <int N> __device__ __forceinline__ void store_row(float *p, const float (&v)[N]) {
     if constexpr (N == 1) {
@@ -86,6 +105,52 @@ template <int N> __device__ __forceinline__ void store_row(__nv_bfloat16 *p, con
                        pack_bf16(v[6], v[7]));
     }
 }
+
+// 8 elements of a row, as loaded; 0 past K.
+template <typename TX> struct Raw8 {
+    uint4 u[sizeof(TX) / 2];
+    __device__ __forceinline__ void load(const TX *row, int c, int K, bool vec) {
+        if (vec && c + 8 <= K) {
+#pragma unroll
+            for (int q = 0; q < int(sizeof(TX)) / 2; ++q) // stays where it is written
+                asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(u[q].x), "=r"(u[q].y), "=r"(u[q].z), "=r"(u[q].w)
+                             : "l"(reinterpret_cast<const uint4 *>(row + c) + q)
+                             : "memory");
+        } else {
+            uint32_t w[sizeof(TX) * 2];
+#pragma unroll
+            for (int q = 0; q < int(sizeof(TX)) * 2; ++q) {
+                w[q] = 0;
+                if constexpr (sizeof(TX) == 4) {
+                    if (c + q < K)
+                        w[q] = __float_as_uint(row[c + q]);
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+                        if (c + 2 * q + b < K)
+                            w[q] |= uint32_t(__bfloat16_as_ushort(row[c + 2 * q + b])) << (16 * b);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < int(sizeof(TX)) / 2; ++q)
+                u[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint4 a = u[0];
+        if constexpr (sizeof(TX) == 4) {
+            const uint4 b = u[1];
+            v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y);
+            v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
+            v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y);
+            v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
+        } else {
+            v[0] = bf16_lo(a.x), v[1] = bf16_hi(a.x), v[2] = bf16_lo(a.y), v[3] = bf16_hi(a.y);
+            v[4] = bf16_lo(a.z), v[5] = bf16_hi(a.z), v[6] = bf16_lo(a.w), v[7] = bf16_hi(a.w);
+        }
+    }
+};
 
 // A token's slots, KK <= kMaxSlots, held by one warp: lane l keeps slots l
 // and l + 32.  A slot counts when its position lies in [0, cap).
@@ -123,7 +188,7 @@ struct WarpSlots {
     }
 };
 
-// dispatch: a warp takes (token, segment of the row), loads 32 words at a time
+// dispatch: a warp takes (token, segment of the row), loads 128 words at a time
 // and stores them at each of the token's positions: a copy of the bits, so W
 // is only the widest word (16, 4 or 2 bytes) that rows, pitches and addresses
 // are multiples of.  ldx, ldxs, seg and D count words.
@@ -133,6 +198,7 @@ __global__ void __launch_bounds__(256)
                          int64_t units, int nseg, int seg, int KK, int D, W *__restrict__ xs,
                          int64_t ldxs, int cap) {
     pdl_wait();
+    pdl_trigger();
     const int lane = threadIdx.x & 31;
     const int64_t unit = blockIdx.x * int64_t(blockDim.x >> 5) + (threadIdx.x >> 5);
     if (unit >= units)
@@ -145,27 +211,31 @@ __global__ void __launch_bounds__(256)
     const uint32_t m1 = __ballot_sync(0xffffffffu, sl.p1 >= 0);
     if (!(m0 | m1))
         return;
-    for (int col = s0; col < s1; col += 32) {
-        const int c = col + lane;
-        W v{};
-        if (c < s1)
-            v = x[t * ldx + c];
-        for (uint32_t m = m0; m; m &= m - 1) {
-            const int64_t p = __shfl_sync(0xffffffffu, sl.p0, __ffs(m) - 1);
-            if (c < s1)
-                xs[p * ldxs + c] = v;
-        }
-        for (uint32_t m = m1; m; m &= m - 1) {
-            const int64_t p = __shfl_sync(0xffffffffu, sl.p1, __ffs(m) - 1);
-            if (c < s1)
-                xs[p * ldxs + c] = v;
-        }
+    for (int col = s0; col < s1; col += 128) {
+        W v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (col + 32 * q + lane < s1)
+                v[q] = x[t * ldx + col + 32 * q + lane];
+        auto copy = [&](int64_t p) {
+            W *to = xs + p * ldxs + col + lane;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (col + 32 * q + lane < s1)
+                    to[32 * q] = v[q];
+        };
+        for (uint32_t m = m0; m; m &= m - 1)
+            copy(__shfl_sync(0xffffffffu, sl.p0, __ffs(m) - 1));
+        for (uint32_t m = m1; m; m &= m - 1)
+            copy(__shfl_sync(0xffffffffu, sl.p1, __ffs(m) - 1));
     }
 }
 
 // combine and the dispatch gradient: out[t] = (out[t] +) sum of rw[p] y[p]
 // over the token's positions in ascending order (ascending expert id), f32
 // fused multiply-adds, one rounding at the end.  rw == nullptr: weight 1.
+// A warp takes (token, segment of the row) and has eight positions' loads under
+// way at a time.
 template <typename TY, typename TO, int N>
 __global__ void __launch_bounds__(256)
     combine_rows_kernel(const TY *__restrict__ y, int64_t ldy, int cap,
@@ -173,7 +243,10 @@ __global__ void __launch_bounds__(256)
                         int64_t units, int nseg, int seg, int KK, int D, TO *__restrict__ out,
                         int64_t ldo, int accumulate) {
     pdl_wait();
-    __shared__ int spos[8][kMaxSlots];
+    pdl_trigger();
+    constexpr int B = 8;
+    __shared__ int spos[8][kMaxSlots + B];
+    __shared__ float sw[8][kMaxSlots + B];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t unit = blockIdx.x * int64_t(blockDim.x >> 5) + warp;
     if (unit >= units)
@@ -183,6 +256,15 @@ __global__ void __launch_bounds__(256)
     WarpSlots sl;
     sl.load(tok_pos, t, KK, cap);
     const int n = sl.sort(KK, spos[warp]);
+    // The last batch is filled up with the last position: loaded again, not added.
+    const int fill = n ? spos[warp][n - 1] : 0;
+    for (int j = lane; j < n + B; j += 32) {
+        if (j >= n)
+            spos[warp][j] = fill;
+        else
+            sw[warp][j] = rw ? rw[spos[warp][j]] : 1.f;
+    }
+    __syncwarp();
     for (int c = s0 + lane * N; c < s1; c += 32 * N) {
         float acc[N];
         if (accumulate)
@@ -191,14 +273,20 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
             for (int q = 0; q < N; ++q)
                 acc[q] = 0.f;
-        for (int j = 0; j < n; ++j) {
-            const int64_t p = spos[warp][j];
-            const float w = rw ? rw[p] : 1.f;
-            float v[N];
-            load_row<N>(y + p * ldy + c, v);
+        for (int j0 = 0; j0 < n; j0 += B) {
+            RowVec<TY, N> v[B];
 #pragma unroll
-            for (int q = 0; q < N; ++q)
-                acc[q] = fmaf(w, v[q], acc[q]);
+            for (int b = 0; b < B; ++b)
+                v[b].load(y + int64_t(spos[warp][j0 + b]) * ldy + c);
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                float f[N];
+                v[b].get(f);
+                if (j0 + b < n)
+#pragma unroll
+                    for (int q = 0; q < N; ++q)
+                        acc[q] = fmaf(sw[warp][j0 + b], f[q], acc[q]);
+            }
         }
         store_row<N>(out + t * ldo + c, acc);
     }
@@ -216,31 +304,63 @@ __global__ void __launch_bounds__(256)
                         int KK, int D, TY *__restrict__ dy, int64_t lddy,
                         float *__restrict__ dwt) {
     pdl_wait();
+    pdl_trigger();
+    // Vectors of dout a thread keeps while it goes through the positions.
+    constexpr int C = 4;
     __shared__ float part[8][kMaxSlots];
+    __shared__ int spos[kMaxSlots];
+    __shared__ float sw[kMaxSlots];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int64_t t = blockIdx.x;
-    for (int j = 0; j < KK; ++j) {
-        const int64_t p = tok_pos[t * KK + j];
-        float dot = 0.f;
-        if (p >= 0 && p < cap) {
-            const float w = rw[p];
-            for (int c = threadIdx.x * N; c < D; c += blockDim.x * N) {
-                float g[N], v[N], o[N];
-                load_row<N>(dout + t * lddo + c, g);
-                load_row<N>(y + p * ldy + c, v);
+    for (int j = threadIdx.x; j < KK; j += blockDim.x) {
+        int p = tok_pos[t * KK + j];
+        if (p >= cap)
+            p = -1;
+        spos[j] = p;
+        sw[j] = p >= 0 ? rw[p] : 0.f;
+    }
+    for (int j = lane; j < KK; j += 32)
+        part[warp][j] = 0.f;
+    __syncthreads();
+    const int step = blockDim.x * N;
+    for (int c0 = threadIdx.x * N; c0 - int(threadIdx.x) * N < D; c0 += C * step) {
+        RowVec<TD, N> g[C];
 #pragma unroll
-                for (int q = 0; q < N; ++q) {
-                    dot = fmaf(g[q], v[q], dot);
-                    o[q] = w * g[q];
+        for (int q = 0; q < C; ++q)
+            if (c0 + q * step < D)
+                g[q].load(dout + t * lddo + c0 + q * step);
+#pragma unroll 2
+        for (int j = 0; j < KK; ++j) {
+            const int64_t p = spos[j];
+            if (p < 0)
+                continue; // uniform over the CTA
+            const float w = sw[j];
+            RowVec<TY, N> v[C];
+#pragma unroll
+            for (int q = 0; q < C; ++q)
+                if (c0 + q * step < D)
+                    v[q].load(y + p * ldy + c0 + q * step);
+            float dot = 0.f;
+#pragma unroll
+            for (int q = 0; q < C; ++q) {
+                if (c0 + q * step < D) {
+                    float gf[N], vf[N], o[N];
+                    g[q].get(gf);
+                    v[q].get(vf);
+#pragma unroll
+                    for (int s = 0; s < N; ++s) {
+                        dot = fmaf(gf[s], vf[s], dot);
+                        o[s] = w * gf[s];
+                    }
+                    store_row<N>(dy + p * lddy + c0 + q * step, o);
                 }
-                store_row<N>(dy + p * lddy + c, o);
             }
-        }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (lane == 0)
-            part[warp][j] = dot;
+            for (int o = 16; o > 0; o >>= 1)
+                dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            if (lane == 0)
+                part[warp][j] += dot;
+        }
     }
     __syncthreads();
     for (int k = threadIdx.x; k < K; k += blockDim.x) {
@@ -248,8 +368,7 @@ __global__ void __launch_bounds__(256)
         float d = 0.f;
         for (int j = 0; j <= k; ++j) {
             if (idx[t * K + j] == e) { // the id's first slot
-                const int p = tok_pos[t * KK + j];
-                if (p >= 0 && p < cap)
+                if (spos[j] >= 0)
                     for (int w = 0; w < warps; ++w)
                         d += part[w][j];
                 break;
