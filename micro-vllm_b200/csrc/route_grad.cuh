@@ -130,13 +130,14 @@ __global__ void __launch_bounds__(256)
 // The same with the router's columns in shared memory.  Gathered from L2 the
 // rows are 4 T K H bytes (1.9 GB for 8192 tokens of 8 out of 384 experts, H
 // 7168), which L2 serves at about half of what shared memory does; so a CTA
-// keeps LPT * 4 columns of every expert and goes through tokens, LPT lanes
-// each.  The (column block, token) plane is cut evenly over the CTAs, column
+// keeps LPT * 4 columns of every expert (and a row of zeros for slots without
+// one) and goes through tokens, LPT lanes each.  The (column block, token) plane is cut evenly over the CTAs, column
 // blocks outermost.
 template <typename TO, int LPT>
 __global__ void __launch_bounds__(512)
     route_dx_tile_kernel(const RouteGradArgs a, TO *__restrict__ dx, int64_t lddx, int vec) {
     extern __shared__ __align__(16) float rg_tile[];
+    __shared__ __align__(16) int2 pairs[16][2][32]; // (row of the tile, dz) of a warp's slots
     constexpr int COLS = LPT * 4, TPW = 32 / LPT; // tokens a warp has at a time
     pdl_wait();
     pdl_trigger();
@@ -151,11 +152,13 @@ __global__ void __launch_bounds__(512)
         const int t0 = int(at - int64_t(b) * a.T);
         const int t1 = int(min(int64_t(a.T), t0 + end - at));
         __syncthreads(); // the last block's readers are done
-        for (int i = threadIdx.x; i < a.E * LPT; i += blockDim.x) {
+        for (int i = threadIdx.x; i < (a.E + 1) * LPT; i += blockDim.x) {
             const int e = i / LPT, c = (i - e * LPT) * 4;
             const float *src = a.router + int64_t(e) * a.H + c0 + c;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (vec && c0 + c + 4 <= a.H) {
+            if (e == a.E) {
+                // zeros
+            } else if (vec && c0 + c + 4 <= a.H) {
                 v = *reinterpret_cast<const float4 *>(src);
             } else {
                 if (c0 + c < a.H)
@@ -174,15 +177,17 @@ __global__ void __launch_bounds__(512)
         // by lane, the next batch's loaded before this one is worked off.
         const int bt = max(1, LPT / a.K), lk = lane % LPT;
         const int stride = 16 * TPW * bt;
-        auto fetch = [&](int t, int k0, int &e, float &dz) { // slots k0.. of tokens t..
-            e = -1, dz = 0.f;
+        auto fetch = [&](int t, int k0) { // slots k0.. of tokens t..
+            int e = a.E;
+            float dz = 0.f;
             const int tt = t + (a.K <= LPT ? lk / a.K : 0), k = a.K <= LPT ? lk % a.K : k0 + lk;
             if (tt < min(t1, t + bt) && k < a.K) {
                 e = a.idx[int64_t(tt) * a.K + k];
                 dz = a.dz[int64_t(tt) * a.K + k];
-                if (e >= a.E)
-                    e = -1;
+                if (e < 0 || e >= a.E)
+                    e = a.E, dz = 0.f;
             }
+            return make_int2(e * COLS, __float_as_int(dz));
         };
         const int c = c0 + col4;
         const bool whole = vec && c + 4 <= a.H;
@@ -200,14 +205,14 @@ __global__ void __launch_bounds__(512)
             }
         };
         int tb = t0 + (warp * TPW + sub) * bt;
-        int e_next;
-        float dz_next;
-        fetch(tb, 0, e_next, dz_next);
+        int2 next = fetch(tb, 0);
         const int rounds = (t1 - t0 + stride - 1) / stride; // the same for every lane
         for (int i = 0; i < rounds; ++i, tb += stride) {
-            int e = e_next;
-            float dz = dz_next;
-            fetch(tb + stride, 0, e_next, dz_next);
+            // Two buffers: the last round's readers may still be at theirs.
+            const int2 *slots = pairs[warp][i & 1] + sub * LPT;
+            pairs[warp][i & 1][lane] = next;
+            __syncwarp();
+            next = fetch(tb + stride, 0);
             for (int s = 0; s < bt; ++s) {
                 const int t = tb + s;
                 const bool live = t < t1;
@@ -215,19 +220,20 @@ __global__ void __launch_bounds__(512)
                 if (live && a.accumulate)
                     old(t, acc);
                 for (int k0 = 0; k0 < a.K; k0 += LPT) {
-                    if (k0 > 0) // more slots than lanes: bt is 1
-                        fetch(tb, k0, e, dz);
+                    if (k0 > 0) { // more slots than lanes: bt is 1
+                        __syncwarp();
+                        pairs[warp][i & 1][lane] = fetch(tb, k0);
+                        __syncwarp();
+                    }
                     const int n = min(LPT, a.K - k0);
 #pragma unroll 8
                     for (int j = 0; j < n; ++j) {
-                        const int ej = __shfl_sync(0xffffffffu, e, s * a.K + j, LPT);
-                        const float dj = __shfl_sync(0xffffffffu, dz, s * a.K + j, LPT);
-                        if (ej >= 0) {
-                            const float4 v =
-                                *reinterpret_cast<const float4 *>(rg_tile + ej * COLS + col4);
-                            acc[0] = fmaf(dj, v.x, acc[0]), acc[1] = fmaf(dj, v.y, acc[1]);
-                            acc[2] = fmaf(dj, v.z, acc[2]), acc[3] = fmaf(dj, v.w, acc[3]);
-                        }
+                        const int2 p = slots[s * a.K + j];
+                        const float4 v =
+                            *reinterpret_cast<const float4 *>(rg_tile + p.x + col4);
+                        const float dj = __int_as_float(p.y);
+                        acc[0] = fmaf(dj, v.x, acc[0]), acc[1] = fmaf(dj, v.y, acc[1]);
+                        acc[2] = fmaf(dj, v.z, acc[2]), acc[3] = fmaf(dj, v.w, acc[3]);
                     }
                 }
                 if (live) {
@@ -317,9 +323,10 @@ __global__ void __launch_bounds__(256)
         const int off = xoff[e], n = min(nr[e], a.cap);
         const int p0 = off + rb * kRgRows, p1 = min(min(off + n, p0 + kRgRows), a.cap);
         const int c = cb * kRgCols + lane * 8;
+        const bool inside = vec && (cb + 1) * kRgCols <= a.H;
         float acc[8] = {};
-        // 32 rows at a time, their tokens and dz by lane; rows that do not
-        // count are row 0 with dz 0, and not added
+        // 32 rows at a time, their tokens and dz by lane; one that does not
+        // count loads token 0's and is not added
         auto slots = [&](int pb, int &t, float &dz) {
             const int p = pb + lane;
             t = -1, dz = 0.f;
@@ -341,22 +348,28 @@ __global__ void __launch_bounds__(256)
             for (int j0 = 0; j0 < cnt; j0 += B) {
                 Raw8<TX> xv[B];
                 int tj[B];
+                float dj[B];
 #pragma unroll
                 for (int j = 0; j < B; ++j) {
                     tj[j] = __shfl_sync(0xffffffffu, t, j0 + j);
-                    if (tj[j] >= 0 && c < a.H)
-                        xv[j].load(x + tj[j] * ldx, c, a.H, vec);
+                    dj[j] = __shfl_sync(0xffffffffu, dz, j0 + j);
+                }
+                if (inside) { // uniform over the warp: loads side by side
+#pragma unroll
+                    for (int j = 0; j < B; ++j)
+                        xv[j].load_whole(x + max(tj[j], 0) * ldx + c);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < B; ++j)
+                        xv[j].load(x + max(tj[j], 0) * ldx, min(c, a.H), a.H, vec);
                 }
 #pragma unroll
                 for (int j = 0; j < B; ++j) {
-                    const float dj = __shfl_sync(0xffffffffu, dz, j0 + j);
-                    if (tj[j] >= 0) {
-                        float f[8];
-                        xv[j].get(f);
+                    float f[8];
+                    xv[j].get(f);
 #pragma unroll
-                        for (int s = 0; s < 8; ++s)
-                            acc[s] = fmaf(dj, f[s], acc[s]);
-                    }
+                    for (int s = 0; s < 8; ++s)
+                        acc[s] = tj[j] >= 0 ? fmaf(dj[j], f[s], acc[s]) : acc[s];
                 }
             }
         }
@@ -375,10 +388,7 @@ __global__ void __launch_bounds__(256)
         float base[8] = {};
         if (nblk > 1) {
             float *mine = a.partial + int64_t(slot) * a.H + c;
-#pragma unroll
-            for (int s = 0; s < 8; ++s)
-                if (c + s < a.H)
-                    mine[s] = acc[s];
+            put(mine, acc);
             __threadfence();
             __syncwarp();
             int arrived = 0;
@@ -390,11 +400,21 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
             for (int s = 0; s < 8; ++s)
                 acc[s] = 0.f;
-            for (int k = 0; k < nblk; ++k) {
+            const float *from = a.partial + int64_t(first[e]) * a.H + c;
+            if (whole && (cb + 1) * kRgCols <= a.H) {
+#pragma unroll 4
+                for (int k = 0; k < nblk; ++k, from += a.H) {
+                    const float4 u = __ldcg(reinterpret_cast<const float4 *>(from));
+                    const float4 w = __ldcg(reinterpret_cast<const float4 *>(from) + 1);
+                    acc[0] += u.x, acc[1] += u.y, acc[2] += u.z, acc[3] += u.w;
+                    acc[4] += w.x, acc[5] += w.y, acc[6] += w.z, acc[7] += w.w;
+                }
+            } else {
+                for (int k = 0; k < nblk; ++k, from += a.H)
 #pragma unroll
-                for (int s = 0; s < 8; ++s)
-                    if (c + s < a.H)
-                        acc[s] += __ldcg(a.partial + int64_t(first[e] + k) * a.H + c + s);
+                    for (int s = 0; s < 8; ++s)
+                        if (c + s < a.H)
+                            acc[s] += __ldcg(from + s);
             }
         }
         if (a.accumulate) {

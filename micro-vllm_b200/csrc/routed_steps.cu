@@ -240,8 +240,8 @@ int route_dx(cudaStream_t st, const RouteGradArgs &a, int sms, TO *dx, int64_t l
         return MVLLM_OK;
     }
     // The widest column block whose experts fit shared memory.
-    const int lpt = a.E * 512 <= kRgSmem ? 32 : a.E * 256 <= kRgSmem ? 16 : 8;
-    const int smem = a.E * lpt * 16;
+    const int lpt = (a.E + 1) * 512 <= kRgSmem ? 32 : (a.E + 1) * 256 <= kRgSmem ? 16 : 8;
+    const int smem = (a.E + 1) * lpt * 16;
     const int64_t work = int64_t((a.H + 4 * lpt - 1) / (4 * lpt)) * a.T;
     const int per_sm = std::max(1, std::min(4, kRgSmem / std::max(smem, 1)));
     const unsigned grid = unsigned(std::min<int64_t>(int64_t(sms) * per_sm, (work + 15) / 16));

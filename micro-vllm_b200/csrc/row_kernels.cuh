@@ -109,6 +109,11 @@ template <int N> __device__ __forceinline__ void store_row(__nv_bfloat16 *p, con
 // 8 elements of a row, as loaded; 0 past K.
 template <typename TX> struct Raw8 {
     uint4 u[sizeof(TX) / 2];
+    __device__ __forceinline__ void load_whole(const TX *p) {
+#pragma unroll
+        for (int q = 0; q < int(sizeof(TX)) / 2; ++q)
+            u[q] = reinterpret_cast<const uint4 *>(p)[q];
+    }
     __device__ __forceinline__ void load(const TX *row, int c, int K, bool vec) {
         if (vec && c + 8 <= K) {
 #pragma unroll
