@@ -3,6 +3,7 @@
 #include "matvec_q4.cuh"
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <map>
 #include <mutex>
@@ -129,13 +130,42 @@ template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
         return MVLLM_OK;
     }
 
+    // The rule's answer by sizes; asking it takes longer than a small product.
+    static int cached_plan(const void *kern, MatvecPlan &p, int rows_each, int items, int nb,
+                           int sms, int *ranks, int *grid) {
+        struct Answer {
+            MatvecPlan p;
+            int ranks, grid;
+        };
+        static std::mutex mu;
+        static std::map<std::array<int, 6>, Answer> seen;
+        const std::array<int, 6> key = {p.N, p.K, p.rows_most, rows_each, items, nb};
+        std::lock_guard<std::mutex> lk(mu);
+        auto it = seen.find(key);
+        if (it == seen.end()) {
+            Answer a{p, 1, 1};
+            if (int rc = plan(kern, a.p, rows_each, items, nb, sms, &a.ranks, &a.grid))
+                return rc;
+            if (seen.size() >= 4096) // a caller of ever new sizes
+                seen.clear();
+            it = seen.emplace(key, a).first;
+        }
+        const int y_f32 = p.y_f32, x_vec = p.x_vec;
+        p = it->second.p;
+        p.y_f32 = y_f32, p.x_vec = x_vec;
+        *ranks = it->second.ranks, *grid = it->second.grid;
+        return MVLLM_OK;
+    }
+
     static int launch(cudaStream_t st, MatvecArgs a, MatvecPlan p, int items, int sms,
                       const void *x, int64_t ldx, void *y, int64_t ldy) {
         auto kern = matvec_q4_kernel<FMT, TX, NT, GRAD>;
         int ranks = 1, grid = 1;
-        MVB_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMvSmem));
-        if (int rc = plan(reinterpret_cast<const void *>(kern), p, (a.rows + a.nb - 1) / a.nb, items, a.nb,
-                          sms, &ranks, &grid))
+        static const cudaError_t sized = cudaFuncSetAttribute(
+            kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMvSmem);
+        MVB_TRY(sized);
+        if (int rc = cached_plan(reinterpret_cast<const void *>(kern), p,
+                                 (a.rows + a.nb - 1) / a.nb, items, a.nb, sms, &ranks, &grid))
             return rc;
         const int smem = layout(p, p.chunk, ranks, a.nb);
         if (smem > kMvSmem)

@@ -29,13 +29,18 @@ struct RouteGradArgs {
     float scale;
     float *dz;      // [T, K] the slots' dz
     float *dzp;     // [cap] the sorted positions' dz
-    int *arrived;   // [E, column blocks] partial sums of an expert that are done
+    int *arrived;   // [E, column blocks] partial sums of an expert that are done,
+                    // and one more: the drouter items taken
     float *partial; // [row blocks][H]
 };
 
 constexpr int kRgCols = 256; // columns of a drouter item
 constexpr int kRgRows = 128; // sorted rows of a drouter item
 constexpr int kRgSmem = 200 * 1024;
+#ifndef RGW
+#define RGW 32
+#endif
+constexpr int kRgWarps = RGW; // of a dx CTA
 
 // dz of lane k's slot (K <= 32, one warp a token); 0 for lanes past K and ids
 // outside [0, E).
@@ -134,10 +139,10 @@ __global__ void __launch_bounds__(256)
 // one) and goes through tokens, LPT lanes each.  The (column block, token) plane is cut evenly over the CTAs, column
 // blocks outermost.
 template <typename TO, int LPT>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(32 * kRgWarps)
     route_dx_tile_kernel(const RouteGradArgs a, TO *__restrict__ dx, int64_t lddx, int vec) {
     extern __shared__ __align__(16) float rg_tile[];
-    __shared__ __align__(16) int2 pairs[16][2][32]; // (row of the tile, dz) of a warp's slots
+    __shared__ __align__(16) int2 pairs[kRgWarps][2][32]; // (row of the tile, dz) of a warp's slots
     constexpr int COLS = LPT * 4, TPW = 32 / LPT; // tokens a warp has at a time
     pdl_wait();
     pdl_trigger();
@@ -176,7 +181,7 @@ __global__ void __launch_bounds__(512)
         // A group of LPT lanes takes BT tokens at a time, their slots' ids and dz
         // by lane, the next batch's loaded before this one is worked off.
         const int bt = max(1, LPT / a.K), lk = lane % LPT;
-        const int stride = 16 * TPW * bt;
+        const int stride = kRgWarps * TPW * bt;
         auto fetch = [&](int t, int k0) { // slots k0.. of tokens t..
             int e = a.E;
             float dz = 0.f;
@@ -254,11 +259,10 @@ __global__ void __launch_bounds__(512)
     }
 }
 
-// drouter[e] = sum over e's sorted rows of dz x[rows].  An item is (eight
-// blocks of kRgCols columns, an expert, kRgRows of its rows), a column block
-// for each of the CTA's warps, which go on without meeting; a warp has eight
-// (f32: four) rows' loads under way.  Items run column group by column group,
-// so the columns of x that all experts gather from (16 T kRgCols bytes in
+// drouter[e] = sum over e's sorted rows of dz x[rows].  An item is (a block of
+// kRgCols columns, an expert, kRgRows of its rows); each warp takes the next
+// one, and has eight (f32: four) rows' loads under way.  Items run by groups of
+// eight column blocks, so the columns of x that all experts gather from (16 T kRgCols bytes in
 // bf16) stay in L2.  An expert of several items leaves its partial sums in the
 // workspace, and the warp that arrives last adds them in order; one without
 // rows gets zeros.
@@ -306,11 +310,18 @@ __global__ void __launch_bounds__(256)
     // (No more than the workspace holds, whatever nr says.)
     const int blocks = min(first[a.E], a.cap / kRgRows + a.E);
     const int ncol = (a.H + kRgCols - 1) / kRgCols, groups = (ncol + 7) / 8;
-    for (int64_t it = blockIdx.x; it < int64_t(blocks) * groups; it += gridDim.x) {
-        const int cg = int(it / blocks), slot = int(it - int64_t(cg) * blocks);
-        const int cb = cg * 8 + warp;
+    const int total = blocks * groups * 8;
+    for (;;) { // a warp at a time: items differ in rows by a hundredfold
+        int ticket = 0;
+        if (lane == 0)
+            ticket = atomicAdd(&a.arrived[a.E * ncol], 1);
+        ticket = __shfl_sync(0xffffffffu, ticket, 0);
+        if (ticket >= total)
+            break;
+        const int cg = ticket / (blocks * 8), slot = ticket / 8 - cg * blocks;
+        const int cb = cg * 8 + (ticket & 7);
         if (cb >= ncol)
-            continue; // uniform over the warp; warps do not meet here
+            continue;
         int lo = 0, hi = a.E; // the last expert with first[e] <= slot
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;

@@ -243,13 +243,13 @@ int route_dx(cudaStream_t st, const RouteGradArgs &a, int sms, TO *dx, int64_t l
     const int lpt = (a.E + 1) * 512 <= kRgSmem ? 32 : (a.E + 1) * 256 <= kRgSmem ? 16 : 8;
     const int smem = (a.E + 1) * lpt * 16;
     const int64_t work = int64_t((a.H + 4 * lpt - 1) / (4 * lpt)) * a.T;
-    const int per_sm = std::max(1, std::min(4, kRgSmem / std::max(smem, 1)));
+    const int per_sm = std::max(1, std::min(64 / kRgWarps, kRgSmem / smem));
     const unsigned grid = unsigned(std::min<int64_t>(int64_t(sms) * per_sm, (work + 15) / 16));
 #define MVB_DX(L)                                                                              \
     do {                                                                                       \
         MVB_TRY(cudaFuncSetAttribute(route_dx_tile_kernel<TO, L>,                              \
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kRgSmem));   \
-        MVB_TRY(launch_serial(route_dx_tile_kernel<TO, L>, dim3(grid), dim3(512), smem, st, a, \
+        MVB_TRY(launch_serial(route_dx_tile_kernel<TO, L>, dim3(grid), dim3(32 * kRgWarps), smem, st, a, \
                               dx, lddx, int(vec)));                                            \
     } while (0)
     if (lpt == 32)
@@ -283,8 +283,9 @@ size_t mvllm_moe_route_grad_workspace(int T, int H, int E, int K) {
     if (T < 0 || H < 1 || E < 1 || K < 1)
         return 0;
     const size_t slots = size_t(T) * K, ncol = (size_t(H) + kRgCols - 1) / kRgCols;
-    // dz by slot and by position, counters, partial sums of each row block
-    return (2 * slots + E * ncol + (slots / kRgRows + E) * H) * sizeof(float) + 4 * 256;
+    // dz by slot and by position, counters, partial sums of each row block, all
+    // on 256-byte boundaries
+    return (2 * slots + E * ncol + 1 + (slots / kRgRows + E) * H) * sizeof(float) + 5 * 256;
 }
 
 int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t ldx, int T, int H,
@@ -323,9 +324,9 @@ int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t l
     };
     a.dz = take(slots);
     a.dzp = take(slots);
-    a.arrived = reinterpret_cast<int *>(take(size_t(E) * ncol));
+    a.arrived = reinterpret_cast<int *>(take(size_t(E) * ncol + 1));
     a.partial = take((slots / kRgRows + E) * H);
-    const int counters = drouter ? E * ncol : 0;
+    const int counters = drouter ? E * ncol + 1 : 0;
     const int warps = std::max(T, (counters + 31) / 32);
     MVB_TRY(launch_serial(route_dz_kernel, dim3((warps + 7) / 8), dim3(256), 0, st, a, counters));
     if (T > 0 && dx) {

@@ -670,42 +670,53 @@ def route_dev(x, router, bias, K, idx, wt, scores, choice, stream=None):
 # ------------------------------------- the routed layer's steps, with gradients --
 def _on(t, name):
     """A device tensor of the library's device."""
-    if t is None or not t.is_cuda:
-        raise ValueError(f"{name}: a CUDA tensor is needed")
-    if _device is not None and t.device.index != _device:
-        raise ValueError(f"{name}: on {t.device}, the library runs on cuda:{_device}")
+    at = -1 if t is None else t.get_device()
+    if at != _device:
+        if at < 0:
+            raise ValueError(f"{name}: a CUDA tensor is needed")
+        if _device is not None:
+            raise ValueError(f"{name}: on cuda:{at}, the library runs on cuda:{_device}")
 
 
-def _rows(t, name, shape, out=False):
-    """Pointer, dtype code and row pitch of a row matrix: f32 or bf16, its
-    elements side by side within a row; an output's rows may not overlap."""
+def _dtype_name(dtype):
+    """The dtype's name; str() of one costs more than the rest of a check."""
+    name = _dtype_names.get(dtype)
+    if name is None:
+        name = _dtype_names[dtype] = str(dtype)
+    return name
+
+
+_dtype_names = {}
+_ROW_DTYPES = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16}
+
+
+def _rows(t, name, rows, cols, out=False):
+    """Address, dtype code and row pitch of a row matrix [rows, cols]: f32 or
+    bf16, its elements side by side within a row; an output's rows may not
+    overlap."""
     _on(t, name)
-    code = _ROW_DTYPES.get(str(t.dtype))
+    code = _ROW_DTYPES.get(_dtype_name(t.dtype))
     if code is None:
         raise ValueError(f"{name}: {t.dtype}, torch.float32 or torch.bfloat16 is needed")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, {shape} is needed")
-    rows, cols = shape
-    pitch = t.stride(0)
-    if cols > 1 and t.stride(1) != 1 and rows:
+    if t.shape != (rows, cols):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, {(rows, cols)} is needed")
+    pitch, step = t.stride()
+    if cols > 1 and step != 1 and rows:
         raise ValueError(f"{name}: the elements of a row must be contiguous")
     if rows <= 1:
         pitch = cols
     if out and pitch < cols:
         raise ValueError(f"{name}: its rows overlap")
-    return C.c_void_p(t.data_ptr()), code, pitch
-
-
-_ROW_DTYPES = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16}
+    return t.data_ptr(), code, pitch
 
 
 def _flat(t, name, dtype, count):
-    """Pointer of a contiguous device tensor of `count` elements or more."""
+    """Address of a contiguous device tensor of `count` elements or more."""
     _on(t, name)
-    if str(t.dtype) != dtype or not t.is_contiguous() or t.numel() < count:
+    if _dtype_name(t.dtype) != dtype or not t.is_contiguous() or t.numel() < count:
         raise ValueError(f"{name}: a contiguous {dtype} tensor of at least {count} is needed, "
                          f"got {t.dtype} {tuple(t.shape)}")
-    return C.c_void_p(t.data_ptr())
+    return t.data_ptr()
 
 
 def _slots(tok_pos):
@@ -718,7 +729,7 @@ def _slots(tok_pos):
 def _matrix(t, name):
     if t is None or t.dim() != 2:
         raise ValueError(f"{name}: a 2-D tensor is needed")
-    return tuple(t.shape)
+    return t.shape
 
 
 def _stream_at(stream, t):
@@ -726,7 +737,7 @@ def _stream_at(stream, t):
     if stream is None:
         import torch
         stream = torch.cuda.current_stream(t.device)
-    return C.c_void_p(stream.cuda_stream)
+    return stream.cuda_stream
 
 
 def dispatch_dev(x, tok_pos, xs, stream=None):
@@ -735,8 +746,8 @@ def dispatch_dev(x, tok_pos, xs, stream=None):
     as they were."""
     T, KK, pos = _slots(tok_pos)
     cap, D = _matrix(xs, "xs")
-    px, tx, ldx = _rows(x, "x", (T, D))
-    po, to, ldo = _rows(xs, "xs", (cap, D), out=True)
+    px, tx, ldx = _rows(x, "x", T, D)
+    po, to, ldo = _rows(xs, "xs", cap, D, out=True)
     if tx != to:
         raise ValueError("xs: the dtype of x is needed")
     _check(lib().mvllm_moe_dispatch_dev(_stream_at(stream, x), px, tx, ldx, pos, T, KK, D, po, ldo,
@@ -747,8 +758,8 @@ def dispatch_grad_dev(dxs, tok_pos, dx, accumulate=False, stream=None):
     """dx[t] (+)= sum_j dxs[tok_pos[t, j]], the gradient of dispatch_dev."""
     T, KK, pos = _slots(tok_pos)
     cap, D = _matrix(dxs, "dxs")
-    pi, ti, ldi = _rows(dxs, "dxs", (cap, D))
-    po, to, ldo = _rows(dx, "dx", (T, D), out=True)
+    pi, ti, ldi = _rows(dxs, "dxs", cap, D)
+    po, to, ldo = _rows(dx, "dx", T, D, out=True)
     _check(lib().mvllm_moe_dispatch_grad_dev(_stream_at(stream, dx), pi, ti, ldi, cap, pos, T, KK,
                                              D, po, to, ldo, int(bool(accumulate))))
 
@@ -759,8 +770,8 @@ def combine_dev(y, rw, tok_pos, out, accumulate=False, stream=None):
     wrote."""
     T, KK, pos = _slots(tok_pos)
     cap, D = _matrix(y, "y")
-    pi, ti, ldi = _rows(y, "y", (cap, D))
-    po, to, ldo = _rows(out, "out", (T, D), out=True)
+    pi, ti, ldi = _rows(y, "y", cap, D)
+    po, to, ldo = _rows(out, "out", T, D, out=True)
     _check(lib().mvllm_moe_combine_dev(
         _stream_at(stream, out), pi, ti, ldi, cap, _flat(rw, "rw", "torch.float32",
                                                          min(cap, T * KK)),
@@ -774,9 +785,9 @@ def combine_grad_dev(dout, y, rw, tok_pos, idx, dy, dwt, stream=None):
     T, KK, pos = _slots(tok_pos)
     K = _matrix(idx, "idx")[1]
     cap, D = _matrix(y, "y")
-    pd, td, ldd = _rows(dout, "dout", (T, D))
-    pi, ti, ldi = _rows(y, "y", (cap, D))
-    po, to, ldo = _rows(dy, "dy", (cap, D), out=True)
+    pd, td, ldd = _rows(dout, "dout", T, D)
+    pi, ti, ldi = _rows(y, "y", cap, D)
+    po, to, ldo = _rows(dy, "dy", cap, D, out=True)
     if to != ti:
         raise ValueError("dy: the dtype of y is needed")
     _check(lib().mvllm_moe_combine_grad_dev(
@@ -801,8 +812,8 @@ def route_grad_dev(x, router, idx, scores, dwt, nr, xoff, rows, tok_pos, dx, dro
     T, KK, pos = _slots(tok_pos)
     E, H = _matrix(router, "router")
     K = _matrix(idx, "idx")[1]
-    px, tx, ldx = _rows(x, "x", (T, H))
-    pd, td, ldd = (None, DTYPE_F32, 0) if dx is None else _rows(dx, "dx", (T, H), out=True)
+    px, tx, ldx = _rows(x, "x", T, H)
+    pd, td, ldd = (None, DTYPE_F32, 0) if dx is None else _rows(dx, "dx", T, H, out=True)
     if workspace is None:
         workspace = torch.empty(route_grad_workspace_bytes(T, H, E, K), dtype=torch.uint8,
                                 device=x.device)
@@ -829,8 +840,8 @@ def _q4(fmt, w, scales, I, O):
 def _matvec(entry, fmt, x, w, scales, y, I, O, stream):
     pw, ps = _q4(fmt, w, scales, I, O)
     S = x.shape[0]
-    px, tx, ldx = _rows(x, "the input rows", tuple(x.shape))
-    py, ty, ldy = _rows(y, "the output rows", (S, y.shape[1]), out=True)
+    px, tx, ldx = _rows(x, "the input rows", S, x.shape[1])
+    py, ty, ldy = _rows(y, "the output rows", S, y.shape[1], out=True)
     _check(entry(_stream_at(stream, x), fmt, px, tx, ldx, pw, ps, S, I, O, py, ty, ldy))
 
 
@@ -851,8 +862,8 @@ def _expert_matvec(entry, fmt, x, w, scales, nr, xoff, y, I, O, stream):
     if fmt not in (FMT_INT4_G64, FMT_MXFP4):
         raise ValueError(f"fmt {fmt}: FMT_INT4_G64 or FMT_MXFP4 is needed")
     nb, cap = nr.numel(), x.shape[0]
-    px, tx, ldx = _rows(x, "the input rows", tuple(x.shape))
-    py, ty, ldy = _rows(y, "the output rows", (cap, y.shape[1]), out=True)
+    px, tx, ldx = _rows(x, "the input rows", cap, x.shape[1])
+    py, ty, ldy = _rows(y, "the output rows", cap, y.shape[1], out=True)
     _check(entry(_stream_at(stream, x), fmt, nb, px, tx, ldx, cap,
                  _flat(nr, "nr", "torch.int32", nb), _flat(xoff, "xoff", "torch.int32", nb),
                  _flat(w, "w", "torch.int64", nb), _flat(scales, "scales", "torch.int64", nb),
