@@ -41,9 +41,9 @@ int max_clusters(const void *kern, int threads, int ranks, int smem, int *out) {
     return MVLLM_OK;
 }
 
-template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
+template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
     using F = MvFormat<FMT>;
-    static constexpr int T = MvTerms<FMT, TX, GRAD>::T, RP = 8 * NT / T;
+    static constexpr int T = MvTerms<FMT, TX, GRAD, FINE>::T, RP = 8 * NT / T;
     static constexpr int TILE = GRAD ? kMvCols : kMvRows, STEP = GRAD ? kMvRows : kMvCols;
     static constexpr int WARPS = mv_warps<NT, GRAD>(), THREADS = 32 * WARPS;
     static constexpr int RING = WARPS * mv_ring<NT, GRAD>() * F::STAGE;
@@ -159,7 +159,7 @@ template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
 
     static int launch(cudaStream_t st, MatvecArgs a, MatvecPlan p, int items, int sms,
                       const void *x, int64_t ldx, void *y, int64_t ldy) {
-        auto kern = matvec_q4_kernel<FMT, TX, NT, GRAD>;
+        auto kern = matvec_q4_kernel<FMT, TX, NT, GRAD, FINE>;
         int ranks = 1, grid = 1;
         static const cudaError_t sized = cudaFuncSetAttribute(
             kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMvSmem);
@@ -189,30 +189,38 @@ template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
 
 // Rows of a matrix that a launch takes at a time: enough operand columns for
 // the average expert (all rows of a single matrix), at most 32 (gradient: 16).
-template <int FMT, typename TX, bool GRAD>
+template <int FMT, typename TX, bool GRAD, bool FINE>
 int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, int sms, const void *x,
                 int64_t ldx, void *y, int64_t ldy) {
-    constexpr int T = MvTerms<FMT, TX, GRAD>::T;
+    constexpr int T = MvTerms<FMT, TX, GRAD, FINE>::T;
     const int avg = (a.rows + a.nb - 1) / a.nb;
     auto items = [&](int rp) {
         return a.nb == 1 ? (a.rows + rp - 1) / rp
                          : std::min(a.rows, a.nb * ((avg + rp - 1) / rp));
     };
+    // One more than the average expert's rows, for the uneven ones; the
+    // gradient's wider form costs more than the second pass it saves them.
     const int want = a.nb == 1 || GRAD ? avg : avg + 1;
     if (want <= 8 / T)
-        return MvHost<FMT, TX, 1, GRAD>::launch(st, a, p, items(8 / T), sms, x, ldx, y, ldy);
+        return MvHost<FMT, TX, 1, GRAD, FINE>::launch(st, a, p, items(8 / T), sms, x, ldx, y, ldy);
     if (GRAD || want <= 16 / T)
-        return MvHost<FMT, TX, 2, GRAD>::launch(st, a, p, items(16 / T), sms, x, ldx, y, ldy);
+        return MvHost<FMT, TX, 2, GRAD, FINE>::launch(st, a, p, items(16 / T), sms, x, ldx, y,
+                                                      ldy);
     if constexpr (!GRAD)
-        return MvHost<FMT, TX, 4, false>::launch(st, a, p, items(32 / T), sms, x, ldx, y, ldy);
+        return MvHost<FMT, TX, 4, false, FINE>::launch(st, a, p, items(32 / T), sms, x, ldx, y,
+                                                       ldy);
     return MVLLM_OK;
 }
 
 template <int FMT, typename TX>
 int matvec_way(cudaStream_t st, bool grad, const MatvecArgs &a, const MatvecPlan &p, int sms,
                const void *x, int64_t ldx, void *y, int64_t ldy) {
-    return grad ? matvec_rows<FMT, TX, true>(st, a, p, sms, x, ldx, y, ldy)
-                : matvec_rows<FMT, TX, false>(st, a, p, sms, x, ldx, y, ldy);
+    if (!grad)
+        return matvec_rows<FMT, TX, false, false>(st, a, p, sms, x, ldx, y, ldy);
+    if constexpr (FMT == MVLLM_FMT_INT4_G64 && sizeof(TX) == 2)
+        if (p.y_f32)
+            return matvec_rows<FMT, TX, true, true>(st, a, p, sms, x, ldx, y, ldy);
+    return matvec_rows<FMT, TX, true, false>(st, a, p, sms, x, ldx, y, ldy);
 }
 
 int matvec_any(const char *who, void *stream, bool grad, const MatvecArgs &a, const void *x, int x_dtype, int64_t ldx, void *y, int y_dtype, int64_t ldy) {

@@ -78,14 +78,18 @@ template <int FMT> struct MvFormat {
     static constexpr int STAGE = kMvRows * (kMvCols / 2 + 16);
 };
 
-// Parts an x element is split into, and rows that 8 * NT operand columns hold.
-template <int FMT, typename TX, bool GRAD> struct MvTerms {
+// Parts an x element is split into; 8 * NT operand columns hold 8 * NT / T
+// rows.
+template <int FMT, typename TX, bool GRAD, bool FINE> struct MvTerms {
     static constexpr bool F32 = sizeof(TX) == 4;
     // forward: f16 parts, 11 bits each, scaled per group: bf16 fits one, f32
     // takes two (22 bits).  Gradient: bf16 parts, 8 bits each: bf16 rows of
-    // an MXFP4 matrix fit one; times an int4 matrix's f32 scale two keep 16 to
-    // 17 bits; f32 takes three (24 bits).
-    static constexpr int T = GRAD ? (F32 ? 3 : FMT == MVLLM_FMT_INT4_G64 ? 2 : 1) : (F32 ? 2 : 1);
+    // an MXFP4 matrix fit one, f32 takes three (24 bits); bf16 rows times an
+    // int4 matrix's f32 scales take three where the result is f32 (FINE), and
+    // two, 16 to 17 bits, where it is rounded to bf16's 8.
+    static constexpr int T =
+        !GRAD ? (F32 ? 2 : 1)
+              : (F32 ? 3 : FMT == MVLLM_FMT_INT4_G64 ? (FINE ? 3 : 2) : 1);
 };
 
 __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src) {
@@ -383,7 +387,7 @@ __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(uint32
 template <int FMT, typename TX, int NT>
 __device__ __forceinline__ void mv_fetch_rows(uint8_t *xs, int pitch, const TX *x, int64_t ldx,
                                               int r0, int n, int c0, int cols, int K, bool vec) {
-    constexpr int T = MvTerms<FMT, TX, false>::T;
+    constexpr int T = MvTerms<FMT, TX, false, false>::T;
     static_assert(sizeof(TX) == 2 * T, "raw elements fit their parts' places");
     for (MvGroups<32 * mv_warps<NT, false>()> at(cols / 8); at.r < n; at.next()) {
         const TX *row = x + int64_t(r0 + at.r) * ldx;
@@ -406,7 +410,7 @@ __device__ __forceinline__ void mv_fetch_rows(uint8_t *xs, int pitch, const TX *
 template <int FMT, typename TX, int NT>
 __device__ __forceinline__ bool mv_stage_forward(uint8_t *xs, float *ex, int pitch, int n, int cols,
                                                  bool try_common, uint32_t *row_max) {
-    constexpr int T = MvTerms<FMT, TX, false>::T, RP = 8 * NT / T;
+    constexpr int T = MvTerms<FMT, TX, false, false>::T, RP = 8 * NT / T;
     constexpr int GL = MvFormat<FMT>::G / 8; // lanes of a group
     using Groups = MvGroups<32 * mv_warps<NT, false>()>;
     const int lane = threadIdx.x & 31;
@@ -492,8 +496,8 @@ template <int FMT, typename TX, int NT>
 __device__ __forceinline__ void mv_stage_gradient(uint8_t *xs, int pitch, const TX *x, int64_t ldx,
                                                   int r0, int n, int c0, int cols, int K, bool vec,
                                                   bool have, const MvHeld<TX, NT> &held) {
-    constexpr int T = MvTerms<FMT, TX, true>::T;
     constexpr bool I4 = FMT == MVLLM_FMT_INT4_G64;
+    constexpr int T = I4 ? 1 : MvTerms<FMT, TX, true, false>::T; // int4: split later
     held.each(x, ldx, r0, n, c0, cols, K, vec, have, [&](const Raw8<TX> &raw, int r, int q) {
         float v[8];
         raw.get(v);
@@ -545,7 +549,7 @@ __device__ __forceinline__ void mv_forward(uint32_t st, int half, const uint32_t
                                            const float *ex,
                                            float (&acc)[2][NT][4]) {
     using F = MvFormat<FMT>;
-    constexpr int T = MvTerms<FMT, TX, false>::T, RP = 8 * NT / T;
+    constexpr int T = MvTerms<FMT, TX, false, false>::T, RP = 8 * NT / T;
     constexpr int BPG = F::G / 32; // 32-column blocks of a group
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     float sc[2][2][kMvCols / F::G];
@@ -648,11 +652,10 @@ __device__ __forceinline__ void mv_forward(uint32_t st, int half, const uint32_t
 // repeats the unit with CAREFUL, which keeps such a product whole in its first
 // part.  For MXFP4 CAREFUL stands for scale codes 0 and above 127, which the
 // short form of the scale's bits does not cover.
-template <int FMT, typename TX, int NT, bool CAREFUL>
+template <int FMT, int T, int NT, bool CAREFUL>
 __device__ __forceinline__ void mv_gradient(uint32_t st, int half, const uint32_t (&xs)[NT],
                                             float (&acc)[4][4][NT][4]) {
     constexpr bool I4 = FMT == MVLLM_FMT_INT4_G64;
-    constexpr int T = MvTerms<FMT, TX, true>::T;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     float pick[NT][3]; // int4: factors of hi, r (T = 2) or hi, r, mid (T = 3)
 #pragma unroll
@@ -792,7 +795,7 @@ template <int FMT, typename TX, int NT, bool GRAD> constexpr int mv_red_pitch() 
     return GRAD ? kMvCols + 1 : 36;
 }
 template <int FMT, typename TX, int NT, bool GRAD> constexpr int mv_red_size() {
-    return (GRAD ? 8 * NT : 8 * NT / MvTerms<FMT, TX, GRAD>::T) *
+    return (GRAD ? 8 * NT : 8 * NT / MvTerms<FMT, TX, GRAD, false>::T) *
            mv_red_pitch<FMT, TX, NT, GRAD>();
 }
 template <int FMT, typename TX, bool GRAD> __host__ __device__ constexpr int mv_x_pitch(int cols) {
@@ -876,12 +879,12 @@ struct MvUnit {
 // take them in turn, each streaming its tasks' stages through its own ring, so
 // the main loop has no barrier.  The wk x cluster partial sums of an output
 // meet in (distributed) shared memory and are added in a fixed order.
-template <int FMT, typename TX, int NT, bool GRAD>
+template <int FMT, typename TX, int NT, bool GRAD, bool FINE>
 __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
     matvec_q4_kernel(const MatvecArgs a, const MatvecPlan pl, const TX *__restrict__ x,
                      int64_t ldx, void *__restrict__ y, int64_t ldy) {
     using F = MvFormat<FMT>;
-    constexpr int T = MvTerms<FMT, TX, GRAD>::T, RP = 8 * NT / T, ST = mv_ring<NT, GRAD>();
+    constexpr int T = MvTerms<FMT, TX, GRAD, FINE>::T, RP = 8 * NT / T, ST = mv_ring<NT, GRAD>();
     constexpr int kMvWarps = mv_warps<NT, GRAD>(), kMvThreads = 32 * kMvWarps;
     constexpr int TILE = GRAD ? kMvCols : kMvRows, STEP = GRAD ? kMvRows : kMvCols;
     constexpr int RPITCH = mv_red_pitch<FMT, TX, NT, GRAD>();
@@ -1123,9 +1126,9 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
                             xat[nt] = xcol[nt] + step * (STEP * XB);
                         if constexpr (GRAD)
                             if (careful || (FMT == MVLLM_FMT_MXFP4 && mv_odd_codes(st, half)))
-                                mv_gradient<FMT, TX, NT, true>(st, half, xat, accg);
+                                mv_gradient<FMT, T, NT, true>(st, half, xat, accg);
                             else
-                                mv_gradient<FMT, TX, NT, false>(st, half, xat, accg);
+                                mv_gradient<FMT, T, NT, false>(st, half, xat, accg);
                         else if (common)
                             mv_forward<FMT, TX, NT, true>(st, half, xat, ex, accf);
                         else
