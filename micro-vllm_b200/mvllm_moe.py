@@ -732,12 +732,20 @@ def _matrix(t, name):
     return t.shape
 
 
+_raw_stream = None  # device index -> handle of torch's current stream
+
+
 def _stream_at(stream, t):
-    """The given stream, or the current one of the tensor's device."""
-    if stream is None:
+    """Handle of the given stream, or of the current one of the tensor's device."""
+    global _raw_stream
+    if stream is not None:
+        return stream.cuda_stream
+    if _raw_stream is None:
         import torch
-        stream = torch.cuda.current_stream(t.device)
-    return stream.cuda_stream
+        # without a Stream object around it, which takes 2 us to make
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
+    return _raw_stream(t.get_device())
 
 
 def dispatch_dev(x, tok_pos, xs, stream=None):

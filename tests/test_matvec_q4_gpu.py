@@ -251,3 +251,50 @@ def test_agrees_with_the_serial_product(moe):
         W = rc.decode(w, s, fmt, I)
         size = x.double().abs() @ W.T.abs()
         assert ((a - b).double().abs() <= (I / 16 + 64 + I * 0.5) * 2.0 ** -22 * size).all()
+
+
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_f32_results_keep_f32_precision(moe, fmt, dtype):
+    """With f32 results the parts of an element keep at least 22 bits (one
+    exact part for bf16 where the scale is a power of two): every term is off
+    by at most 2^-22, the sums' roundings by about as much, and random errors
+    add up to less in norm: 2^-20 of the result's."""
+    S, I, O = 6, 2048, 640
+    gen = torch.Generator().manual_seed(23)
+    w, s = rc.packed(gen, fmt, O, I, "cuda", spread=2)
+    W = rc.decode(w, s, fmt, I)
+    x, dy = (torch.randn(S, n, generator=gen).cuda().to(dtype) for n in (I, O))
+    y, dx = torch.empty(S, O, device="cuda"), torch.empty(S, I, device="cuda")
+    moe.matvec_q4_dev(fmt, x, w, s, y)
+    moe.matvec_q4_grad_dev(fmt, dy, w, s, dx)
+    for got, want in ((y, x.double() @ W.T), (dx, dy.double() @ W)):
+        assert (got.double() - want).norm() <= 2.0 ** -20 * want.norm()
+
+
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+def test_products_beyond_f32(moe, fmt):
+    """Finite rows and scales whose product passes f32's range: infinities of
+    the right sign, not NaN, and the other rows as ever."""
+    S, I, O = 3, 320, 128
+    gen = torch.Generator().manual_seed(29)
+    w, s = rc.packed(gen, fmt, O, I, "cuda", spread=0)
+    w.fill_(0x77 if fmt == MXFP4 else 0xFF)  # every weight 6, or 7
+    if fmt == INT4:
+        s.fill_(2.0 ** 100)
+    else:
+        s.fill_(227)
+    W = rc.decode(w, s, fmt, I)
+    for dtype in (F32, BF16):
+        dy = torch.ones(S, O, device="cuda", dtype=dtype) * 2.0 ** -110
+        dy[1] = 2.0 ** 60
+        dx = torch.empty(S, I, device="cuda")
+        moe.matvec_q4_grad_dev(fmt, dy, w, s, dx)
+        assert torch.isposinf(dx[1]).all()
+        check(dx[[0, 2]], dy[[0, 2]], W.T, O, "gradient")
+        x = torch.ones(S, I, device="cuda", dtype=dtype) * 2.0 ** -110
+        x[1] = -2.0 ** 60
+        y = torch.empty(S, O, device="cuda")
+        moe.matvec_q4_dev(fmt, x, w, s, y)
+        assert torch.isneginf(y[1]).all()
+        check(y[[0, 2]], x[[0, 2]], W, I, "forward")
