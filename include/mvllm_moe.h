@@ -526,10 +526,12 @@ MVLLM_API int mvllm_moe_dense_ffn_dev(void *stream, int fmt, int T, int H, int O
  *      MVLLM_DTYPE_*, row r at element r * ld; an input's ld may be 0 (one row
  *      for all), an output's is at least its width.  tok_pos [T, KK], KK =
  *      K + n_shared <= 64, rows, rw, nr, xoff are mvllm_moe_permute_dev's.
- *      Positions outside [0, rows_cap) count as no slot; rows of an output
- *      that no position names (behind the last segment) are left as they were.
+ *      rw has rows_cap entries; positions outside [0, rows_cap) count as no
+ *      slot; rows of an output that no position names (behind the last
+ *      segment) are left as they were.  D, H, I, O <= 2^30.
  *      Sums are f32 in a fixed order (results repeat to the bit) and round
- *      once.  Inputs and outputs may not overlap.  Stream-ordered, no host
+ *      once.  Inputs and outputs may not overlap; calls that may run at the
+ *      same time need a workspace each.  Stream-ordered, no host
  *      sync, no allocation, capturable; T = 0 (no rows) does nothing except
  *      where an output is still to be cleared (drouter). ---- */
 /* xs[tok_pos[t, j]] = x[t]: a copy of the bits (xs of x's dtype). */
@@ -581,15 +583,17 @@ MVLLM_API int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype,
                                        size_t workspace_bytes);
 /* Few rows times a 4-bit matrix (fmt 4 or 7): y[r] = W x[r] for S rows, y
  * [S, O], in tolerance mode: f32 sums in another order than
- * mvllm_matmul_dev's, f32 rows of x to f32 precision.  Weights are read once
- * for up to 8 rows; any S runs, but hundreds of rows per matrix are
- * mvllm_moe_layer_dev's tensor-core path's work.  Every alignment and odd I
- * run; rows of 16-byte multiples run fastest. */
+ * mvllm_matmul_dev's, f32 rows of x in two f16 parts (22 bits beside the
+ * largest value of their scale group).  A pass over the weights serves up to
+ * 32 rows (16 in f32); any S runs, but hundreds of rows per matrix are the
+ * tensor-core path's work (mvllm_moe_layer_dev).  Every alignment and odd I
+ * run; packed rows of 16-byte multiples run fastest. */
 MVLLM_API int mvllm_matvec_q4_dev(void *stream, int fmt, const void *x, int x_dtype, int64_t ldx,
                                   const void *w, const void *scales, int S, int I, int O, void *y,
                                   int y_dtype, int64_t ldy);
 /* Its gradient for the rows, the weights being frozen: dx[r] = W^T dy[r],
- * dy [S, O], dx [S, I]. */
+ * dy [S, O], dx [S, I]; a pass serves 2 to 16 rows.  The products dy * scale of
+ * int4 go in two bf16 parts where dx is bf16, in three where it is f32. */
 MVLLM_API int mvllm_matvec_q4_grad_dev(void *stream, int fmt, const void *dy, int dy_dtype,
                                        int64_t lddy, const void *w, const void *scales, int S,
                                        int I, int O, void *dx, int dx_dtype, int64_t lddx);

@@ -27,14 +27,14 @@ int host_device(int *device, int *sms);
 
 // Makes the library's device current for one call and puts the caller's back.
 struct DeviceScope {
-    int saved = -1, sms = 0;
+    int saved = -1, device = -1, sms = 0;
     int enter() {
-        int dev = -1, cur = -1;
-        if (int rc = host_device(&dev, &sms))
+        int cur = -1;
+        if (int rc = host_device(&device, &sms))
             return rc;
         MVB_TRY(cudaGetDevice(&cur));
-        if (cur != dev) {
-            MVB_TRY(cudaSetDevice(dev));
+        if (cur != device) {
+            MVB_TRY(cudaSetDevice(device));
             saved = cur;
         }
         return MVLLM_OK;

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <array>
+#include <atomic>
 #include <cmath>
 #include <map>
 #include <mutex>
@@ -16,12 +17,12 @@ namespace {
 using bf = __nv_bfloat16;
 
 // Clusters of `ranks` CTAs that fit the device at once (one CTA per SM),
-// asked once per kernel and shared-memory size.
-int max_clusters(const void *kern, int threads, int ranks, int smem, int *out) {
+// asked once per device, kernel and shared-memory size.
+int max_clusters(const void *kern, int threads, int ranks, int smem, int device, int *out) {
     static std::mutex mu;
-    static std::map<std::tuple<const void *, int, int>, int> seen;
+    static std::map<std::tuple<int, const void *, int, int>, int> seen;
     std::lock_guard<std::mutex> lk(mu);
-    auto key = std::make_tuple(kern, ranks, smem);
+    auto key = std::make_tuple(device, kern, ranks, smem);
     auto it = seen.find(key);
     if (it == seen.end()) {
         cudaLaunchConfig_t cfg{};
@@ -74,8 +75,8 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
     // another at the rate of its share of the memory or of what its warps
     // dequantise, a fixed cost per unit, the rounds that the units need, and
     // the rows it stages.
-    static int plan(const void *kern, MatvecPlan &p, int rows_each, int items, int nb, int sms,
-                    int *ranks, int *grid) {
+    static int plan(const void *kern, MatvecPlan &p, int rows_each, int items, int nb,
+                    const DeviceScope &dev, int *ranks, int *grid) {
         const int tiles = (p.N + TILE - 1) / TILE, steps = (p.K + STEP - 1) / STEP;
         const double compute = (GRAD ? 26.0 : 40.0) / (1.0 + 0.25 * (NT - 1)); // B/ns of a CTA
         const int most = GRAD ? WARPS : 64;
@@ -85,9 +86,9 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
             const int slice = (steps + c - 1) / c;
             if (c > 1 && slice * (c - 1) >= steps)
                 break;
-            int nc = sms;
+            int nc = dev.sms;
             if (c > 1)
-                if (int rc = max_clusters(kern, THREADS, c, kMvSmem, &nc))
+                if (int rc = max_clusters(kern, THREADS, c, kMvSmem, dev.device, &nc))
                     return rc;
             for (int wo = 1; wo <= std::min(most, tiles); ++wo) {
                 for (int wk = 1; wo * wk <= most && wk <= slice && wk <= WARPS; ++wk) {
@@ -132,19 +133,19 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
 
     // The rule's answer by sizes; asking it takes longer than a small product.
     static int cached_plan(const void *kern, MatvecPlan &p, int rows_each, int items, int nb,
-                           int sms, int *ranks, int *grid) {
+                           const DeviceScope &dev, int *ranks, int *grid) {
         struct Answer {
             MatvecPlan p;
             int ranks, grid;
         };
         static std::mutex mu;
-        static std::map<std::array<int, 6>, Answer> seen;
-        const std::array<int, 6> key = {p.N, p.K, p.rows_most, rows_each, items, nb};
+        static std::map<std::array<int, 7>, Answer> seen;
+        const std::array<int, 7> key = {dev.device, p.N, p.K, p.rows_most, rows_each, items, nb};
         std::lock_guard<std::mutex> lk(mu);
         auto it = seen.find(key);
         if (it == seen.end()) {
             Answer a{p, 1, 1};
-            if (int rc = plan(kern, a.p, rows_each, items, nb, sms, &a.ranks, &a.grid))
+            if (int rc = plan(kern, a.p, rows_each, items, nb, dev, &a.ranks, &a.grid))
                 return rc;
             if (seen.size() >= 4096) // a caller of ever new sizes
                 seen.clear();
@@ -157,18 +158,21 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
         return MVLLM_OK;
     }
 
-    static int launch(cudaStream_t st, MatvecArgs a, MatvecPlan p, int items, int sms,
+    static int launch(cudaStream_t st, MatvecArgs a, MatvecPlan p, int items, const DeviceScope &dev,
                       const void *x, int64_t ldx, void *y, int64_t ldy) {
         auto kern = matvec_q4_kernel<FMT, TX, NT, GRAD, FINE>;
         int ranks = 1, grid = 1;
-        static const cudaError_t sized = cudaFuncSetAttribute(
-            kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMvSmem);
-        MVB_TRY(sized);
+        static std::atomic<int> sized{-1}; // the device whose kernel may take the memory
+        if (sized.load() != dev.device) {
+            MVB_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kMvSmem));
+            sized.store(dev.device);
+        }
         if (int rc = cached_plan(reinterpret_cast<const void *>(kern), p,
-                                 (a.rows + a.nb - 1) / a.nb, items, a.nb, sms, &ranks, &grid))
+                                 (a.rows + a.nb - 1) / a.nb, items, a.nb, dev, &ranks, &grid))
             return rc;
         const int smem = layout(p, p.chunk, ranks, a.nb);
-        if (smem > kMvSmem)
+        if (p.range < 1 || smem > kMvSmem)
             return host_fail(MVLLM_ERR_UNSUPPORTED, "matvec_q4: %d bytes of shared memory", smem);
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(grid);
@@ -190,7 +194,7 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
 // Rows of a matrix that a launch takes at a time: enough operand columns for
 // the average expert (all rows of a single matrix), at most 32 (gradient: 16).
 template <int FMT, typename TX, bool GRAD, bool FINE>
-int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, int sms, const void *x,
+int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, const DeviceScope &dev, const void *x,
                 int64_t ldx, void *y, int64_t ldy) {
     constexpr int T = MvTerms<FMT, TX, GRAD, FINE>::T;
     const int avg = (a.rows + a.nb - 1) / a.nb;
@@ -202,32 +206,33 @@ int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, int s
     // gradient's wider form costs more than the second pass it saves them.
     const int want = a.nb == 1 || GRAD ? avg : avg + 1;
     if (want <= 8 / T)
-        return MvHost<FMT, TX, 1, GRAD, FINE>::launch(st, a, p, items(8 / T), sms, x, ldx, y, ldy);
+        return MvHost<FMT, TX, 1, GRAD, FINE>::launch(st, a, p, items(8 / T), dev, x, ldx, y, ldy);
     if (GRAD || want <= 16 / T)
-        return MvHost<FMT, TX, 2, GRAD, FINE>::launch(st, a, p, items(16 / T), sms, x, ldx, y,
+        return MvHost<FMT, TX, 2, GRAD, FINE>::launch(st, a, p, items(16 / T), dev, x, ldx, y,
                                                       ldy);
     if constexpr (!GRAD)
-        return MvHost<FMT, TX, 4, false, FINE>::launch(st, a, p, items(32 / T), sms, x, ldx, y,
+        return MvHost<FMT, TX, 4, false, FINE>::launch(st, a, p, items(32 / T), dev, x, ldx, y,
                                                        ldy);
     return MVLLM_OK;
 }
 
 template <int FMT, typename TX>
-int matvec_way(cudaStream_t st, bool grad, const MatvecArgs &a, const MatvecPlan &p, int sms,
+int matvec_way(cudaStream_t st, bool grad, const MatvecArgs &a, const MatvecPlan &p, const DeviceScope &dev,
                const void *x, int64_t ldx, void *y, int64_t ldy) {
     if (!grad)
-        return matvec_rows<FMT, TX, false, false>(st, a, p, sms, x, ldx, y, ldy);
+        return matvec_rows<FMT, TX, false, false>(st, a, p, dev, x, ldx, y, ldy);
     if constexpr (FMT == MVLLM_FMT_INT4_G64 && sizeof(TX) == 2)
         if (p.y_f32)
-            return matvec_rows<FMT, TX, true, true>(st, a, p, sms, x, ldx, y, ldy);
-    return matvec_rows<FMT, TX, true, false>(st, a, p, sms, x, ldx, y, ldy);
+            return matvec_rows<FMT, TX, true, true>(st, a, p, dev, x, ldx, y, ldy);
+    return matvec_rows<FMT, TX, true, false>(st, a, p, dev, x, ldx, y, ldy);
 }
 
-int matvec_any(const char *who, void *stream, bool grad, const MatvecArgs &a, const void *x, int x_dtype, int64_t ldx, void *y, int y_dtype, int64_t ldy) {
+int matvec_any(const char *who, void *stream, bool grad, const MatvecArgs &a, const void *x,
+               int x_dtype, int64_t ldx, void *y, int y_dtype, int64_t ldy) {
     const int out = grad ? a.I : a.O;
     if ((a.fmt != MVLLM_FMT_INT4_G64 && a.fmt != MVLLM_FMT_MXFP4) ||
-        (a.rows > 0 && (!x || !y)) || a.I < 1 ||
-        a.O < 1 || a.rows < 0 || ldx < 0 || ldy < out ||
+        (a.rows > 0 && (!x || !y)) || a.I < 1 || a.O < 1 || a.I > kMvMaxSide ||
+        a.O > kMvMaxSide || a.rows < 0 || a.rows > kMvMaxSide || ldx < 0 || ldy < out ||
         (x_dtype != MVLLM_DTYPE_F32 && x_dtype != MVLLM_DTYPE_BF16) ||
         (y_dtype != MVLLM_DTYPE_F32 && y_dtype != MVLLM_DTYPE_BF16))
         return host_fail(MVLLM_ERR_INVALID, "%s: invalid arguments", who);
@@ -242,12 +247,17 @@ int matvec_any(const char *who, void *stream, bool grad, const MatvecArgs &a, co
     p.y_f32 = y_dtype == MVLLM_DTYPE_F32;
     p.rows_most = a.rows;
     const bool fx = x_dtype == MVLLM_DTYPE_F32, i4 = a.fmt == MVLLM_FMT_INT4_G64;
-    p.x_vec = ((reinterpret_cast<uintptr_t>(x) | uint64_t(ldx) * (fx ? 4 : 2)) & 15u) == 0;
-    if (i4)
-        return fx ? matvec_way<MVLLM_FMT_INT4_G64, float>(st, grad, a, p, dev.sms, x, ldx, y, ldy)
-                  : matvec_way<MVLLM_FMT_INT4_G64, bf>(st, grad, a, p, dev.sms, x, ldx, y, ldy);
-    return fx ? matvec_way<MVLLM_FMT_MXFP4, float>(st, grad, a, p, dev.sms, x, ldx, y, ldy)
-              : matvec_way<MVLLM_FMT_MXFP4, bf>(st, grad, a, p, dev.sms, x, ldx, y, ldy);
+    const uint64_t pitch = a.rows > 1 ? uint64_t(ldx) * (fx ? 4 : 2) : 0;
+    p.x_vec = ((reinterpret_cast<uintptr_t>(x) | pitch) & 15u) == 0;
+    try { // the plans' tables allocate
+        if (i4)
+            return fx ? matvec_way<MVLLM_FMT_INT4_G64, float>(st, grad, a, p, dev, x, ldx, y, ldy)
+                      : matvec_way<MVLLM_FMT_INT4_G64, bf>(st, grad, a, p, dev, x, ldx, y, ldy);
+        return fx ? matvec_way<MVLLM_FMT_MXFP4, float>(st, grad, a, p, dev, x, ldx, y, ldy)
+                  : matvec_way<MVLLM_FMT_MXFP4, bf>(st, grad, a, p, dev, x, ldx, y, ldy);
+    } catch (...) {
+        return host_fail(MVLLM_ERR_NOMEM, "%s: out of host memory", who);
+    }
 }
 
 int matvec_one(const char *who, void *stream, bool grad, int fmt, const void *x, int x_dtype,

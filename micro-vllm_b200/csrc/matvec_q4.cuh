@@ -51,6 +51,7 @@ template <int NT, bool GRAD> constexpr int mv_ring() { return GRAD ? 4 : 2; }
 constexpr int kMvSmem = 226 * 1024; // dynamic part of the 227 KB
 constexpr int kMvRows = 32, kMvCols = 256; // weights of a warp's stage
 constexpr int kMvMaxExperts = 1024;
+constexpr int kMvMaxSide = 1 << 30; // rows and columns: steps past them stay in 32 bits
 
 // How a launch cuts its work, filled by the host (matvec_plan).
 struct MatvecPlan {

@@ -8,7 +8,9 @@
 //   dz_k = dm_k s'(z_k),  s' = s (1 - s)                     sigmoid
 //                         s' = (1 - e^(-s^2)) / (2 s)        sqrt(softplus),
 // the second from softplus' = sigmoid(z) = 1 - e^(-softplus) and s^2 =
-// softplus: both need the scores alone.  Then
+// softplus: both need the scores alone.  With w_k = m_k / M the product is
+// taken as (g_k - sum_j g_j w_j) w_k (s' / m_k), whose factors stay in range
+// where all scores of a token are tiny.  Then
 //   dx[t]      = sum_k dz_k router[idx_k]
 //   drouter[e] = sum over the tokens routed to e of dz x[t].
 // Only K of a token's E logits have a gradient, so the two products are
@@ -37,10 +39,7 @@ struct RouteGradArgs {
 constexpr int kRgCols = 256; // columns of a drouter item
 constexpr int kRgRows = 128; // sorted rows of a drouter item
 constexpr int kRgSmem = 200 * 1024;
-#ifndef RGW
-#define RGW 32
-#endif
-constexpr int kRgWarps = RGW; // of a dx CTA
+constexpr int kRgWarps = 32; // of a dx CTA
 
 // dz of lane k's slot (K <= 32, one warp a token); 0 for lanes past K and ids
 // outside [0, E).
@@ -54,18 +53,20 @@ __device__ __forceinline__ float route_slot_grad(const RouteGradArgs &a, int64_t
         m = fmaxf(a.scores[t * a.E + e], 0.f);
         g = a.scale * a.dwt[t * a.K + lane];
     }
-    float M = 0.f, G = 0.f;
-    for (int k = 0; k < a.K; ++k) { // slot order, the same on every lane
-        const float mk = __shfl_sync(0xffffffffu, m, k), gk = __shfl_sync(0xffffffffu, g, k);
-        M += mk;
-        G = fmaf(gk, mk, G);
-    }
-    if (e < 0 || !(m > 0.f))
+    float M = 0.f, G = 0.f; // sums in slot order, the same on every lane
+    for (int k = 0; k < a.K; ++k)
+        M += __shfl_sync(0xffffffffu, m, k);
+    const bool live = e >= 0 && m > 0.f;
+    const float w = live ? m / M : 0.f;
+    for (int k = 0; k < a.K; ++k)
+        G = fmaf(__shfl_sync(0xffffffffu, g, k), __shfl_sync(0xffffffffu, w, k), G);
+    if (!live)
         return 0.f;
-    const float dm = (g - G / M) / M;
-    const float slope = a.score_fn == MVLLM_SCORE_SQRT_SOFTPLUS ? -expm1f(-m * m) / (2.f * m)
-                                                                : m * (1.f - m);
-    return dm * slope;
+    const float mm = m * m;
+    const float slope = a.score_fn != MVLLM_SCORE_SQRT_SOFTPLUS ? 1.f - m
+                        : mm < 0x1p-24f                         ? 0.5f // 1 - e^-mm = mm
+                                                                : -expm1f(-mm) / (2.f * mm);
+    return (g - G) * w * slope;
 }
 
 // A warp per token: the slots' dz, and at the sorted position of each id their
@@ -136,8 +137,8 @@ __global__ void __launch_bounds__(256)
 // rows are 4 T K H bytes (1.9 GB for 8192 tokens of 8 out of 384 experts, H
 // 7168), which L2 serves at about half of what shared memory does; so a CTA
 // keeps LPT * 4 columns of every expert (and a row of zeros for slots without
-// one) and goes through tokens, LPT lanes each.  The (column block, token) plane is cut evenly over the CTAs, column
-// blocks outermost.
+// one) and goes through tokens, LPT lanes each.  The (column block, token) plane is cut evenly over the
+// CTAs, column blocks outermost.
 template <typename TO, int LPT>
 __global__ void __launch_bounds__(32 * kRgWarps)
     route_dx_tile_kernel(const RouteGradArgs a, TO *__restrict__ dx, int64_t lddx, int vec) {
@@ -262,10 +263,10 @@ __global__ void __launch_bounds__(32 * kRgWarps)
 // drouter[e] = sum over e's sorted rows of dz x[rows].  An item is (a block of
 // kRgCols columns, an expert, kRgRows of its rows); each warp takes the next
 // one, and has eight (f32: four) rows' loads under way.  Items run by groups of
-// eight column blocks, so the columns of x that all experts gather from (16 T kRgCols bytes in
-// bf16) stay in L2.  An expert of several items leaves its partial sums in the
-// workspace, and the warp that arrives last adds them in order; one without
-// rows gets zeros.
+// eight column blocks, so the columns of x that all experts gather from (16 T
+// kRgCols bytes in bf16) stay in L2.  An expert of several items leaves its
+// partial sums in the workspace, and the warp that arrives last adds them in
+// order; one without rows gets zeros.
 template <typename TX>
 __global__ void __launch_bounds__(256)
     route_dw_kernel(const RouteGradArgs a, const TX *__restrict__ x, int64_t ldx, int vec,

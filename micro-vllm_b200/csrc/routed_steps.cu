@@ -27,6 +27,7 @@ int row_vec(unsigned align, size_t bytes) {
 }
 
 constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr int kMaxRow = 1 << 30; // elements of a row: steps past its end stay in 32 bits
 
 // Segments of a row of `words` lane-words for T tokens: as few as fill the
 // device with warps (32 per SM), each a multiple of `piece` words.
@@ -49,7 +50,7 @@ int mvllm_moe_dispatch_dev(void *stream, const void *x, int dtype, int64_t ldx,
                            const int *tok_pos, int T, int KK, int D, void *xs, int64_t ldxs,
                            int rows_cap) {
     if ((T > 0 && (!x || !tok_pos || (!xs && rows_cap > 0))) || T < 0 || KK < 1 ||
-        KK > kMaxSlots || D < 1 || ldx < 0 || ldxs < D || rows_cap < 0 || !row_dtype(dtype))
+        KK > kMaxSlots || D < 1 || D > kMaxRow || ldx < 0 || ldxs < D || rows_cap < 0 || !row_dtype(dtype))
         return host_fail(MVLLM_ERR_INVALID, "dispatch_dev: invalid arguments");
     DeviceScope dev;
     if (int rc = dev.enter())
@@ -108,7 +109,7 @@ int combine_any(const char *who, void *stream, const void *y, int y_dtype, int64
                 const float *rw, const int *tok_pos, int T, int KK, int D, void *out,
                 int out_dtype, int64_t ldo, int accumulate) {
     if ((T > 0 && ((!y && cap > 0) || !tok_pos || !out)) || T < 0 || KK < 1 || KK > kMaxSlots ||
-        D < 1 || ldy < 0 || ldo < D || cap < 0 || !row_dtype(y_dtype) || !row_dtype(out_dtype))
+        D < 1 || D > kMaxRow || ldy < 0 || ldo < D || cap < 0 || !row_dtype(y_dtype) || !row_dtype(out_dtype))
         return host_fail(MVLLM_ERR_INVALID, "%s: invalid arguments", who);
     DeviceScope dev;
     if (int rc = dev.enter())
@@ -183,9 +184,8 @@ int mvllm_moe_combine_grad_dev(void *stream, const void *dout, int dout_dtype, i
                                const float *rw, const int *tok_pos, const int *idx, int T, int K,
                                int KK, int D, void *dy, int64_t lddy, float *dwt) {
     if ((T > 0 && (!dout || !tok_pos || !idx || !dwt || (rows_cap > 0 && (!y || !rw || !dy)))) ||
-        T < 0 || K < 1 || KK < K ||
-        KK > kMaxSlots || D < 1 || lddo < 0 || ldy < 0 || lddy < D || rows_cap < 0 ||
-        !row_dtype(dout_dtype) || !row_dtype(y_dtype))
+        T < 0 || K < 1 || KK < K || KK > kMaxSlots || D < 1 || D > kMaxRow || lddo < 0 ||
+        ldy < 0 || lddy < D || rows_cap < 0 || !row_dtype(dout_dtype) || !row_dtype(y_dtype))
         return host_fail(MVLLM_ERR_INVALID, "combine_grad_dev: invalid arguments");
     DeviceScope dev;
     if (int rc = dev.enter())
@@ -296,11 +296,12 @@ int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t l
                              float *drouter, int accumulate, void *workspace,
                              size_t workspace_bytes) {
     if ((T > 0 && (!x || !idx || !scores || !dwt || !rows || !tok_pos || (!dx && !drouter))) ||
-        !router || !nr || !xoff || T < 0 || H < 1 || E < 1 || E > 1024 || K < 1 || K > 32 || KK < K ||
-        KK > kMaxSlots || ldx < 0 || (dx && lddx < H) || !row_dtype(x_dtype) ||
+        !router || !nr || !xoff || T < 0 || H < 1 || H > kMaxRow || E < 1 || E > 1024 || K < 1 ||
+        K > 32 || KK < K || KK > kMaxSlots || ldx < 0 || (dx && lddx < H) || !row_dtype(x_dtype) ||
         (dx && !row_dtype(dx_dtype)) ||
         (score_fn != MVLLM_SCORE_SIGMOID && score_fn != MVLLM_SCORE_SQRT_SOFTPLUS) ||
-        int64_t(T) * KK > kMaxGrid)
+        int64_t(T) * KK > kMaxGrid ||
+        (int64_t(T) * K / kRgRows + E) * (H / kRgCols + 8) > kMaxGrid)
         return host_fail(MVLLM_ERR_INVALID, "route_grad_dev: invalid arguments");
     if (!workspace || workspace_bytes < mvllm_moe_route_grad_workspace(T, H, E, K))
         return host_fail(MVLLM_ERR_WORKSPACE, "route_grad_dev: workspace %zu < %zu",
@@ -308,6 +309,8 @@ int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t l
     DeviceScope dev;
     if (int rc = dev.enter())
         return rc;
+    if (T == 0 && !drouter)
+        return MVLLM_OK;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     RouteGradArgs a{};
     a.idx = idx, a.scores = scores, a.dwt = dwt, a.tok_pos = tok_pos, a.router = router;
@@ -327,7 +330,7 @@ int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t l
     a.arrived = reinterpret_cast<int *>(take(size_t(E) * ncol + 1));
     a.partial = take((slots / kRgRows + E) * H);
     const int counters = drouter ? E * ncol + 1 : 0;
-    const int warps = std::max(T, (counters + 31) / 32);
+    const unsigned warps = std::max(T, counters / 32 + 1);
     MVB_TRY(launch_serial(route_dz_kernel, dim3((warps + 7) / 8), dim3(256), 0, st, a, counters));
     if (T > 0 && dx) {
         const int rc = dx_dtype == MVLLM_DTYPE_F32

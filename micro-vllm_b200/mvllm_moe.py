@@ -719,6 +719,13 @@ def _flat(t, name, dtype, count):
     return t.data_ptr()
 
 
+def _grid(t, name, dtype, shape):
+    """Address of a contiguous device tensor of exactly this shape."""
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, {shape} is needed")
+    return _flat(t, name, dtype, 0)
+
+
 def _slots(tok_pos):
     if tok_pos.dim() != 2:
         raise ValueError(f"tok_pos: shape {tuple(tok_pos.shape)}, [T, K + n_shared] is needed")
@@ -780,10 +787,10 @@ def combine_dev(y, rw, tok_pos, out, accumulate=False, stream=None):
     cap, D = _matrix(y, "y")
     pi, ti, ldi = _rows(y, "y", cap, D)
     po, to, ldo = _rows(out, "out", T, D, out=True)
-    _check(lib().mvllm_moe_combine_dev(
-        _stream_at(stream, out), pi, ti, ldi, cap, _flat(rw, "rw", "torch.float32",
-                                                         min(cap, T * KK)),
-        pos, T, KK, D, po, to, ldo, int(bool(accumulate))))
+    weights = _flat(rw, "rw", "torch.float32", min(cap, T * KK))
+    _check(lib().mvllm_moe_combine_dev(_stream_at(stream, out), pi, ti, ldi,
+                                       min(cap, rw.numel()), weights, pos, T, KK, D, po, to, ldo,
+                                       int(bool(accumulate))))
 
 
 def combine_grad_dev(dout, y, rw, tok_pos, idx, dy, dwt, stream=None):
@@ -798,11 +805,11 @@ def combine_grad_dev(dout, y, rw, tok_pos, idx, dy, dwt, stream=None):
     po, to, ldo = _rows(dy, "dy", cap, D, out=True)
     if to != ti:
         raise ValueError("dy: the dtype of y is needed")
+    weights = _flat(rw, "rw", "torch.float32", min(cap, T * KK))
     _check(lib().mvllm_moe_combine_grad_dev(
-        _stream_at(stream, dout), pd, td, ldd, pi, ti, ldi, cap,
-        _flat(rw, "rw", "torch.float32", min(cap, T * KK)), pos,
-        _flat(idx, "idx", "torch.int32", T * K), T, K, KK, D, po, ldo,
-        _flat(dwt, "dwt", "torch.float32", T * K)))
+        _stream_at(stream, dout), pd, td, ldd, pi, ti, ldi, min(cap, rw.numel()), weights, pos,
+        _grid(idx, "idx", "torch.int32", (T, K)), T, K, KK, D, po, ldo,
+        _grid(dwt, "dwt", "torch.float32", (T, K))))
 
 
 def route_grad_workspace_bytes(T, H, E, K) -> int:
@@ -823,15 +830,19 @@ def route_grad_dev(x, router, idx, scores, dwt, nr, xoff, rows, tok_pos, dx, dro
     px, tx, ldx = _rows(x, "x", T, H)
     pd, td, ldd = (None, DTYPE_F32, 0) if dx is None else _rows(dx, "dx", T, H, out=True)
     if workspace is None:
-        workspace = torch.empty(route_grad_workspace_bytes(T, H, E, K), dtype=torch.uint8,
-                                device=x.device)
+        with torch.cuda.stream(stream):  # memory that stream alone uses
+            workspace = torch.empty(route_grad_workspace_bytes(T, H, E, K), dtype=torch.uint8,
+                                    device=x.device)
+    _on(workspace, "workspace")
+    if not workspace.is_contiguous():
+        raise ValueError("workspace: a contiguous tensor is needed")
     f32, i32 = "torch.float32", "torch.int32"
     _check(lib().mvllm_moe_route_grad_dev(
-        _stream_at(stream, x), px, tx, ldx, T, H, _flat(router, "router", f32, E * H), E, K,
-        _flat(idx, "idx", i32, T * K), _flat(scores, "scores", f32, T * E),
-        _flat(dwt, "dwt", f32, T * K), score_fn, routed_scale, _flat(nr, "nr", i32, E),
+        _stream_at(stream, x), px, tx, ldx, T, H, _grid(router, "router", f32, (E, H)), E, K,
+        _grid(idx, "idx", i32, (T, K)), _grid(scores, "scores", f32, (T, E)),
+        _grid(dwt, "dwt", f32, (T, K)), score_fn, routed_scale, _flat(nr, "nr", i32, E),
         _flat(xoff, "xoff", i32, E), _flat(rows, "rows", i32, T * K), pos, KK, pd, td, ldd,
-        None if drouter is None else _flat(drouter, "drouter", f32, E * H),
+        None if drouter is None else _grid(drouter, "drouter", f32, (E, H)),
         int(bool(accumulate)), _dp(workspace), workspace.numel() * workspace.element_size()))
 
 

@@ -170,3 +170,24 @@ def test_combine_form():
             at = [int(p["tok_pos"][t, j]) for j in range(K)
                   if idx[t, j] == idx[t, k] and p["tok_pos"][t, j] >= 0]
             assert torch.allclose(dw[t, k], dots[at[0]] if at else torch.tensor(0.0).double())
+
+
+def test_sizes_beyond_the_arithmetic_are_refused(lib):
+    big = (1 << 30) + 1
+    refused(lib, "mvllm_moe_dispatch_dev", [None, P, 1, 64, P, 4, 2, 64, P, 2 * big, 8],
+            [(7, big)])
+    refused(lib, "mvllm_moe_dispatch_grad_dev",
+            [None, P, 1, 64, 8, P, 4, 2, 64, P, 0, 2 * big, 0], [(8, big)])
+    refused(lib, "mvllm_moe_combine_dev", [None, P, 1, 64, 8, P, P, 4, 2, 64, P, 0, 2 * big, 0],
+            [(9, big)])
+    refused(lib, "mvllm_moe_combine_grad_dev",
+            [None, P, 1, 64, P, 1, 64, 8, P, P, P, 4, 2, 2, 64, P, 2 * big, P], [(14, big)])
+    refused(lib, "mvllm_moe_route_grad_dev",
+            [None, P, 1, 64, 4, 64, P, 8, 2, P, P, P, 0, 1.0, P, P, P, P, 2, P, 0, 2 * big, P, 0,
+             P, 1 << 20], [(5, big), (4, 1 << 30)])
+    for way in ("", "_grad"):
+        refused(lib, f"mvllm_matvec_q4{way}_dev",
+                [None, 4, P, 0, 64, P, P, 2, 64, 64, P, 0, 2 * big], [(7, big), (8, big), (9, big)])
+        refused(lib, f"mvllm_moe_matvec_q4{way}_dev",
+                [None, 7, 3, P, 0, 64, 8, P, P, P, P, 64, 64, P, 0, 2 * big],
+                [(6, big), (11, big), (12, big)])
