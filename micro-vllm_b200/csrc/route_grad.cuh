@@ -19,6 +19,8 @@
 
 #include "row_kernels.cuh"
 
+#include <type_traits>
+
 namespace mvb {
 
 struct RouteGradArgs {
@@ -28,18 +30,18 @@ struct RouteGradArgs {
     const int *tok_pos;  // [T, KK]
     const float *router; // [E, H]
     int T, K, KK, E, H, cap, score_fn, accumulate;
+    int block;      // sorted rows of a drouter item
+    int counters;   // of `arrived`; 0 where drouter is not asked for
     float scale;
-    float *dz;      // [T, K] the slots' dz
-    float *dzp;     // [cap] the sorted positions' dz
+    float *dzp;     // [cap] the sorted positions' dz, null likewise
     int *arrived;   // [E, column blocks] partial sums of an expert that are done,
                     // and one more: the drouter items taken
     float *partial; // [row blocks][H]
 };
 
 constexpr int kRgCols = 256; // columns of a drouter item
-constexpr int kRgRows = 128; // sorted rows of a drouter item
-constexpr int kRgSmem = 200 * 1024;
-constexpr int kRgWarps = 32; // of a dx CTA
+constexpr int kRgRows = 128; // sorted rows of a drouter item, at least
+constexpr int kRgThreads = 256; // of a dx CTA
 
 // dz of lane k's slot (K <= 32, one warp a token); 0 for lanes past K and ids
 // outside [0, E).
@@ -69,20 +71,10 @@ __device__ __forceinline__ float route_slot_grad(const RouteGradArgs &a, int64_t
     return (g - G) * w * slope;
 }
 
-// A warp per token: the slots' dz, and at the sorted position of each id their
-// sum (slots that repeat an id add to the first one's).  Clears the drouter
-// kernel's counters.
-__global__ void __launch_bounds__(256) route_dz_kernel(const RouteGradArgs a, int counters) {
-    pdl_wait();
-    pdl_trigger();
+// At the sorted position of each id the sum of its slots' dz (slots that
+// repeat an id add to the first one's), for drouter.
+__device__ __forceinline__ void route_put_grad(const RouteGradArgs &a, int64_t t, int e, float dz) {
     const int lane = threadIdx.x & 31;
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < counters; i += gridDim.x * blockDim.x)
-        a.arrived[i] = 0;
-    const int64_t t = blockIdx.x * int64_t(blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (t >= a.T)
-        return;
-    int e;
-    const float dz = route_slot_grad(a, t, e);
     float sum = 0.f;
     for (int k = 0; k < a.K; ++k) {
         const float dk = __shfl_sync(0xffffffffu, dz, k);
@@ -90,32 +82,56 @@ __global__ void __launch_bounds__(256) route_dz_kernel(const RouteGradArgs a, in
             sum += dk;
     }
     if (lane < a.K) {
-        a.dz[t * a.K + lane] = dz;
         const int p = a.tok_pos[t * a.KK + lane];
         if (p >= 0 && p < a.cap)
             a.dzp[p] = sum;
     }
 }
+// Clears the drouter kernel's counters.
+__device__ __forceinline__ void route_clear(const RouteGradArgs &a) {
+    for (int64_t i = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; i < a.counters;
+         i += int64_t(gridDim.x) * blockDim.x)
+        a.arrived[i] = 0;
+}
 
-// dx[t] = sum_k dz_k router[idx_k], each router row gathered from L2: a CTA
-// per token, for calls of fewer slots than experts.
+// What drouter needs, where dx is not asked for: a warp per token.
+__global__ void __launch_bounds__(256) route_dz_kernel(const RouteGradArgs a) {
+    pdl_wait();
+    pdl_trigger();
+    route_clear(a);
+    const int64_t t = blockIdx.x * int64_t(blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (t >= a.T)
+        return;
+    int e;
+    const float dz = route_slot_grad(a, t, e);
+    route_put_grad(a, t, e, dz);
+}
+
+// dx[t] = sum_k dz_k router[idx_k], the router's rows gathered from L2: a CTA
+// takes (token, segment of the row).  Bound by L2, 4 T K H bytes at about 20
+// TB/s.  (A form with some columns of every expert in shared memory, which the
+// CTA's tokens then read, took 25 to 60% longer up to 64 slots per expert and
+// was never more than 7% ahead.)
 template <typename TO, int N>
-__global__ void __launch_bounds__(256)
-    route_dx_gather_kernel(const RouteGradArgs a, TO *__restrict__ dx, int64_t lddx) {
+__global__ void __launch_bounds__(kRgThreads)
+    route_dx_kernel(const RouteGradArgs a, int nseg, int seg, TO *__restrict__ dx, int64_t lddx) {
     pdl_wait();
     pdl_trigger();
     __shared__ float sdz[32];
     __shared__ int se[32];
-    const int64_t t = blockIdx.x;
+    const int64_t t = blockIdx.x / nseg;
+    const int part = static_cast<int>(blockIdx.x % nseg);
+    const int s0 = part * seg, s1 = min(a.H, s0 + seg);
     if (threadIdx.x < 32) {
-        int e = -1;
-        if (int(threadIdx.x) < a.K)
-            e = a.idx[t * a.K + threadIdx.x];
-        sdz[threadIdx.x] = e >= 0 && e < a.E ? a.dz[t * a.K + threadIdx.x] : 0.f;
-        se[threadIdx.x] = e >= a.E ? -1 : e;
+        int e;
+        const float dz = route_slot_grad(a, t, e);
+        sdz[threadIdx.x] = dz, se[threadIdx.x] = e;
+        if (part == 0 && a.dzp)
+            route_put_grad(a, t, e, dz);
     }
+    route_clear(a);
     __syncthreads();
-    for (int c = threadIdx.x * N; c < a.H; c += blockDim.x * N) {
+    for (int c = s0 + threadIdx.x * N; c < s1; c += kRgThreads * N) {
         float acc[N] = {};
         if (a.accumulate)
             load_row<N>(dx + t * lddx + c, acc);
@@ -133,140 +149,13 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// The same with the router's columns in shared memory.  Gathered from L2 the
-// rows are 4 T K H bytes (1.9 GB for 8192 tokens of 8 out of 384 experts, H
-// 7168), which L2 serves at about half of what shared memory does; so a CTA
-// keeps LPT * 4 columns of every expert (and a row of zeros for slots without
-// one) and goes through tokens, LPT lanes each.  The (column block, token) plane is cut evenly over the
-// CTAs, column blocks outermost.
-template <typename TO, int LPT>
-__global__ void __launch_bounds__(32 * kRgWarps)
-    route_dx_tile_kernel(const RouteGradArgs a, TO *__restrict__ dx, int64_t lddx, int vec) {
-    extern __shared__ __align__(16) float rg_tile[];
-    __shared__ __align__(16) int2 pairs[kRgWarps][2][32]; // (row of the tile, dz) of a warp's slots
-    constexpr int COLS = LPT * 4, TPW = 32 / LPT; // tokens a warp has at a time
-    pdl_wait();
-    pdl_trigger();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int sub = lane / LPT, col4 = (lane % LPT) * 4;
-    const int blocks = (a.H + COLS - 1) / COLS;
-    const int64_t plane = int64_t(blocks) * a.T;
-    int64_t at = plane * blockIdx.x / gridDim.x;
-    const int64_t end = plane * (blockIdx.x + 1) / gridDim.x;
-    while (at < end) {
-        const int b = int(at / a.T), c0 = b * COLS;
-        const int t0 = int(at - int64_t(b) * a.T);
-        const int t1 = int(min(int64_t(a.T), t0 + end - at));
-        __syncthreads(); // the last block's readers are done
-        for (int i = threadIdx.x; i < (a.E + 1) * LPT; i += blockDim.x) {
-            const int e = i / LPT, c = (i - e * LPT) * 4;
-            const float *src = a.router + int64_t(e) * a.H + c0 + c;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (e == a.E) {
-                // zeros
-            } else if (vec && c0 + c + 4 <= a.H) {
-                v = *reinterpret_cast<const float4 *>(src);
-            } else {
-                if (c0 + c < a.H)
-                    v.x = src[0];
-                if (c0 + c + 1 < a.H)
-                    v.y = src[1];
-                if (c0 + c + 2 < a.H)
-                    v.z = src[2];
-                if (c0 + c + 3 < a.H)
-                    v.w = src[3];
-            }
-            *reinterpret_cast<float4 *>(rg_tile + e * COLS + c) = v;
-        }
-        __syncthreads();
-        // A group of LPT lanes takes BT tokens at a time, their slots' ids and dz
-        // by lane, the next batch's loaded before this one is worked off.
-        const int bt = max(1, LPT / a.K), lk = lane % LPT;
-        const int stride = kRgWarps * TPW * bt;
-        auto fetch = [&](int t, int k0) { // slots k0.. of tokens t..
-            int e = a.E;
-            float dz = 0.f;
-            const int tt = t + (a.K <= LPT ? lk / a.K : 0), k = a.K <= LPT ? lk % a.K : k0 + lk;
-            if (tt < min(t1, t + bt) && k < a.K) {
-                e = a.idx[int64_t(tt) * a.K + k];
-                dz = a.dz[int64_t(tt) * a.K + k];
-                if (e < 0 || e >= a.E)
-                    e = a.E, dz = 0.f;
-            }
-            return make_int2(e * COLS, __float_as_int(dz));
-        };
-        const int c = c0 + col4;
-        const bool whole = vec && c + 4 <= a.H;
-        auto old = [&](int64_t t, float (&acc)[4]) {
-            if (whole) {
-                load_row<4>(dx + t * lddx + c, acc);
-                return;
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float o[1] = {0.f};
-                if (c + q < a.H)
-                    load_row<1>(dx + t * lddx + c + q, o);
-                acc[q] = o[0];
-            }
-        };
-        int tb = t0 + (warp * TPW + sub) * bt;
-        int2 next = fetch(tb, 0);
-        const int rounds = (t1 - t0 + stride - 1) / stride; // the same for every lane
-        for (int i = 0; i < rounds; ++i, tb += stride) {
-            // Two buffers: the last round's readers may still be at theirs.
-            const int2 *slots = pairs[warp][i & 1] + sub * LPT;
-            pairs[warp][i & 1][lane] = next;
-            __syncwarp();
-            next = fetch(tb + stride, 0);
-            for (int s = 0; s < bt; ++s) {
-                const int t = tb + s;
-                const bool live = t < t1;
-                float acc[4] = {};
-                if (live && a.accumulate)
-                    old(t, acc);
-                for (int k0 = 0; k0 < a.K; k0 += LPT) {
-                    if (k0 > 0) { // more slots than lanes: bt is 1
-                        __syncwarp();
-                        pairs[warp][i & 1][lane] = fetch(tb, k0);
-                        __syncwarp();
-                    }
-                    const int n = min(LPT, a.K - k0);
-#pragma unroll 8
-                    for (int j = 0; j < n; ++j) {
-                        const int2 p = slots[s * a.K + j];
-                        const float4 v =
-                            *reinterpret_cast<const float4 *>(rg_tile + p.x + col4);
-                        const float dj = __int_as_float(p.y);
-                        acc[0] = fmaf(dj, v.x, acc[0]), acc[1] = fmaf(dj, v.y, acc[1]);
-                        acc[2] = fmaf(dj, v.z, acc[2]), acc[3] = fmaf(dj, v.w, acc[3]);
-                    }
-                }
-                if (live) {
-                    if (whole) {
-                        store_row<4>(dx + t * lddx + c, acc);
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const float o[1] = {acc[q]};
-                            if (c + q < a.H)
-                                store_row<1>(dx + t * lddx + c + q, o);
-                        }
-                    }
-                }
-            }
-        }
-        at += t1 - t0;
-    }
-}
-
 // drouter[e] = sum over e's sorted rows of dz x[rows].  An item is (a block of
-// kRgCols columns, an expert, kRgRows of its rows); each warp takes the next
+// kRgCols columns, an expert, `block` of its rows); each warp takes the next
 // one, and has eight (f32: four) rows' loads under way.  Items run by groups of
 // eight column blocks, so the columns of x that all experts gather from (16 T
 // kRgCols bytes in bf16) stay in L2.  An expert of several items leaves its
 // partial sums in the workspace, and the warp that arrives last adds them in
-// order; one without rows gets zeros.
+// order; one without rows gets zeros.  Bound by the latency of the gathers.
 template <typename TX>
 __global__ void __launch_bounds__(256)
     route_dw_kernel(const RouteGradArgs a, const TX *__restrict__ x, int64_t ldx, int vec,
@@ -283,7 +172,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int e = 4 * int(threadIdx.x) + k;
-        n4[k] = e < a.E ? max(1, (min(nr[e], a.cap) + kRgRows - 1) / kRgRows) : 0;
+        n4[k] = e < a.E ? max(1, (min(nr[e], a.cap) + a.block - 1) / a.block) : 0;
         v += n4[k];
     }
     int before = -v;
@@ -309,7 +198,7 @@ __global__ void __launch_bounds__(256)
     }
     __syncthreads();
     // (No more than the workspace holds, whatever nr says.)
-    const int blocks = min(first[a.E], a.cap / kRgRows + a.E);
+    const int blocks = min(first[a.E], a.cap / a.block + a.E);
     const int ncol = (a.H + kRgCols - 1) / kRgCols, groups = (ncol + 7) / 8;
     const int total = blocks * groups * 8;
     for (;;) { // a warp at a time: items differ in rows by a hundredfold
@@ -333,7 +222,7 @@ __global__ void __launch_bounds__(256)
         }
         const int e = lo, rb = slot - first[e], nblk = first[e + 1] - first[e];
         const int off = xoff[e], n = min(nr[e], a.cap);
-        const int p0 = off + rb * kRgRows, p1 = min(min(off + n, p0 + kRgRows), a.cap);
+        const int p0 = off + rb * a.block, p1 = min(min(off + n, p0 + a.block), a.cap);
         const int c = cb * kRgCols + lane * 8;
         const bool inside = vec && (cb + 1) * kRgCols <= a.H;
         float acc[8] = {};
@@ -357,6 +246,8 @@ __global__ void __launch_bounds__(256)
             const float dz = dz_next;
             slots(pb + 32, t_next, dz_next);
             const int cnt = min(32, p1 - pb);
+            const uint32_t odd = __ballot_sync(0xffffffffu, t < 0);
+            const int whole = odd ? __ffs(odd) - 1 : 32; // rows that count, from the first on
             for (int j0 = 0; j0 < cnt; j0 += B) {
                 Raw8<TX> xv[B];
                 int tj[B];
@@ -375,14 +266,22 @@ __global__ void __launch_bounds__(256)
                     for (int j = 0; j < B; ++j)
                         xv[j].load(x + max(tj[j], 0) * ldx, min(c, a.H), a.H, vec);
                 }
+                auto add = [&](auto some) { // `some` of them may not count
 #pragma unroll
-                for (int j = 0; j < B; ++j) {
-                    float f[8];
-                    xv[j].get(f);
+                    for (int j = 0; j < B; ++j) {
+                        if (some.value && tj[j] < 0)
+                            continue;
+                        float f[8];
+                        xv[j].get(f);
 #pragma unroll
-                    for (int s = 0; s < 8; ++s)
-                        acc[s] = tj[j] >= 0 ? fmaf(dj[j], f[s], acc[s]) : acc[s];
-                }
+                        for (int s = 0; s < 8; s += 2)
+                            ffma2(acc[s], acc[s + 1], f[s], f[s + 1], dj[j]);
+                    }
+                };
+                if (j0 + B <= whole)
+                    add(std::false_type{});
+                else
+                    add(std::true_type{});
             }
         }
         float *out = drouter + int64_t(e) * a.H + c;

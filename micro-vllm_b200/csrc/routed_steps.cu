@@ -29,13 +29,13 @@ int row_vec(unsigned align, size_t bytes) {
 constexpr int64_t kMaxGrid = 0x7fffffff;
 constexpr int kMaxRow = 1 << 30; // elements of a row: steps past its end stay in 32 bits
 
-// Segments of a row of `words` lane-words for T tokens: as few as fill the
-// device with warps (32 per SM), each a multiple of `piece` words.
+// Segments of a row of `total` lane-words for T tokens: as few as give `wanted`
+// of them in all, each a multiple of `piece` words.
 struct Segments {
     int n, words;
-    Segments(int T, int total, int piece, int sms) {
+    Segments(int T, int total, int piece, int wanted) {
         const int most = (total + piece - 1) / piece;
-        const int64_t want = (int64_t(sms) * 32 + T - 1) / T;
+        const int64_t want = (int64_t(wanted) + T - 1) / T;
         n = int(std::max<int64_t>(1, std::min<int64_t>(most, want)));
         words = (most + n - 1) / n * piece;
         n = (total + words - 1) / words;
@@ -50,7 +50,8 @@ int mvllm_moe_dispatch_dev(void *stream, const void *x, int dtype, int64_t ldx,
                            const int *tok_pos, int T, int KK, int D, void *xs, int64_t ldxs,
                            int rows_cap) {
     if ((T > 0 && (!x || !tok_pos || (!xs && rows_cap > 0))) || T < 0 || KK < 1 ||
-        KK > kMaxSlots || D < 1 || D > kMaxRow || ldx < 0 || ldxs < D || rows_cap < 0 || !row_dtype(dtype))
+        KK > kMaxSlots || D < 1 || D > kMaxRow || ldx < 0 || ldxs < D || rows_cap < 0 ||
+        !row_dtype(dtype))
         return host_fail(MVLLM_ERR_INVALID, "dispatch_dev: invalid arguments");
     DeviceScope dev;
     if (int rc = dev.enter())
@@ -59,22 +60,24 @@ int mvllm_moe_dispatch_dev(void *stream, const void *x, int dtype, int64_t ldx,
         return MVLLM_OK;
     const unsigned al = std::min(row_align(x, ldx, D, dtype), row_align(xs, ldxs, D, dtype));
     const int64_t b = dtype_bytes(dtype), w = al >= 16 ? 16 : al >= 4 ? 4 : 2;
-    const int words = int(D * b / w);
-    const Segments s(T, words, 32, dev.sms);
-    const int64_t units = int64_t(T) * s.n, grid = (units + 7) / 8;
+    // A lane's words: one of 16 bytes, four narrower ones (4096 tokens to 8
+    // positions each, 2051 bf16: 32 us, 74 by one).
+    const int words = int(D * b / w), piece = w == 16 ? 32 : 128;
+    const int pieces = (words + piece - 1) / piece;
+    const int64_t units = int64_t(T) * pieces, grid = (units + 7) / 8;
     if (grid > kMaxGrid)
         return host_fail(MVLLM_ERR_INVALID, "dispatch_dev: T too large");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define MVB_DISPATCH(W)                                                                        \
-    MVB_TRY(launch_serial(dispatch_rows_kernel<W>, dim3(unsigned(grid)), dim3(256), 0, st,     \
-                          static_cast<const W *>(x), ldx *b / w, tok_pos, units, s.n,          \
-                          s.words, KK, words, static_cast<W *>(xs), ldxs *b / w, rows_cap))
+#define MVB_DISPATCH(W, Q)                                                                     \
+    MVB_TRY(launch_serial(dispatch_rows_kernel<W, Q>, dim3(unsigned(grid)), dim3(256), 0, st,  \
+                          static_cast<const W *>(x), ldx *b / w, tok_pos, units, pieces, KK,   \
+                          words, static_cast<W *>(xs), ldxs *b / w, rows_cap))
     if (w == 16)
-        MVB_DISPATCH(uint4);
+        MVB_DISPATCH(uint4, 1);
     else if (w == 4)
-        MVB_DISPATCH(uint32_t);
+        MVB_DISPATCH(uint32_t, 4);
     else
-        MVB_DISPATCH(uint16_t);
+        MVB_DISPATCH(uint16_t, 4);
 #undef MVB_DISPATCH
     return MVLLM_OK;
 }
@@ -87,7 +90,9 @@ template <typename TY, typename TO>
 int combine_launch(cudaStream_t st, int sms, int n, const TY *y, int64_t ldy, int cap, const float *rw,
                    const int *tok_pos, int T, int KK, int D, TO *out, int64_t ldo,
                    int accumulate) {
-    const Segments s(T, (D + n - 1) / n, 32, sms);
+    // 64 warps per SM: whole rows leave 64 tokens of 8 rows of 7168 bf16 at 30 us
+    // in place of 4.0; the finest cut costs 4096 tokens 93 in place of 85.
+    const Segments s(T, (D + n - 1) / n, 32, sms * 64);
     const int64_t units = int64_t(T) * s.n, grid = (units + 7) / 8;
     if (grid > kMaxGrid)
         return host_fail(MVLLM_ERR_INVALID, "combine: T too large");
@@ -109,7 +114,8 @@ int combine_any(const char *who, void *stream, const void *y, int y_dtype, int64
                 const float *rw, const int *tok_pos, int T, int KK, int D, void *out,
                 int out_dtype, int64_t ldo, int accumulate) {
     if ((T > 0 && ((!y && cap > 0) || !tok_pos || !out)) || T < 0 || KK < 1 || KK > kMaxSlots ||
-        D < 1 || D > kMaxRow || ldy < 0 || ldo < D || cap < 0 || !row_dtype(y_dtype) || !row_dtype(out_dtype))
+        D < 1 || D > kMaxRow || ldy < 0 || ldo < D || cap < 0 || !row_dtype(y_dtype) ||
+        !row_dtype(out_dtype))
         return host_fail(MVLLM_ERR_INVALID, "%s: invalid arguments", who);
     DeviceScope dev;
     if (int rc = dev.enter())
@@ -228,37 +234,19 @@ int route_dx(cudaStream_t st, const RouteGradArgs &a, int sms, TO *dx, int64_t l
     const int type = sizeof(TO) == 4 ? MVLLM_DTYPE_F32 : MVLLM_DTYPE_BF16;
     const bool vec = std::min(row_align(a.router, a.H, a.H, MVLLM_DTYPE_F32), 16u) == 16 &&
                      row_align(dx, lddx, a.H, type) >= 4 * sizeof(TO);
-    // Fewer slots than experts: loading every expert's columns once costs more
-    // than gathering the slots' rows.
-    if (int64_t(a.T) * a.K < 2 * a.E) {
-        if (vec)
-            MVB_TRY(launch_serial(route_dx_gather_kernel<TO, 4>, dim3(a.T), dim3(256), 0, st, a, dx,
-                                  lddx));
-        else
-            MVB_TRY(launch_serial(route_dx_gather_kernel<TO, 1>, dim3(a.T), dim3(256), 0, st, a, dx,
-                                  lddx));
-        return MVLLM_OK;
-    }
-    // The widest column block whose experts fit shared memory.
-    const int lpt = (a.E + 1) * 512 <= kRgSmem ? 32 : (a.E + 1) * 256 <= kRgSmem ? 16 : 8;
-    const int smem = (a.E + 1) * lpt * 16;
-    const int64_t work = int64_t((a.H + 4 * lpt - 1) / (4 * lpt)) * a.T;
-    const int per_sm = std::max(1, std::min(64 / kRgWarps, kRgSmem / smem));
-    const unsigned grid = unsigned(std::min<int64_t>(int64_t(sms) * per_sm, (work + 15) / 16));
-#define MVB_DX(L)                                                                              \
-    do {                                                                                       \
-        MVB_TRY(cudaFuncSetAttribute(route_dx_tile_kernel<TO, L>,                              \
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize, kRgSmem));   \
-        MVB_TRY(launch_serial(route_dx_tile_kernel<TO, L>, dim3(grid), dim3(32 * kRgWarps), smem, st, a, \
-                              dx, lddx, int(vec)));                                            \
-    } while (0)
-    if (lpt == 32)
-        MVB_DX(32);
-    else if (lpt == 16)
-        MVB_DX(16);
+    const int n = vec ? 4 : 1;
+    // As few segments as make four CTAs per SM: 48 tokens of H 7168 take 5.9 us
+    // in place of 17.8 in one segment each.
+    const Segments s(a.T, a.H / n, kRgThreads, sms * 4);
+    const int64_t grid = int64_t(a.T) * s.n;
+    if (grid > kMaxGrid)
+        return host_fail(MVLLM_ERR_INVALID, "route_grad_dev: T too large");
+    if (vec)
+        MVB_TRY(launch_serial(route_dx_kernel<TO, 4>, dim3(unsigned(grid)), dim3(kRgThreads), 0, st,
+                              a, s.n, s.words * n, dx, lddx));
     else
-        MVB_DX(8);
-#undef MVB_DX
+        MVB_TRY(launch_serial(route_dx_kernel<TO, 1>, dim3(unsigned(grid)), dim3(kRgThreads), 0, st,
+                              a, s.n, s.words * n, dx, lddx));
     return MVLLM_OK;
 }
 
@@ -283,9 +271,9 @@ size_t mvllm_moe_route_grad_workspace(int T, int H, int E, int K) {
     if (T < 0 || H < 1 || E < 1 || K < 1)
         return 0;
     const size_t slots = size_t(T) * K, ncol = (size_t(H) + kRgCols - 1) / kRgCols;
-    // dz by slot and by position, counters, partial sums of each row block, all
-    // on 256-byte boundaries
-    return (2 * slots + E * ncol + 1 + (slots / kRgRows + E) * H) * sizeof(float) + 5 * 256;
+    // dz by position, counters, partial sums of each row block, all on 256-byte
+    // boundaries
+    return (slots + E * ncol + 1 + (slots / kRgRows + E) * H) * sizeof(float) + 4 * 256;
 }
 
 int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t ldx, int T, int H,
@@ -325,19 +313,26 @@ int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t l
         at += n * sizeof(float);
         return p;
     };
-    a.dz = take(slots);
-    a.dzp = take(slots);
-    a.arrived = reinterpret_cast<int *>(take(size_t(E) * ncol + 1));
-    a.partial = take((slots / kRgRows + E) * H);
-    const int counters = drouter ? E * ncol + 1 : 0;
-    const unsigned warps = std::max(T, counters / 32 + 1);
-    MVB_TRY(launch_serial(route_dz_kernel, dim3((warps + 7) / 8), dim3(256), 0, st, a, counters));
-    if (T > 0 && dx) {
+    if (drouter) {
+        a.dzp = take(slots);
+        a.arrived = reinterpret_cast<int *>(take(size_t(E) * ncol + 1));
+        a.partial = take((slots / kRgRows + E) * H);
+        a.counters = E * ncol + 1;
+        // Long row blocks leave fewer partial sums, short ones more items to
+        // share: 256 rows where that makes 14 items per SM, else 128.  (65536
+        // slots of 384 experts, H 7168: 105 us by 256, 124 by 128; 32768 of
+        // 64, H 2048: 40 and 28; 512 rows cost uneven experts 12 us more.)
+        a.block = int64_t(slots / (2 * kRgRows)) * ncol >= 14 * dev.sms ? 2 * kRgRows : kRgRows;
+    }
+    if (T > 0 && dx) { // dz on the way
         const int rc = dx_dtype == MVLLM_DTYPE_F32
                            ? route_dx(st, a, dev.sms, static_cast<float *>(dx), lddx)
                            : route_dx(st, a, dev.sms, static_cast<__nv_bfloat16 *>(dx), lddx);
         if (rc)
             return rc;
+    } else {
+        const unsigned warps = std::max(T, a.counters / 32 + 1);
+        MVB_TRY(launch_serial(route_dz_kernel, dim3((warps + 7) / 8), dim3(256), 0, st, a));
     }
     if (drouter) {
         const int rc =

@@ -193,14 +193,15 @@ struct WarpSlots {
     }
 };
 
-// dispatch: a warp takes (token, segment of the row), loads 128 words at a time
-// and stores them at each of the token's positions: a copy of the bits, so W
-// is only the widest word (16, 4 or 2 bytes) that rows, pitches and addresses
-// are multiples of.  ldx, ldxs, seg and D count words.
-template <typename W>
+// dispatch: a warp takes (token, piece of the row), loads Q words a lane and
+// stores them at each of the token's positions: a copy of the bits, so W is
+// only the widest word (16, 4 or 2 bytes) that rows, pitches and addresses are
+// multiples of.  ldx, ldxs and D count words.  Bound by memory: 4096 tokens to
+// 8 positions each, 7168 bf16, 6.1 TB/s.
+template <typename W, int Q>
 __global__ void __launch_bounds__(256)
     dispatch_rows_kernel(const W *__restrict__ x, int64_t ldx, const int *__restrict__ tok_pos,
-                         int64_t units, int nseg, int seg, int KK, int D, W *__restrict__ xs,
+                         int64_t units, int pieces, int KK, int D, W *__restrict__ xs,
                          int64_t ldxs, int cap) {
     pdl_wait();
     pdl_trigger();
@@ -208,32 +209,30 @@ __global__ void __launch_bounds__(256)
     const int64_t unit = blockIdx.x * int64_t(blockDim.x >> 5) + (threadIdx.x >> 5);
     if (unit >= units)
         return;
-    const int64_t t = unit / nseg;
-    const int s0 = static_cast<int>(unit - t * nseg) * seg, s1 = min(D, s0 + seg);
+    const int64_t t = unit / pieces;
+    const int col = static_cast<int>(unit - t * pieces) * 32 * Q + lane;
     WarpSlots sl;
     sl.load(tok_pos, t, KK, cap);
     const uint32_t m0 = __ballot_sync(0xffffffffu, sl.p0 >= 0);
     const uint32_t m1 = __ballot_sync(0xffffffffu, sl.p1 >= 0);
     if (!(m0 | m1))
         return;
-    for (int col = s0; col < s1; col += 128) {
-        W v[4];
+    W v[Q];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (col + 32 * q + lane < s1)
-                v[q] = x[t * ldx + col + 32 * q + lane];
-        auto copy = [&](int64_t p) {
-            W *to = xs + p * ldxs + col + lane;
+    for (int q = 0; q < Q; ++q)
+        if (col + 32 * q < D)
+            v[q] = x[t * ldx + col + 32 * q];
+    auto copy = [&](int64_t p) {
+        W *to = xs + p * ldxs + col;
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (col + 32 * q + lane < s1)
-                    to[32 * q] = v[q];
-        };
-        for (uint32_t m = m0; m; m &= m - 1)
-            copy(__shfl_sync(0xffffffffu, sl.p0, __ffs(m) - 1));
-        for (uint32_t m = m1; m; m &= m - 1)
-            copy(__shfl_sync(0xffffffffu, sl.p1, __ffs(m) - 1));
-    }
+        for (int q = 0; q < Q; ++q)
+            if (col + 32 * q < D)
+                to[32 * q] = v[q];
+    };
+    for (uint32_t m = m0; m; m &= m - 1)
+        copy(__shfl_sync(0xffffffffu, sl.p0, __ffs(m) - 1));
+    for (uint32_t m = m1; m; m &= m - 1)
+        copy(__shfl_sync(0xffffffffu, sl.p1, __ffs(m) - 1));
 }
 
 // combine and the dispatch gradient: out[t] = (out[t] +) sum of rw[p] y[p]
@@ -270,16 +269,23 @@ __global__ void __launch_bounds__(256)
             sw[warp][j] = rw ? rw[spos[warp][j]] : 1.f;
     }
     __syncwarp();
-    const TY *row[B]; // of the batch's positions; most tokens have one batch
-    float w[B];
-    auto batch = [&](int j0) {
+    // Narrow vectors, whose many steps repeat the address arithmetic, keep the
+    // first batch's rows and weights in registers; for 16-byte vectors those
+    // registers cost more (109 against 91 us on 4096 tokens of 8 rows of 7168
+    // bf16 summed into f32).
+    constexpr bool HELD = N * sizeof(TY) < 16;
+    const TY *row[HELD ? B : 1];
+    float w[HELD ? B : 1];
+    auto hold = [&](int j0) {
+        if constexpr (HELD) {
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
-            row[b] = y + int64_t(spos[warp][j0 + b]) * ldy;
-            w[b] = sw[warp][j0 + b];
+            for (int b = 0; b < B; ++b) {
+                row[b] = y + int64_t(spos[warp][j0 + b]) * ldy;
+                w[b] = sw[warp][j0 + b];
+            }
         }
     };
-    batch(0);
+    hold(0);
     for (int c = s0 + lane * N; c < s1; c += 32 * N) {
         float acc[N];
         if (accumulate)
@@ -289,22 +295,29 @@ __global__ void __launch_bounds__(256)
             for (int q = 0; q < N; ++q)
                 acc[q] = 0.f;
         for (int j0 = 0; j0 < n; j0 += B) {
-            // (Sixteen-byte vectors look their rows up again: the registers of
-            // the addresses cost more than that, 99 against 92 us on 4096
-            // tokens of 8 rows of 7168 bf16.)
-            if (n > B || N * sizeof(TY) >= 16)
-                batch(j0);
+            if (n > B)
+                hold(j0);
             RowVec<TY, N> v[B];
 #pragma unroll
-            for (int b = 0; b < B; ++b)
-                v[b].load(row[b] + c);
+            for (int b = 0; b < B; ++b) {
+                if constexpr (HELD)
+                    v[b].load(row[b] + c);
+                else
+                    v[b].load(y + int64_t(spos[warp][j0 + b]) * ldy + c);
+            }
 #pragma unroll
             for (int b = 0; b < B; ++b) {
                 float f[N];
                 v[b].get(f);
+                if constexpr (HELD) {
 #pragma unroll
-                for (int q = 0; q < N; ++q)
-                    acc[q] = j0 + b < n ? fmaf(w[b], f[q], acc[q]) : acc[q];
+                    for (int q = 0; q < N; ++q)
+                        acc[q] = j0 + b < n ? fmaf(w[b], f[q], acc[q]) : acc[q];
+                } else if (j0 + b < n) {
+#pragma unroll
+                    for (int q = 0; q < N; ++q)
+                        acc[q] = fmaf(sw[warp][j0 + b], f[q], acc[q]);
+                }
             }
         }
         store_row<N>(out + t * ldo + c, acc);
