@@ -4,7 +4,6 @@
 
 #include <algorithm>
 #include <array>
-#include <atomic>
 #include <cmath>
 #include <map>
 #include <mutex>
@@ -42,6 +41,31 @@ int max_clusters(const void *kern, int threads, int ranks, int smem, int device,
     return MVLLM_OK;
 }
 
+// Passes over nb matrices for `rows` rows, rp a pass: experts' rows are taken
+// to be Poisson distributed, an expert's passes being the k >= 0 with more
+// than k rp rows.
+double expected_passes(int rows, int nb, int rp) {
+    if (nb == 1)
+        return (rows + rp - 1) / rp;
+    const double mean = double(rows) / nb;
+    double p = std::exp(-mean), below = 0.0, passes = 0.0;
+    if (p < 1e-200)
+        return nb * (mean / rp + 0.5);
+    for (int k = 0, n = 0; below < 0.999 && n < rows; ++k) {
+        for (; n <= k * rp; ++n) // below: at most k rp rows
+            below += p, p *= mean / (n + 1);
+        passes += std::max(0.0, 1.0 - below);
+    }
+    return std::min<double>(rows, std::max(1.0, nb * passes));
+}
+
+// A plan, its launch and the rule's estimate of its time.
+struct MvCut {
+    MatvecPlan p{};
+    int ranks = 1, grid = 1;
+    double ns = 1e30;
+};
+
 template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
     using F = MvFormat<FMT>;
     static constexpr int T = MvTerms<FMT, TX, GRAD, FINE>::T, RP = 8 * NT / T;
@@ -70,17 +94,28 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
     }
 
     // How the work is cut.  The candidates are clusters of 1, 2, 4 or 8 CTAs
-    // along the reduction, ranges of wo tiles and wk parts of each; the rule
-    // estimates each one's time: the stages that a CTA's warps take one after
-    // another at the rate of its share of the memory or of what its warps
-    // dequantise, a fixed cost per unit, the rounds that the units need, and
-    // the rows it stages.
-    static int plan(const void *kern, MatvecPlan &p, int rows_each, int items, int nb,
-                    const DeviceScope &dev, int *ranks, int *grid) {
+    // along the reduction, ranges of wo tiles and wk parts of each.  The rule
+    // estimates each one's time: the rounds that its units need, in each the
+    // stages that a CTA's warps take one after another, at the rate of its
+    // share of the memory or of what its warps dequantise, and the unit's own
+    // cost, with the partial sums it adds up; and the rows that are staged.
+    // The constants (ns, bytes and elements per ns of a CTA) were fitted to 272
+    // measured shapes of both formats and directions, 1 to 1024 rows: its answer
+    // is 3% slower than the best of about 60 cuts of each on average.  (Rows
+    // staged at 20 elements per ns and 1500 ns a unit, first guesses, left 11%
+    // and up to twice the time.)
+    static int plan(MvCut &cut, int nb, const DeviceScope &dev) {
+        MatvecPlan &p = cut.p;
+        const double items = expected_passes(p.rows_most, nb, RP);
         const int tiles = (p.N + TILE - 1) / TILE, steps = (p.K + STEP - 1) / STEP;
-        const double compute = (GRAD ? 26.0 : 40.0) / (1.0 + 0.25 * (NT - 1)); // B/ns of a CTA
+        const double compute = // of a CTA's warps
+            GRAD ? (NT == 1 ? 25.0 : 21.0) : NT == 1 ? 42.0 : NT == 2 ? 28.0 : 17.0;
+        const double fill = GRAD ? 1.05 : 0.58;        // of its warps that reach it
+        const double latency = GRAD ? 1200.0 : 580.0;  // of a stage, at least
+        const double staging = GRAD ? (sizeof(TX) == 4 ? 2.9 : 13.0)
+                                    : (sizeof(TX) == 4 ? 4.1 : 7.8);
+        const double rows_most = std::min<double>(RP, (p.rows_most + nb - 1) / nb);
         const int most = GRAD ? WARPS : 64;
-        double best = 1e30;
         MatvecPlan q = p;
         for (int c = 1; c <= 8; c *= 2) {
             const int slice = (steps + c - 1) / c;
@@ -88,7 +123,7 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
                 break;
             int nc = dev.sms;
             if (c > 1)
-                if (int rc = max_clusters(kern, THREADS, c, kMvSmem, dev.device, &nc))
+                if (int rc = max_clusters(kernel(), THREADS, c, kMvSmem, dev.device, &nc))
                     return rc;
             for (int wo = 1; wo <= std::min(most, tiles); ++wo) {
                 for (int wk = 1; wo * wk <= most && wk <= slice && wk <= WARPS; ++wk) {
@@ -101,29 +136,32 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
                     const int tasks = wo * wk, active = std::min(tasks, WARPS);
                     const int serial = (tasks + WARPS - 1) / WARPS * ((slice + wk - 1) / wk);
                     const int nr = (tiles + wo - 1) / wo;
-                    const double units = double(items) * nr, busy = std::min<double>(units, nc);
+                    const double units = items * nr, busy = std::min<double>(units, nc);
                     const double rounds = std::ceil(units / nc);
                     const double chunks = (slice + chunk - 1) / chunk;
-                    // fewer warps than three quarters: the CTA is slower itself
-                    const double rate = std::min(compute * std::min(1.0, active / (0.75 * WARPS)),
-                                                 6000.0 / (busy * c));
-                    const double stage = std::max(active * F::STAGE / rate, 400.0);
-                    // rows are staged once per matrix, or, in chunks, for every
-                    // unit with nothing else under way
-                    const double rows = std::min<double>(RP, rows_each) * slice * STEP / 20.0;
-                    const double stagings = chunks > 1 ? rounds : std::ceil(items / double(nc));
-                    const double t = rounds * (serial * stage + 1500.0 + 5000.0 * (chunks - 1) +
-                                               (c > 1 ? 500.0 : 0.0)) +
-                                     stagings * (rows + 500.0);
-                    if (t < best) {
-                        best = t;
+                    const double rate = std::min(
+                        compute * std::min(1.0, active / (fill * WARPS)), 6000.0 / (busy * c));
+                    const double stage = std::max(active * F::STAGE / rate, latency);
+                    const double sums = wo * TILE * rows_most;
+                    const double unit =
+                        GRAD ? 750.0 + sums * (0.09 * wk * T + 0.39) + (c > 1 ? 650.0 : 0.0)
+                             : 2800.0 + sums * 0.215 + (c > 1 ? 320.0 : 0.0);
+                    // rows are staged once for the ranges that a cluster has of an
+                    // item, or, in chunks, for every unit
+                    const double rows = rows_most * slice * STEP / staging + (GRAD ? 380.0 : 120.0);
+                    const double stagings =
+                        chunks > 1 ? rounds : std::min(rounds, std::ceil(items / nc) + (nb > 1));
+                    const double t =
+                        rounds * (serial * stage + unit + (GRAD ? 6500.0 : 4000.0) * (chunks - 1)) +
+                        stagings * rows;
+                    if (t < cut.ns) {
+                        cut.ns = t;
                         p.wo = wo, p.wk = wk, p.range = wo * TILE, p.nranges = nr;
                         p.slice = slice, p.chunk = chunk;
                         // the survey of the rows costs about as much as it
                         // saves a warp in four stages
                         p.try_common = chunks == 1 && (nb > 1 ? 1 : rounds) * serial > 4;
-                        *ranks = c;
-                        *grid = int(busy) * c;
+                        cut.ranks = c, cut.grid = int(std::ceil(busy)) * c;
                     }
                 }
             }
@@ -132,50 +170,43 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
     }
 
     // The rule's answer by sizes; asking it takes longer than a small product.
-    static int cached_plan(const void *kern, MatvecPlan &p, int rows_each, int items, int nb,
-                           const DeviceScope &dev, int *ranks, int *grid) {
-        struct Answer {
-            MatvecPlan p;
-            int ranks, grid;
-        };
+    static int cut_for(const MatvecPlan &p, int nb, const DeviceScope &dev, MvCut &cut) {
         static std::mutex mu;
-        static std::map<std::array<int, 7>, Answer> seen;
-        const std::array<int, 7> key = {dev.device, p.N, p.K, p.rows_most, rows_each, items, nb};
+        static std::map<std::array<int, 5>, MvCut> seen;
+        static int sized = -1; // the device whose kernel may take the memory
+        const std::array<int, 5> key = {dev.device, p.N, p.K, p.rows_most, nb};
         std::lock_guard<std::mutex> lk(mu);
+        if (sized != dev.device) {
+            MVB_TRY(cudaFuncSetAttribute(kernel(), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kMvSmem));
+            sized = dev.device;
+        }
         auto it = seen.find(key);
         if (it == seen.end()) {
-            Answer a{p, 1, 1};
-            if (int rc = plan(kern, a.p, rows_each, items, nb, dev, &a.ranks, &a.grid))
+            MvCut c{p};
+            if (int rc = plan(c, nb, dev))
                 return rc;
             if (seen.size() >= 4096) // a caller of ever new sizes
                 seen.clear();
-            it = seen.emplace(key, a).first;
+            it = seen.emplace(key, c).first;
         }
-        const int y_f32 = p.y_f32, x_vec = p.x_vec;
-        p = it->second.p;
-        p.y_f32 = y_f32, p.x_vec = x_vec;
-        *ranks = it->second.ranks, *grid = it->second.grid;
+        cut = it->second;
+        cut.p.y_f32 = p.y_f32, cut.p.x_vec = p.x_vec, cut.p.y_vec = p.y_vec;
         return MVLLM_OK;
     }
+    static const void *kernel() {
+        return reinterpret_cast<const void *>(matvec_q4_kernel<FMT, TX, NT, GRAD, FINE>);
+    }
 
-    static int launch(cudaStream_t st, MatvecArgs a, MatvecPlan p, int items, const DeviceScope &dev,
-                      const void *x, int64_t ldx, void *y, int64_t ldy) {
-        auto kern = matvec_q4_kernel<FMT, TX, NT, GRAD, FINE>;
-        int ranks = 1, grid = 1;
-        static std::atomic<int> sized{-1}; // the device whose kernel may take the memory
-        if (sized.load() != dev.device) {
-            MVB_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kMvSmem));
-            sized.store(dev.device);
-        }
-        if (int rc = cached_plan(reinterpret_cast<const void *>(kern), p,
-                                 (a.rows + a.nb - 1) / a.nb, items, a.nb, dev, &ranks, &grid))
-            return rc;
+    static int launch(cudaStream_t st, const MatvecArgs &a, MvCut cut, const void *x, int64_t ldx,
+                      void *y, int64_t ldy) {
+        MatvecPlan &p = cut.p;
+        const int ranks = cut.ranks;
         const int smem = layout(p, p.chunk, ranks, a.nb);
         if (p.range < 1 || smem > kMvSmem)
             return host_fail(MVLLM_ERR_UNSUPPORTED, "matvec_q4: %d bytes of shared memory", smem);
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(grid);
+        cfg.gridDim = dim3(cut.grid);
         cfg.blockDim = dim3(THREADS);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = st;
@@ -186,39 +217,45 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
         at[1].val.clusterDim.x = ranks, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
         cfg.attrs = at;
         cfg.numAttrs = 2;
-        MVB_TRY(cudaLaunchKernelEx(&cfg, kern, a, p, static_cast<const TX *>(x), ldx, y, ldy));
+        MVB_TRY(cudaLaunchKernelEx(&cfg, matvec_q4_kernel<FMT, TX, NT, GRAD, FINE>, a, p,
+                                   static_cast<const TX *>(x), ldx, y, ldy));
         return MVLLM_OK;
     }
 };
 
-// Rows of a matrix that a launch takes at a time: enough operand columns for
-// the average expert (all rows of a single matrix), at most 32 (gradient: 16).
+// Rows that a pass over a matrix takes: all rows of a single matrix where 8,
+// 16 or 32 operand columns (gradient: 8 or 16) hold them, as many as that for
+// more.  Experts, whose rows differ, take the width whose plan has the lowest
+// estimate: 48 experts of 16 rows on average, 7168 -> 2048, take 183 us by 16
+// rows a pass and 253 by 32, 160 experts of 20, 6144 -> 1536, 614 and 462.
 template <int FMT, typename TX, bool GRAD, bool FINE>
-int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, const DeviceScope &dev, const void *x,
-                int64_t ldx, void *y, int64_t ldy) {
+int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, const DeviceScope &dev,
+                const void *x, int64_t ldx, void *y, int64_t ldy) {
     constexpr int T = MvTerms<FMT, TX, GRAD, FINE>::T;
-    const int avg = (a.rows + a.nb - 1) / a.nb;
-    auto items = [&](int rp) {
-        return a.nb == 1 ? (a.rows + rp - 1) / rp
-                         : std::min(a.rows, a.nb * ((avg + rp - 1) / rp));
-    };
-    // One more than the average expert's rows, for the uneven ones; the
-    // gradient's wider form costs more than the second pass it saves them.
-    const int want = a.nb == 1 || GRAD ? avg : avg + 1;
-    if (want <= 8 / T)
-        return MvHost<FMT, TX, 1, GRAD, FINE>::launch(st, a, p, items(8 / T), dev, x, ldx, y, ldy);
-    if (GRAD || want <= 16 / T)
-        return MvHost<FMT, TX, 2, GRAD, FINE>::launch(st, a, p, items(16 / T), dev, x, ldx, y,
-                                                      ldy);
-    if constexpr (!GRAD)
-        return MvHost<FMT, TX, 4, false, FINE>::launch(st, a, p, items(32 / T), dev, x, ldx, y,
-                                                       ldy);
-    return MVLLM_OK;
+    using One = MvHost<FMT, TX, 1, GRAD, FINE>;
+    using Two = MvHost<FMT, TX, 2, GRAD, FINE>;
+    using Four = MvHost<FMT, TX, GRAD ? 2 : 4, GRAD, FINE>;
+    MvCut one, two, four;
+    const bool some = a.nb > 1, wide = !GRAD && (some || a.rows > 16 / T);
+    if (some || a.rows <= 8 / T)
+        if (int rc = One::cut_for(p, a.nb, dev, one))
+            return rc;
+    if (some || (a.rows > 8 / T && !wide))
+        if (int rc = Two::cut_for(p, a.nb, dev, two))
+            return rc;
+    if (wide)
+        if (int rc = Four::cut_for(p, a.nb, dev, four))
+            return rc;
+    if (one.ns <= two.ns && one.ns <= four.ns)
+        return One::launch(st, a, one, x, ldx, y, ldy);
+    if (two.ns <= four.ns)
+        return Two::launch(st, a, two, x, ldx, y, ldy);
+    return Four::launch(st, a, four, x, ldx, y, ldy);
 }
 
 template <int FMT, typename TX>
-int matvec_way(cudaStream_t st, bool grad, const MatvecArgs &a, const MatvecPlan &p, const DeviceScope &dev,
-               const void *x, int64_t ldx, void *y, int64_t ldy) {
+int matvec_way(cudaStream_t st, bool grad, const MatvecArgs &a, const MatvecPlan &p,
+               const DeviceScope &dev, const void *x, int64_t ldx, void *y, int64_t ldy) {
     if (!grad)
         return matvec_rows<FMT, TX, false, false>(st, a, p, dev, x, ldx, y, ldy);
     if constexpr (FMT == MVLLM_FMT_INT4_G64 && sizeof(TX) == 2)
@@ -246,6 +283,9 @@ int matvec_any(const char *who, void *stream, bool grad, const MatvecArgs &a, co
     p.N = out, p.K = grad ? a.O : a.I;
     p.y_f32 = y_dtype == MVLLM_DTYPE_F32;
     p.rows_most = a.rows;
+    const uint64_t ey = p.y_f32 ? 4 : 2;
+    p.y_vec = ((reinterpret_cast<uintptr_t>(y) | (a.rows > 1 ? uint64_t(ldy) * ey : 0)) &
+               (4 * ey - 1)) == 0;
     const bool fx = x_dtype == MVLLM_DTYPE_F32, i4 = a.fmt == MVLLM_FMT_INT4_G64;
     const uint64_t pitch = a.rows > 1 ? uint64_t(ldx) * (fx ? 4 : 2) : 0;
     p.x_vec = ((reinterpret_cast<uintptr_t>(x) | pitch) & 15u) == 0;

@@ -62,6 +62,7 @@ struct MatvecPlan {
     int slice;     // stages of the reduction per CTA of the cluster
     int chunk;     // stages whose rows are staged in shared memory at a time
     int x_vec;     // rows of x start on 16-byte boundaries
+    int y_vec;     // rows of y on boundaries of four elements
     int rows_most; // rows that one matrix can have
     int y_f32;
     int try_common; // a main loop long enough to pay for the survey of the rows
@@ -136,8 +137,10 @@ __device__ __forceinline__ uint32_t mv_cluster_addr(uint32_t addr, int rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+__device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, const float (&v)[4]) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v[0]),
+                 "f"(v[1]), "f"(v[2]), "f"(v[3])
+                 : "memory");
 }
 
 // A stage in shared memory: 32 weight rows of 128 bytes, 16-byte chunk c of
@@ -941,13 +944,13 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
     } else {
         items = (a.rows + RP - 1) / RP;
     }
-    const int64_t total = int64_t(items) * pl.nranges;
+    const int total = items * pl.nranges; // below the elements of y
     const int rows_w = GRAD ? pl.K : pl.N; // rows of the matrices (O)
 
-    auto decode = [&](int64_t u) {
+    auto decode = [&](int u) {
         MvUnit q;
-        q.item = int(u / pl.nranges);
-        q.out0 = int(u - int64_t(q.item) * pl.nranges) * pl.range;
+        q.item = u / pl.nranges;
+        q.out0 = (u - q.item * pl.nranges) * pl.range;
         int r0 = 0, r1 = 0, pass = q.item;
         if (a.wt) {
             int lo = 0, hi = a.nb; // the last expert with list[e] <= item has it
@@ -1046,12 +1049,16 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
         mv_commit();
     };
     MvUnit cur{};
-    if (cluster < total) {
-        cur = decode(cluster);
+    // A cluster's units follow one another, so that an item's rows are staged
+    // once for its ranges.
+    const int each = total / clusters, more = total - each * clusters;
+    const int u0 = each * cluster + min(cluster, more), u1 = u0 + each + (cluster < more);
+    if (u0 < u1) {
+        cur = decode(u0);
         fetch(cur);
         prologue(cur);
     }
-    for (int64_t u = cluster; u < total; u += clusters) {
+    for (int u = u0; u < u1; ++u) {
         const int tasks = tasks_of(cur);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -1089,7 +1096,7 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
                         } else {
                             // the first unit's rows were asked for before its
                             // weights, the others' after
-                            if (u == cluster)
+                            if (u == u0)
                                 mv_wait<1>();
                             else
                                 mv_wait<0>();
@@ -1152,8 +1159,8 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
             prologue(cur);
         }
         MvUnit next{};
-        if (u + clusters < total)
-            next = decode(u + clusters);
+        if (u + 1 < u1)
+            next = decode(u + 1);
         if constexpr (GRAD) {
             mv_wait<0>();
             __syncthreads(); // the ring is done with before the sums overlay it
@@ -1164,60 +1171,85 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
             // A warp that is done goes on to the next unit's weights; its rows
             // wait until their places are free.
             __syncwarp();
-            if (u + clusters < total)
+            if (u + 1 < u1)
                 prologue(next);
             __syncthreads();
-            if (u + clusters < total)
+            if (u + 1 < u1)
                 fetch(next);
         }
         // The CTA's own wk partial sums (and the gradient's parts) first.  With one CTA per cluster that is the
         // result; else it goes to the CTA that owns the block, and one cluster
         // barrier later each CTA adds up what it was sent.  Two buffers take
         // turns, so that a unit's values cannot meet the next one's.
-        // A warp takes a block of 32 outputs and goes through the rows.
+        // An item is (row, block of 32 outputs), eight lanes of four outputs each;
+        // warps take four at a time.  It is owned by rank item % ranks, there in
+        // slot item / ranks * ranks + sender.  (Distributed shared memory takes
+        // stores of 16 bytes a lane several times as fast as of 4.)
         const int outs = min(pl.range, pl.N - cur.out0), blocks = (outs + 31) / 32;
+        const int all = blocks * cur.n, sub = lane >> 3, o4 = (lane & 7) * 4;
         const int slots = (pl.range / 32 * RP + ranks - 1) / ranks * ranks; // of a mail buffer
         const uint32_t mail = smem_u32(mv_smem + pl.off_mail) + turn * slots * 128;
         const int parts = cur.w ? pl.wk : 0, mask = ranks - 1;
-        for (int b = warp; b < blocks; b += kMvWarps) {
-            const int o = b * 32 + lane;
-            const float *at = red + (o / TILE) * pl.wk * RSIZE + o % TILE;
-            // item = (row, block), owned by rank item % ranks there, slot
-            // item / ranks * ranks + sender
-            int item = b;
-#pragma unroll 2
-            for (int r = 0; r < cur.n; ++r, item += blocks, at += (GRAD ? T : 1) * RPITCH) {
-                float v = 0.f;
-                for (int k = 0; k < parts; ++k)
+        auto out = [&](int r, int o, const float(&v)[4]) {
+            const int64_t at = int64_t(cur.r0 + r) * ldy + cur.out0 + o;
+            if (pl.y_vec && o + 4 <= outs) {
+                if (pl.y_f32)
+                    store_row<4>(static_cast<float *>(y) + at, v);
+                else
+                    store_row<4>(static_cast<__nv_bfloat16 *>(y) + at, v);
+            } else {
 #pragma unroll
-                    for (int q = 0; q < (GRAD ? T : 1); ++q)
-                        v += at[k * RSIZE + q * RPITCH];
-                if (ranks > 1)
-                    st_cluster_f32(mv_cluster_addr(mail + ((item & ~mask) + rank) * 128 + lane * 4,
-                                                   item & mask),
-                                   v);
-                else if (o < outs)
-                    mv_store(y, pl.y_f32, int64_t(cur.r0 + r) * ldy + cur.out0 + o, v);
+                for (int q = 0; q < 4; ++q)
+                    if (o + q < outs)
+                        mv_store(y, pl.y_f32, at + q, v[q]);
             }
+        };
+        for (int item = warp * 4 + sub; item < all; item += kMvWarps * 4) {
+            const int r = item / blocks, o = (item - r * blocks) * 32 + o4;
+            const float *at =
+                red + (o / TILE) * pl.wk * RSIZE + o % TILE + r * ((GRAD ? T : 1) * RPITCH);
+            float v[4] = {};
+            for (int k = 0; k < parts; ++k) {
+                if constexpr (GRAD) {
+#pragma unroll
+                    for (int q = 0; q < T; ++q)
+#pragma unroll
+                        for (int s = 0; s < 4; ++s)
+                            v[s] += at[k * RSIZE + q * RPITCH + s];
+                } else {
+                    const float4 p = *reinterpret_cast<const float4 *>(at + k * RSIZE);
+                    v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+                }
+            }
+            if (ranks > 1)
+                st_cluster_f32x4(
+                    mv_cluster_addr(mail + ((item & ~mask) + rank) * 128 + o4 * 4, item & mask), v);
+            else
+                out(r, o, v);
         }
         if (ranks > 1) {
             mv_cluster_sync();
-            for (int item = warp * ranks + rank; item < blocks * cur.n; item += kMvWarps * ranks) {
-                const int r = item / blocks, o = (item - r * blocks) * 32 + lane;
-                const uint32_t at = mail + (item & ~mask) * 128 + lane * 4;
-                float v = 0.f;
+            for (int item = (warp * 4 + sub) * ranks + rank; item < all;
+                 item += kMvWarps * 4 * ranks) {
+                const int r = item / blocks, o = (item - r * blocks) * 32 + o4;
+                const uint32_t at = mail + (item & ~mask) * 128 + o4 * 4;
+                float v[4] = {};
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    v += c < ranks ? __uint_as_float(lds32(at + c * 128)) : 0.f;
-                if (o < outs)
-                    mv_store(y, pl.y_f32, int64_t(cur.r0 + r) * ldy + cur.out0 + o, v);
+                for (int c = 0; c < 8; ++c) {
+                    if (c < ranks) {
+                        const uint4 p = lds128(at + c * 128);
+                        v[0] += __uint_as_float(p.x), v[1] += __uint_as_float(p.y);
+                        v[2] += __uint_as_float(p.z), v[3] += __uint_as_float(p.w);
+                    }
+                }
+                out(r, o, v);
             }
             turn ^= 1;
         } else {
             __syncthreads();
         }
         cur = next;
-        if (GRAD && u + clusters < total) {
+        if (GRAD && u + 1 < u1) {
             fetch(cur);
             prologue(cur);
         }
