@@ -319,10 +319,13 @@ int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t l
         a.partial = take((slots / kRgRows + E) * H);
         a.counters = E * ncol + 1;
         // Long row blocks leave fewer partial sums, short ones more items to
-        // share: 256 rows where that makes 14 items per SM, else 128.  (65536
-        // slots of 384 experts, H 7168: 105 us by 256, 124 by 128; 32768 of
-        // 64, H 2048: 40 and 28; 512 rows cost uneven experts 12 us more.)
-        a.block = int64_t(slots / (2 * kRgRows)) * ncol >= 14 * dev.sms ? 2 * kRgRows : kRgRows;
+        // share: 64 rows, doubled up to 256 while 24 items per SM remain.
+        // (65536 slots of 384 experts, H 7168, by 256 rows: 97 us; 32768 of 64,
+        // H 2048: 28 by 64 or 128, 36 by 256; 512 rows cost uneven experts 12 us
+        // more.)
+        a.block = kRgRows;
+        while (a.block < 256 && int64_t(slots / (2 * a.block)) * ncol >= 24 * dev.sms)
+            a.block *= 2;
     }
     if (T > 0 && dx) { // dz on the way
         const int rc = dx_dtype == MVLLM_DTYPE_F32
