@@ -6,6 +6,16 @@
 // with W[o, i] = q[o, i] s[o, i / G] decoded from the packed formats (int4
 // with a f32 scale per G = 64 columns, MXFP4 with a ue8m0 scale per G = 32).
 // Sums are f32.
+//
+// The weights are read once per pass of up to 32 rows, 4.5 bits each, so the
+// floor is their bytes; each decodes to an operand of m16n8k16 matrix
+// instructions, which take the rows as the narrow side.  One row of 7168 ->
+// 65536 streams at 4.7 TB/s, 72% of a copy; 7168 -> 16384 (60 MB) takes 17 us
+// for 1 row, 20 for 8, 31 for 16 and 63 for 32.  Beyond the memory it is the
+// decoding that bounds: 520 instructions per stage of a warp for 8 rows, 970
+// to 1290 for 32, issued on 58% and 35% of the cycles; the matrix pipe is busy
+// for 25 to 36%.  Short products are bound by their start: 6 to 7 us for 8 MB,
+// of which the rows' way to the operands is about half.
 #pragma once
 
 #include "row_kernels.cuh"
@@ -42,8 +52,12 @@ __device__ __forceinline__ bool matvec_expert(const MatvecArgs &a, int e, const 
 
 // Warps of a CTA (one CTA per SM) and stages of a warp's ring.  The forward
 // product is bound by the instructions of the dequantisation and wants as many
-// warps to interleave as registers and the staged rows leave room for; the
-// gradient holds 64 or 128 sums per lane.
+// warps to interleave as registers and the staged rows leave room for: with 16
+// warps 16 rows take 7168 -> 16384 in 39 us in place of 35 (registers spill),
+// with 12 warps 32 rows in 91 in place of 70 (the staged rows come in more
+// chunks).  The gradient holds 64 or 128 sums per lane; cut to 128 columns a
+// task it fits 12 or 16 warps, which took 450 and 490 us in place of 385 on 160
+// experts of 1536 x 6144.
 template <int NT, bool GRAD> constexpr int mv_warps() {
     return GRAD || NT == 4 ? 8 : NT == 2 ? 12 : 16;
 }
@@ -881,7 +895,7 @@ struct MvUnit {
 // (a range of outputs); the cluster's CTAs split the reduction.  A CTA's tasks
 // are the range's tiles x wk parts of its slice of the reduction; its warps
 // take them in turn, each streaming its tasks' stages through its own ring, so
-// the main loop has no barrier.  The wk x cluster partial sums of an output
+// the main loop has no barrier (a stage takes a warp about 2 us).  The wk x cluster partial sums of an output
 // meet in (distributed) shared memory and are added in a fixed order.
 template <int FMT, typename TX, int NT, bool GRAD, bool FINE>
 __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
@@ -1050,7 +1064,8 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
     };
     MvUnit cur{};
     // A cluster's units follow one another, so that an item's rows are staged
-    // once for its ranges.
+    // once for its ranges (48 experts of 5 rows, 7168 -> 2048: 111 us, 130 with
+    // the clusters taking units in turn).
     const int each = total / clusters, more = total - each * clusters;
     const int u0 = each * cluster + min(cluster, more), u1 = u0 + each + (cluster < more);
     if (u0 < u1) {
@@ -1177,14 +1192,16 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
             if (u + 1 < u1)
                 fetch(next);
         }
-        // The CTA's own wk partial sums (and the gradient's parts) first.  With one CTA per cluster that is the
-        // result; else it goes to the CTA that owns the block, and one cluster
-        // barrier later each CTA adds up what it was sent.  Two buffers take
+        // The CTA's own wk partial sums (and the gradient's parts) first.  With
+        // one CTA per cluster that is the result; else it goes to the CTA that
+        // owns the block, and one cluster barrier later each CTA adds up what it
+        // was sent.  Two buffers take
         // turns, so that a unit's values cannot meet the next one's.
         // An item is (row, block of 32 outputs), eight lanes of four outputs each;
         // warps take four at a time.  It is owned by rank item % ranks, there in
         // slot item / ranks * ranks + sender.  (Distributed shared memory takes
-        // stores of 16 bytes a lane several times as fast as of 4.)
+        // 16 bytes a lane better than 4: 16 rows of 7168 -> 16384 in 31 us, 35
+        // with four times the stores.)
         const int outs = min(pl.range, pl.N - cur.out0), blocks = (outs + 31) / 32;
         const int all = blocks * cur.n, sub = lane >> 3, o4 = (lane & 7) * 4;
         const int slots = (pl.range / 32 * RP + ranks - 1) / ranks * ranks; // of a mail buffer
