@@ -173,3 +173,96 @@ def test_python_refusals(moe):
     no("int64", moe.expert_matvec_q4_dev, rc.INT4, x, zero, tab, zero, zero, y)
     no("fmt", moe.expert_matvec_q4_grad_dev, 8, y, tab, tab, zero, zero, x)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("fmt", [rc.INT4, rc.MXFP4])
+def test_matrices_past_two_gigabytes(moe, fmt):
+    """Offsets of packed weights beyond 2^31 bytes.  Some outputs of the
+    forward product, and a gradient that only some weight rows enter, against
+    64 bits: length / 16 + 64 additions off by 2^-22 of the magnitudes, as for
+    the other products, and the factors' f16 or bf16 parts."""
+    O, I, S = 70000, 65536, 2
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.randint(0, 256, (O, I // 2), generator=g, dtype=torch.uint8, device="cuda")
+    if fmt == rc.INT4:
+        s = torch.rand(O, I // 64, generator=g, device="cuda") * 0.01 + 1e-4
+    else:
+        s = torch.randint(113, 126, (O, I // 32), generator=g, dtype=torch.uint8, device="cuda")
+    at = torch.tensor([0, 1, 33333, 65535, 65536, 69997, O - 1], device="cuda")
+    W = rc.decode(w[at], s[at], fmt, I)
+    x = torch.randn(S, I, generator=g, device="cuda")
+    y = torch.empty(S, O, device="cuda")
+    moe.matvec_q4_dev(fmt, x, w, s, y)
+    want, size = x.double() @ W.T, x.double().abs() @ W.T.abs()
+    assert ((y[:, at].double() - want).abs() <= (I / 16 + 64) * 2.0 ** -22 * size).all()
+    dy, dx = torch.zeros(S, O, device="cuda"), torch.empty(S, I, device="cuda")
+    dy[:, at] = torch.randn(S, len(at), generator=g, device="cuda")
+    moe.matvec_q4_grad_dev(fmt, dy, w, s, dx)
+    want, size = dy[:, at].double() @ W, dy[:, at].double().abs() @ W.abs()
+    assert ((dx.double() - want).abs() <= (O / 16 + 64) * 2.0 ** -22 * size).all()
+
+
+def test_calls_at_the_same_time(moe):
+    """Two streams and two host threads, sizes that no call has had before."""
+    import threading
+    gen = torch.Generator().manual_seed(8)
+    E, T, K = 12, 75, 3
+    cases = []
+    for I, O in ((1184, 736), (864, 1248)):
+        w, s = rc.packed(gen, rc.INT4, E * O, I, "cuda")
+        tab = torch.tensor([w[e * O].data_ptr() for e in range(E)], device="cuda")
+        sct = torch.tensor([s[e * O].data_ptr() for e in range(E)], device="cuda")
+        idx, wt = rc.routing(gen, T, K, E)
+        plan = rc.device_plan(moe, idx.cuda(), wt.cuda(), E)
+        x = torch.randn(T * K, I, generator=gen).cuda()
+        cases.append((w, s, tab, sct, plan, x, torch.randn(T * K, O, generator=gen).cuda()))
+    torch.cuda.synchronize()
+
+    def step(c, stream, out):
+        w, s, tab, sct, plan, x, dy = c
+        y, dx = torch.zeros_like(dy), torch.zeros_like(x)
+        stream.wait_stream(torch.cuda.current_stream())
+        for _ in range(20):
+            moe.expert_matvec_q4_dev(rc.INT4, x, tab, sct, plan["nr"], plan["xoff"], y,
+                                     stream=stream)
+            moe.expert_matvec_q4_grad_dev(rc.INT4, dy, tab, sct, plan["nr"], plan["xoff"], dx,
+                                          stream=stream)
+        stream.synchronize()
+        out.append((y, dx))
+
+    together = [[], []]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    threads = [threading.Thread(target=step, args=(cases[i], streams[i], together[i]))
+               for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        alone = []
+        step(cases[i], streams[i], alone)
+        for a, b in zip(together[i][0], alone[0]):
+            assert torch.count_nonzero(a) and torch.equal(a, b)
+
+
+def test_first_call_of_a_size_captured(moe):
+    """Nothing that a size's first call does on the host disturbs a capture."""
+    gen = torch.Generator().manual_seed(9)
+    S, I, O = 5, 1376, 928
+    w, s = rc.packed(gen, rc.MXFP4, O, I, "cuda")
+    x, dy = torch.randn(S, I, generator=gen).cuda(), torch.randn(S, O, generator=gen).cuda()
+    outs = [[torch.zeros(S, O, device="cuda"), torch.zeros(S, I, device="cuda")] for _ in range(2)]
+
+    def step(o):
+        moe.matvec_q4_dev(rc.MXFP4, x, w, s, o[0])
+        moe.matvec_q4_grad_dev(rc.MXFP4, dy, w, s, o[1])
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(outs[0])
+    graph.replay()
+    step(outs[1])
+    torch.cuda.synchronize()
+    for a, b in zip(*outs):
+        assert torch.count_nonzero(a) and torch.equal(a, b)
