@@ -387,7 +387,9 @@ __device__ __forceinline__ int mv_shift(float m) {
     const int e = int(__float_as_uint(m) >> 23) - 127;
     return m > 0.f ? min(14 - e, 126) : 0;
 }
-__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }
+__device__ __forceinline__ float exp2_int(int e) {
+    return __uint_as_float(uint32_t(127 + e) << 23);
+}
 
 // Stages rows [r0, r0 + n) of x, columns c0 .. c0 + cols, as the forward
 // product's B operand: f16 parts of x * 2^e, [n T][cols] in 8-column chunks
@@ -550,7 +552,8 @@ __device__ __forceinline__ void mv_int4x8(uint32_t w, uint32_t (&h)[4]) {
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(b) : "r"(w), "r"(m1), "r"(one));
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(c) : "r"(u), "r"(m0), "r"(one));
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(u), "r"(m1), "r"(one));
-    const uint32_t bias = 0x64086408u, sixteenth = 0x2c002c00u, off = 0xd480d480u; // 1032, 1/16, -72
+    // 1032, 1/16, -72
+    const uint32_t bias = 0x64086408u, sixteenth = 0x2c002c00u, off = 0xd480d480u;
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(h[0]) : "r"(a), "r"(bias));
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(h[1]) : "r"(b), "r"(sixteenth), "r"(off));
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(h[2]) : "r"(c), "r"(bias));
@@ -895,8 +898,9 @@ struct MvUnit {
 // (a range of outputs); the cluster's CTAs split the reduction.  A CTA's tasks
 // are the range's tiles x wk parts of its slice of the reduction; its warps
 // take them in turn, each streaming its tasks' stages through its own ring, so
-// the main loop has no barrier (a stage takes a warp about 2 us).  The wk x cluster partial sums of an output
-// meet in (distributed) shared memory and are added in a fixed order.
+// the main loop has no barrier (a stage takes a warp about 2 us).  The wk x
+// cluster partial sums of an output meet in (distributed) shared memory and are
+// added in a fixed order.
 template <int FMT, typename TX, int NT, bool GRAD, bool FINE>
 __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
     matvec_q4_kernel(const MatvecArgs a, const MatvecPlan pl, const TX *__restrict__ x,
@@ -1098,14 +1102,15 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
                 if (cur.w && staged != cur.item) { // uniform over the CTA
                     if constexpr (GRAD) {
                         __syncthreads(); // the last readers of x are done
-                        mv_stage_gradient<FMT, TX, NT>(mv_smem + pl.off_x, pitch, x, ldx, cur.r0, cur.n,
-                                                       (k0 + c0) * STEP, cols, pl.K, pl.x_vec, c0 == 0,
-                                                       held);
+                        mv_stage_gradient<FMT, TX, NT>(mv_smem + pl.off_x, pitch, x, ldx, cur.r0,
+                                                       cur.n, (k0 + c0) * STEP, cols, pl.K,
+                                                       pl.x_vec, c0 == 0, held);
                     } else {
                         if (c0 > 0) {
                             __syncthreads();
-                            mv_fetch_rows<FMT, TX, NT>(mv_smem + pl.off_x, pitch, x, ldx, cur.r0, cur.n,
-                                                       (k0 + c0) * STEP, cols, pl.K, pl.x_vec);
+                            mv_fetch_rows<FMT, TX, NT>(mv_smem + pl.off_x, pitch, x, ldx, cur.r0,
+                                                       cur.n, (k0 + c0) * STEP, cols, pl.K,
+                                                       pl.x_vec);
                             mv_commit();
                             mv_wait<0>();
                         } else {
@@ -1117,9 +1122,9 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
                                 mv_wait<0>();
                         }
                         __syncthreads();
-                        common = mv_stage_forward<FMT, TX, NT>(mv_smem + pl.off_x, ex, pitch, cur.n,
-                                                               cols, pl.try_common && nk <= pl.chunk,
-                                                               row_max);
+                        common = mv_stage_forward<FMT, TX, NT>(
+                            mv_smem + pl.off_x, ex, pitch, cur.n, cols,
+                            pl.try_common && nk <= pl.chunk, row_max);
                     }
                     __syncthreads();
                     if (nk <= pl.chunk)

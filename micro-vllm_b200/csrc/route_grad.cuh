@@ -107,11 +107,14 @@ __global__ void __launch_bounds__(256) route_dz_kernel(const RouteGradArgs a) {
     route_put_grad(a, t, e, dz);
 }
 
-// dx[t] = sum_k dz_k router[idx_k], the router's rows gathered from L2: a CTA
-// takes (token, segment of the row).  Bound by L2, 4 T K H bytes at about 20
-// TB/s.  (A form with some columns of every expert in shared memory, which the
-// CTA's tokens then read, took 25 to 60% longer up to 64 slots per expert and
-// was never more than 7% ahead.)
+// dx[t] = sum_k dz_k router[idx_k], the router's rows gathered: a CTA takes
+// (token, segment of the row).  The gathers are 4 T K H bytes, 1.9 GB in 102 us
+// for 8192 tokens of 8 out of 384 experts, H 7168; half of the sectors hit L1,
+// whose throughput and the issue slots both stand at 78%.  (A form with some
+// columns of every expert in shared memory, which the CTA's tokens then read,
+// took 25 to 60% longer up to 64 slots per expert and was never more than 7%
+// ahead; eight columns a lane split the sectors, 117 us in place of 82 on 6144
+// tokens.)
 template <typename TO, int N>
 __global__ void __launch_bounds__(kRgThreads)
     route_dx_kernel(const RouteGradArgs a, int nseg, int seg, TO *__restrict__ dx, int64_t lddx) {
@@ -157,7 +160,9 @@ __global__ void __launch_bounds__(kRgThreads)
 // blocks, so the columns of x that all experts gather from (16 T kRgCols bytes
 // in bf16) stay in L2.  An expert of several items leaves its partial sums in
 // the workspace, and the warp that arrives last adds them in order; one without
-// rows gets zeros.  Bound by the latency of the gathers.
+// rows gets zeros.  Bound by the latency of the gathers, a third of whose
+// sectors miss the near L2; issue slots stand at 52%.  (Rows through a ring of
+// asynchronous copies, three times as many under way, took 140 us.)
 template <typename TX>
 __global__ void __launch_bounds__(256, sizeof(TX) == 4 ? 2 : 4)
     route_dw_kernel(const RouteGradArgs a, const TX *__restrict__ x, int64_t ldx, int vec,

@@ -87,9 +87,9 @@ int mvllm_moe_dispatch_dev(void *stream, const void *x, int dtype, int64_t ldx,
 namespace {
 
 template <typename TY, typename TO>
-int combine_launch(cudaStream_t st, int sms, int n, const TY *y, int64_t ldy, int cap, const float *rw,
-                   const int *tok_pos, int T, int KK, int D, TO *out, int64_t ldo,
-                   int accumulate) {
+int combine_launch(cudaStream_t st, int sms, int n, const TY *y, int64_t ldy, int cap,
+                   const float *rw, const int *tok_pos, int T, int KK, int D, TO *out,
+                   int64_t ldo, int accumulate) {
     // 64 warps per SM: whole rows leave 64 tokens of 8 rows of 7168 bf16 at 30 us
     // in place of 4.0; the finest cut costs 4096 tokens 93 in place of 85.
     const Segments s(T, (D + n - 1) / n, 32, sms * 64);
@@ -135,16 +135,16 @@ int combine_any(const char *who, void *stream, const void *y, int y_dtype, int64
     const bool fy = y_dtype == MVLLM_DTYPE_F32, fo = out_dtype == MVLLM_DTYPE_F32;
     using bf = __nv_bfloat16;
     if (fy && fo)
-        return combine_launch(st, dev.sms, n, static_cast<const float *>(y), ldy, cap, rw, tok_pos, T, KK,
-                              D, static_cast<float *>(out), ldo, accumulate);
+        return combine_launch(st, dev.sms, n, static_cast<const float *>(y), ldy, cap, rw,
+                              tok_pos, T, KK, D, static_cast<float *>(out), ldo, accumulate);
     if (fy)
-        return combine_launch(st, dev.sms, n, static_cast<const float *>(y), ldy, cap, rw, tok_pos, T, KK,
-                              D, static_cast<bf *>(out), ldo, accumulate);
+        return combine_launch(st, dev.sms, n, static_cast<const float *>(y), ldy, cap, rw,
+                              tok_pos, T, KK, D, static_cast<bf *>(out), ldo, accumulate);
     if (fo)
-        return combine_launch(st, dev.sms, n, static_cast<const bf *>(y), ldy, cap, rw, tok_pos, T, KK, D,
-                              static_cast<float *>(out), ldo, accumulate);
-    return combine_launch(st, dev.sms, n, static_cast<const bf *>(y), ldy, cap, rw, tok_pos, T, KK, D,
-                          static_cast<bf *>(out), ldo, accumulate);
+        return combine_launch(st, dev.sms, n, static_cast<const bf *>(y), ldy, cap, rw,
+                              tok_pos, T, KK, D, static_cast<float *>(out), ldo, accumulate);
+    return combine_launch(st, dev.sms, n, static_cast<const bf *>(y), ldy, cap, rw, tok_pos,
+                          T, KK, D, static_cast<bf *>(out), ldo, accumulate);
 }
 
 template <typename TD, typename TY>
@@ -340,7 +340,8 @@ int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t l
     if (drouter) {
         const int rc =
             x_dtype == MVLLM_DTYPE_F32
-                ? route_dw(st, a, dev.sms, static_cast<const float *>(x), ldx, nr, xoff, rows, drouter)
+                ? route_dw(st, a, dev.sms, static_cast<const float *>(x), ldx, nr, xoff, rows,
+                           drouter)
                 : route_dw(st, a, dev.sms, static_cast<const __nv_bfloat16 *>(x), ldx, nr, xoff,
                            rows, drouter);
         if (rc)

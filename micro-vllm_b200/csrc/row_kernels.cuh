@@ -239,7 +239,8 @@ __global__ void __launch_bounds__(256)
 // over the token's positions in ascending order (ascending expert id), f32
 // fused multiply-adds, one rounding at the end.  rw == nullptr: weight 1.
 // A warp takes (token, segment of the row) and has eight positions' loads under
-// way at a time.
+// way at a time.  Bound by memory: 4096 tokens of 8 rows of 7168 bf16 into f32
+// move 587 MB in 93 us, 6.3 TB/s.
 template <typename TY, typename TO, int N>
 __global__ void __launch_bounds__(256)
     combine_rows_kernel(const TY *__restrict__ y, int64_t ldy, int cap,
@@ -324,7 +325,8 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// The combine's gradient, a CTA per token: dy[p] = rw[p] dout[t] and
+// The combine's gradient, a CTA per token (4096 of 8 rows of 7168 bf16, 10% of
+// them padding: 147 us, 6.1 TB/s): dy[p] = rw[p] dout[t] and
 // drw[p] = <dout[t], y[p]> (f32, warps' partial sums added in warp order),
 // then dwt[t, k] = drw of the position that token t has for expert idx[t, k]
 // (a repeated id shares the position of its first slot), 0 where it has none.
