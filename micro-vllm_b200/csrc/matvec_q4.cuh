@@ -142,9 +142,16 @@ __device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
     asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+// The aligned forms want a warp's lanes together, which a loop whose trip count
+// differs between them does not leave.
+__device__ __forceinline__ void mv_cluster_wait() {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void mv_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
-                 "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    mv_cluster_wait();
 }
 __device__ __forceinline__ uint32_t mv_cluster_addr(uint32_t addr, int rank) {
     uint32_t r;
@@ -920,6 +927,10 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
     asm("mov.u32 %0, %%clusterid.x;" : "=r"(cluster));
     asm("mov.u32 %0, %%nclusterid.x;" : "=r"(clusters));
+    // A peer's shared memory is there once the peer has started: every thread
+    // says so here and waits for the others before the first unit's sums.
+    if (ranks > 1)
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     float *ex = reinterpret_cast<float *>(mv_smem + pl.off_ex);
     float *red = reinterpret_cast<float *>(mv_smem + pl.off_red);
     int *list = reinterpret_cast<int *>(mv_smem + pl.off_list); // passes before each expert
@@ -1226,6 +1237,8 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
                         mv_store(y, pl.y_f32, at + q, v[q]);
             }
         };
+        if (ranks > 1 && u == u0)
+            mv_cluster_wait();
         for (int item = warp * 4 + sub; item < all; item += kMvWarps * 4) {
             const int r = item / blocks, o = (item - r * blocks) * 32 + o4;
             const float *at =
@@ -1276,6 +1289,8 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
             prologue(cur);
         }
     }
+    if (ranks > 1 && u0 >= u1) // without units the first wait is still owed
+        mv_cluster_wait();
 }
 
 } // namespace mvb

@@ -1,0 +1,40 @@
+"""Paths of the few-row products that only some plans or values take, on the
+device."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import routed_cases as rc  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+INT4, MXFP4 = rc.INT4, rc.MXFP4
+
+
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+def test_split_reduction_without_weights(moe, fmt):
+    """Long reductions of few outputs are split over a cluster's CTAs; experts
+    without a matrix have nothing to do before their sums (zeros) meet there,
+    right at the start."""
+    E, I, O = 6, 16384, 64
+    w, s = rc.packed(torch.Generator().manual_seed(1), fmt, O, I, "cuda")
+    none = torch.zeros(E, dtype=torch.int64, device="cuda")
+    some, scales = none.clone(), torch.full_like(none, s.data_ptr())
+    some[E - 1] = w.data_ptr()
+    nr = torch.ones(E, dtype=torch.int32, device="cuda")
+    xoff = torch.arange(E, dtype=torch.int32, device="cuda")
+    W = rc.decode(w, s, fmt, I)
+    for rows_in, rows_out, M, call in ((I, O, W.T, moe.expert_matvec_q4_dev),
+                                       (O, I, W, moe.expert_matvec_q4_grad_dev)):
+        x = torch.randn(E, rows_in, generator=torch.Generator().manual_seed(2)).cuda()
+        first = None
+        for _ in range(50):
+            y = torch.full((E, rows_out), 7.0, device="cuda")
+            call(fmt, x, none, scales, nr, xoff, y)
+            assert (y == 0).all()
+            call(fmt, x, some, scales, nr, xoff, y)
+            assert (y[:-1] == 0).all()
+            first = y.clone() if first is None else first
+            assert torch.equal(y, first), "the sums repeat to the bit"
+        want, size = x[-1].double() @ M, x[-1].double().abs() @ M.abs()
+        assert ((first[-1].double() - want).abs() <= (rows_in / 16 + 64) * 2.0 ** -22 * size).all()
