@@ -592,8 +592,8 @@ MVLLM_API int mvllm_matvec_q4_dev(void *stream, int fmt, const void *x, int x_dt
                                   const void *w, const void *scales, int S, int I, int O, void *y,
                                   int y_dtype, int64_t ldy);
 /* Its gradient for the rows, the weights being frozen: dx[r] = W^T dy[r],
- * dy [S, O], dx [S, I]; a pass serves 2 to 16 rows.  The products dy * scale of
- * int4 go in two bf16 parts where dx is bf16, in three where it is f32. */
+ * dy [S, O], dx [S, I]; a pass serves 8 or 16 rows (2 or 5 where f32 rows meet
+ * MXFP4).  The products dy * scale of int4 go in three bf16 parts, 24 bits. */
 MVLLM_API int mvllm_matvec_q4_grad_dev(void *stream, int fmt, const void *dy, int dy_dtype,
                                        int64_t lddy, const void *w, const void *scales, int S,
                                        int I, int O, void *dx, int dx_dtype, int64_t lddx);

@@ -66,9 +66,9 @@ struct MvCut {
     double ns = 1e30;
 };
 
-template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
+template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
     using F = MvFormat<FMT>;
-    static constexpr int T = MvTerms<FMT, TX, GRAD, FINE>::T, RP = 8 * NT / T;
+    static constexpr int T = MvTerms<FMT, TX, GRAD>::T, RP = 8 * NT / T;
     static constexpr int TILE = GRAD ? kMvCols : kMvRows, STEP = GRAD ? kMvRows : kMvCols;
     static constexpr int WARPS = mv_warps<NT, GRAD>(), THREADS = 32 * WARPS;
     static constexpr int RING = WARPS * mv_ring<NT, GRAD>() * F::STAGE;
@@ -83,7 +83,7 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
             p.off_red = at, at += red;
         at = (at + 127) & ~127;
         p.off_x = at;
-        at += (GRAD && FMT == MVLLM_FMT_INT4_G64 ? n : n * T) * mv_x_pitch<FMT, TX, GRAD>(cols);
+        at += n * T * mv_x_pitch<FMT, TX, GRAD>(cols);
         p.off_ex = at, at += GRAD ? 0 : cols / F::G * RP * 4;
         p.off_mail = at; // two buffers
         if (ranks > 1)
@@ -109,7 +109,8 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
         const double items = expected_passes(p.rows_most, nb, RP);
         const int tiles = (p.N + TILE - 1) / TILE, steps = (p.K + STEP - 1) / STEP;
         const double compute = // of a CTA's warps
-            GRAD ? (NT == 1 ? 25.0 : 21.0) : NT == 1 ? 42.0 : NT == 2 ? 28.0 : 17.0;
+            GRAD ? (FMT == MVLLM_FMT_INT4_G64 ? 18.0 : NT == 1 ? 25.0 : 21.0)
+                 : (NT == 1 ? 42.0 : NT == 2 ? 28.0 : 17.0);
         const double fill = GRAD ? 1.05 : 0.58;        // of its warps that reach it
         const double latency = GRAD ? 1200.0 : 580.0;  // of a stage, at least
         const double staging = GRAD ? (sizeof(TX) == 4 ? 2.9 : 13.0)
@@ -144,7 +145,8 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
                     const double stage = std::max(active * F::STAGE / rate, latency);
                     const double sums = wo * TILE * rows_most;
                     const double unit =
-                        GRAD ? 750.0 + sums * (0.09 * wk * T + 0.39) + (c > 1 ? 650.0 : 0.0)
+                        GRAD ? (FMT == MVLLM_FMT_INT4_G64 ? 1500.0 : 750.0) +
+                                   sums * (0.09 * wk * T + 0.39) + (c > 1 ? 650.0 : 0.0)
                              : 2800.0 + sums * 0.215 + (c > 1 ? 320.0 : 0.0);
                     // rows are staged once for the ranges that a cluster has of an
                     // item, or, in chunks, for every unit
@@ -195,7 +197,7 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
         return MVLLM_OK;
     }
     static const void *kernel() {
-        return reinterpret_cast<const void *>(matvec_q4_kernel<FMT, TX, NT, GRAD, FINE>);
+        return reinterpret_cast<const void *>(matvec_q4_kernel<FMT, TX, NT, GRAD>);
     }
 
     static int launch(cudaStream_t st, const MatvecArgs &a, MvCut cut, const void *x, int64_t ldx,
@@ -217,30 +219,32 @@ template <int FMT, typename TX, int NT, bool GRAD, bool FINE> struct MvHost {
         at[1].val.clusterDim.x = ranks, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
         cfg.attrs = at;
         cfg.numAttrs = 2;
-        MVB_TRY(cudaLaunchKernelEx(&cfg, matvec_q4_kernel<FMT, TX, NT, GRAD, FINE>, a, p,
+        MVB_TRY(cudaLaunchKernelEx(&cfg, matvec_q4_kernel<FMT, TX, NT, GRAD>, a, p,
                                    static_cast<const TX *>(x), ldx, y, ldy));
         return MVLLM_OK;
     }
 };
 
 // Rows that a pass over a matrix takes: all rows of a single matrix where 8,
-// 16 or 32 operand columns (gradient: 8 or 16) hold them, as many as that for
-// more.  Experts, whose rows differ, take the width whose plan has the lowest
-// estimate: 48 experts of 16 rows on average, 7168 -> 2048, take 183 us by 16
-// rows a pass and 253 by 32, 160 experts of 20, 6144 -> 1536, 614 and 462.
-template <int FMT, typename TX, bool GRAD, bool FINE>
+// 16 or 32 operand columns (gradient: 8 or 16; int4's: 8, its parts' sums need
+// the registers) hold them, as many as that for more.  Experts, whose rows
+// differ, take the width whose plan has the lowest estimate: 48 experts of 16
+// rows on average, 7168 -> 2048, take 183 us by 16 rows a pass and 253 by 32,
+// 160 experts of 20, 6144 -> 1536, 614 and 462.
+template <int FMT, typename TX, bool GRAD>
 int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, const DeviceScope &dev,
                 const void *x, int64_t ldx, void *y, int64_t ldy) {
-    constexpr int T = MvTerms<FMT, TX, GRAD, FINE>::T;
-    using One = MvHost<FMT, TX, 1, GRAD, FINE>;
-    using Two = MvHost<FMT, TX, 2, GRAD, FINE>;
-    using Four = MvHost<FMT, TX, GRAD ? 2 : 4, GRAD, FINE>;
+    constexpr int T = MvTerms<FMT, TX, GRAD>::T;
+    constexpr bool NARROW = GRAD && FMT == MVLLM_FMT_INT4_G64;
+    using One = MvHost<FMT, TX, 1, GRAD>;
+    using Two = MvHost<FMT, TX, NARROW ? 1 : 2, GRAD>;
+    using Four = MvHost<FMT, TX, NARROW ? 1 : GRAD ? 2 : 4, GRAD>;
     MvCut one, two, four;
     const bool some = a.nb > 1, wide = !GRAD && (some || a.rows > 16 / T);
-    if (some || a.rows <= 8 / T)
+    if (NARROW || some || a.rows <= 8 / T)
         if (int rc = One::cut_for(p, a.nb, dev, one))
             return rc;
-    if (some || (a.rows > 8 / T && !wide))
+    if (!NARROW && (some || (a.rows > 8 / T && !wide)))
         if (int rc = Two::cut_for(p, a.nb, dev, two))
             return rc;
     if (wide)
@@ -257,11 +261,8 @@ template <int FMT, typename TX>
 int matvec_way(cudaStream_t st, bool grad, const MatvecArgs &a, const MatvecPlan &p,
                const DeviceScope &dev, const void *x, int64_t ldx, void *y, int64_t ldy) {
     if (!grad)
-        return matvec_rows<FMT, TX, false, false>(st, a, p, dev, x, ldx, y, ldy);
-    if constexpr (FMT == MVLLM_FMT_INT4_G64 && sizeof(TX) == 2)
-        if (p.y_f32)
-            return matvec_rows<FMT, TX, true, true>(st, a, p, dev, x, ldx, y, ldy);
-    return matvec_rows<FMT, TX, true, false>(st, a, p, dev, x, ldx, y, ldy);
+        return matvec_rows<FMT, TX, false>(st, a, p, dev, x, ldx, y, ldy);
+    return matvec_rows<FMT, TX, true>(st, a, p, dev, x, ldx, y, ldy);
 }
 
 int matvec_any(const char *who, void *stream, bool grad, const MatvecArgs &a, const void *x,

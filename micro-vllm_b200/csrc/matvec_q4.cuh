@@ -94,18 +94,17 @@ template <int FMT> struct MvFormat {
     static constexpr int STAGE = kMvRows * (kMvCols / 2 + 16);
 };
 
-// Parts an x element is split into; 8 * NT operand columns hold 8 * NT / T
-// rows.
-template <int FMT, typename TX, bool GRAD, bool FINE> struct MvTerms {
+// Operand columns that an x element is split over; 8 * NT of them hold
+// 8 * NT / T rows.
+template <int FMT, typename TX, bool GRAD> struct MvTerms {
     static constexpr bool F32 = sizeof(TX) == 4;
     // forward: f16 parts, 11 bits each, scaled per group: bf16 fits one, f32
     // takes two (22 bits).  Gradient: bf16 parts, 8 bits each: bf16 rows of
-    // an MXFP4 matrix fit one, f32 takes three (24 bits); bf16 rows times an
-    // int4 matrix's f32 scales take three where the result is f32 (FINE), and
-    // two, 16 to 17 bits, where it is rounded to bf16's 8.
+    // an MXFP4 matrix fit one, f32 takes three (24 bits).  int4's f32 scales
+    // multiply the rows first; a product's three parts (24 bits) go through one
+    // column, one after another.
     static constexpr int T =
-        !GRAD ? (F32 ? 2 : 1)
-              : (F32 ? 3 : FMT == MVLLM_FMT_INT4_G64 ? (FINE ? 3 : 2) : 1);
+        !GRAD ? (F32 ? 2 : 1) : F32 && FMT != MVLLM_FMT_INT4_G64 ? 3 : 1;
 };
 
 __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src) {
@@ -362,13 +361,12 @@ __device__ __forceinline__ float trunc_bf16(float v) {
 // Part `term` of T of v (rounded to bf16 by the caller): leading 8 bits, the
 // next 8, the rest.  Infinities and NaN are all in the first.
 template <int T> __device__ __forceinline__ float mv_term(float v, int term) {
+    static_assert(T == 1 || T == 3, "parts");
     if (T == 1)
         return v;
     const bool fin = fabsf(v) <= 3.402823466e38f;
     const float h = fin ? trunc_bf16(v) : v;
-    float r = fin ? v - h : 0.f;
-    if (T == 2)
-        return term == 0 ? h : r;
+    const float r = fin ? v - h : 0.f;
     const float m = trunc_bf16(r);
     return term == 0 ? h : term == 1 ? m : r - m;
 }
@@ -414,7 +412,7 @@ __device__ __forceinline__ float exp2_int(int e) {
 template <int FMT, typename TX, int NT>
 __device__ __forceinline__ void mv_fetch_rows(uint8_t *xs, int pitch, const TX *x, int64_t ldx,
                                               int r0, int n, int c0, int cols, int K, bool vec) {
-    constexpr int T = MvTerms<FMT, TX, false, false>::T;
+    constexpr int T = MvTerms<FMT, TX, false>::T;
     static_assert(sizeof(TX) == 2 * T, "raw elements fit their parts' places");
     for (MvGroups<32 * mv_warps<NT, false>()> at(cols / 8); at.r < n; at.next()) {
         const TX *row = x + int64_t(r0 + at.r) * ldx;
@@ -437,7 +435,7 @@ __device__ __forceinline__ void mv_fetch_rows(uint8_t *xs, int pitch, const TX *
 template <int FMT, typename TX, int NT>
 __device__ __forceinline__ bool mv_stage_forward(uint8_t *xs, float *ex, int pitch, int n, int cols,
                                                  bool try_common, uint32_t *row_max) {
-    constexpr int T = MvTerms<FMT, TX, false, false>::T, RP = 8 * NT / T;
+    constexpr int T = MvTerms<FMT, TX, false>::T, RP = 8 * NT / T;
     constexpr int GL = MvFormat<FMT>::G / 8; // lanes of a group
     using Groups = MvGroups<32 * mv_warps<NT, false>()>;
     const int lane = threadIdx.x & 31;
@@ -523,8 +521,8 @@ template <int FMT, typename TX, int NT>
 __device__ __forceinline__ void mv_stage_gradient(uint8_t *xs, int pitch, const TX *x, int64_t ldx,
                                                   int r0, int n, int c0, int cols, int K, bool vec,
                                                   bool have, const MvHeld<TX, NT> &held) {
-    constexpr bool I4 = FMT == MVLLM_FMT_INT4_G64;
-    constexpr int T = I4 ? 1 : MvTerms<FMT, TX, true, false>::T; // int4: split later
+    constexpr bool I4 = FMT == MVLLM_FMT_INT4_G64; // split later
+    constexpr int T = MvTerms<FMT, TX, true>::T;
     held.each(x, ldx, r0, n, c0, cols, K, vec, have, [&](const Raw8<TX> &raw, int r, int q) {
         float v[8];
         raw.get(v);
@@ -577,7 +575,7 @@ __device__ __forceinline__ void mv_forward(uint32_t st, int half, const uint32_t
                                            const float *ex,
                                            float (&acc)[2][NT][4]) {
     using F = MvFormat<FMT>;
-    constexpr int T = MvTerms<FMT, TX, false, false>::T, RP = 8 * NT / T;
+    constexpr int T = MvTerms<FMT, TX, false>::T, RP = 8 * NT / T;
     constexpr int BPG = F::G / 32; // 32-column blocks of a group
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     float sc[2][2][kMvCols / F::G];
@@ -670,135 +668,137 @@ __device__ __forceinline__ void mv_forward(uint32_t st, int half, const uint32_t
 // columns (4 bytes) of rows t, t + 4, t + 8, t + 12 of each 16 and pairs two
 // rows' halfwords, after which the nibble extraction yields (row, row + 4)
 // pairs of one column: the transposition costs 4 byte permutes per 32
-// weights.  MXFP4's scale multiplies the bf16 weight, exact as a power of
-// two; int4's f32 scale multiplies the row's value, before it is split.
+// weights.
 //
-// int4's parts (`col` = this lane's operand column): its own part of a
-// product p is picked without a branch, hi = p's upper 16 bits, r = p - hi:
-// one of 1 * hi, 1 * r, ... by factors 0 and 1, exact.  A product that is not
-// finite comes out as NaN that way; the caller notices the NaN in its sums and
-// repeats the unit with CAREFUL, which keeps such a product whole in its first
-// part.  For MXFP4 CAREFUL stands for scale codes 0 and above 127, which the
-// short form of the scale's bits does not cover.
-template <int FMT, int T, int NT, bool CAREFUL>
-__device__ __forceinline__ void mv_gradient(uint32_t st, int half, const uint32_t (&xs)[NT],
-                                            float (&acc)[4][4][NT][4]) {
-    constexpr bool I4 = FMT == MVLLM_FMT_INT4_G64;
+// p[0]: columns 0..3 of rows (t, t + 4), p[1]: columns 4..7; p[2], p[3] of rows
+// (t + 8, t + 12); of the rows from kb * 16 on, column block h.
+__device__ __forceinline__ void mv_gradient_pairs(uint32_t st, int kb, int h, uint32_t (&p)[4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    float pick[NT][3]; // int4: factors of hi, r (T = 2) or hi, r, mid (T = 3)
+    uint32_t r[4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int term = (nt * 8 + g) % T;
-        pick[nt][0] = term == 0 ? 1.f : 0.f;
-        pick[nt][1] = term == T - 1 ? 1.f : 0.f;
-        pick[nt][2] = term == 1 ? 1.f : term == 2 ? -1.f : 0.f;
-    }
+    for (int j = 0; j < 4; ++j)
+        r[j] = lds32(st + mv_chunk(kb * 16 + t + 4 * j, h * 2 + (g >> 2)) + (g & 3) * 4);
+    p[0] = mv_prmt(r[0], r[1], 0x5410u), p[1] = mv_prmt(r[0], r[1], 0x7632u);
+    p[2] = mv_prmt(r[2], r[3], 0x5410u), p[3] = mv_prmt(r[2], r[3], 0x7632u);
+}
+
+// int4's f32 scale multiplies the row's value, and the product's three parts
+// (its upper 16 bits, those of what is left, the rest: 24 bits in all) are a
+// matrix instruction each.  (Two parts, 16 to 17 bits, show in a bf16 result:
+// ten times as many values one step off, 309 in place of 392 us on 512 rows of
+// 160 experts of 1536 x 6144.)  The first parts have sums of their own: the
+// matrix unit cuts what lies below a sum's last bit, and small parts added to
+// the large sum left 6.8e-7 of the result over 16384 rows, where this leaves
+// 9e-8.  A product that is not finite comes out as NaN; the caller notices the
+// NaN in its sums and repeats the unit with CAREFUL, which keeps such a product
+// whole in its first part.
+template <bool CAREFUL>
+__device__ __forceinline__ void mv_gradient_int4(uint32_t st, uint32_t xs,
+                                                 float (&acc)[4][4][2][4]) {
+    const int t = threadIdx.x & 3;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-        uint32_t sw[4][I4 ? 4 : 2];
+        const uint4 x = lds128(xs + kb * 64); // the rows' values
+        const float v[4] = {__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z),
+                            __uint_as_float(x.w)};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t at = st + kMvRows * 128 + (kb * 16 + t + 4 * j) * 16 + half;
-            if constexpr (I4) {
-                const uint4 v = lds128(at);
-                sw[j][0] = v.x, sw[j][1] = v.y, sw[j][2] = v.z, sw[j][3] = v.w;
-            } else {
-                const uint2 v = lds64(at);
-                sw[j][0] = v.x, sw[j][1] = v.y;
+        for (int h = 0; h < 4; ++h) {
+            uint32_t p[4], b[3][2];
+            float o[3][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float m = v[j] * __uint_as_float(lds32(st + kMvRows * 128 + 4 * h +
+                                                             (kb * 16 + t + 4 * j) * 16));
+                if constexpr (CAREFUL) {
+#pragma unroll
+                    for (int k = 0; k < 3; ++k)
+                        o[k][j] = mv_term<3>(m, k);
+                } else { // the packing takes the upper halves
+                    o[0][j] = m;
+                    o[1][j] = m - trunc_bf16(m);
+                    o[2][j] = o[1][j] - trunc_bf16(o[1][j]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                b[0][j] = mv_prmt(__float_as_uint(o[0][2 * j]), __float_as_uint(o[0][2 * j + 1]),
+                                  0x7632u);
+                b[1][j] = mv_prmt(__float_as_uint(o[1][2 * j]), __float_as_uint(o[1][2 * j + 1]),
+                                  0x7632u);
+                b[2][j] = pack_bf16(o[2][2 * j], o[2][2 * j + 1]);
+            }
+            mv_gradient_pairs(st, kb, h, p);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t a[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) // (128 + code) - 136
+                    a[j] = sub_bf16x2(((p[j] >> (4 * q)) & 0x000f000fu) | 0x43004300u, 0x43084308u);
+                mma_bf16_16816(acc[h][q][1], a[0], a[1], a[2], a[3], b[2][0], b[2][1]);
+                mma_bf16_16816(acc[h][q][0], a[0], a[1], a[2], a[3], b[0][0], b[0][1]);
+                mma_bf16_16816(acc[h][q][1], a[0], a[1], a[2], a[3], b[1][0], b[1][1]);
             }
         }
-        uint32_t bx[NT][2]; // MXFP4: the same for every column
-        float4 bv[NT];      // int4: the rows' values
+    }
+}
+
+// MXFP4's scale multiplies the bf16 weight, exact as a power of two.  CAREFUL
+// covers scale codes 0 and above 128, which the short form of the scale's bits
+// does not.
+template <int NT, bool CAREFUL>
+__device__ __forceinline__ void mv_gradient_mxfp4(uint32_t st, int half, const uint32_t (&xs)[NT],
+                                                  float (&acc)[4][4][NT][4]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        uint32_t sw[4][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint2 v = lds64(st + kMvRows * 128 + (kb * 16 + t + 4 * j) * 16 + half);
+            sw[j][0] = v.x, sw[j][1] = v.y;
+        }
+        uint32_t b[NT][2]; // the same for every column
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            if constexpr (I4) {
-                const uint4 v = lds128(xs[nt] + kb * 64);
-                bv[nt] = make_float4(__uint_as_float(v.x), __uint_as_float(v.y),
-                                     __uint_as_float(v.z), __uint_as_float(v.w));
-            } else {
-                const uint2 v = lds64(xs[nt] + kb * 32);
-                bx[nt][0] = v.x, bx[nt][1] = v.y;
-            }
+            const uint2 v = lds64(xs[nt] + kb * 32);
+            b[nt][0] = v.x, b[nt][1] = v.y;
         }
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
-            uint32_t r[4];
+            uint32_t p[4], m[2], m2[2] = {};
+            mv_gradient_pairs(st, kb, h, p);
+            // 2^(code - 1) = 2^126 * scale as bf16, the weight's bits being
+            // 2^-126 of its value: the code's exponent field plus 126.
+            // Codes above 128 take 2^126 and then the scale, 0 is 0.
+            const uint32_t sel = ((h & 1) * 2 + (g >> 2)) * 0x11u;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                r[j] = lds32(st + mv_chunk(kb * 16 + t + 4 * j, h * 2 + (g >> 2)) + (g & 3) * 4);
-            // p[0]: columns 0..3 of rows (t, t + 4), p[1]: columns 4..7;
-            // p[2], p[3] of rows (t + 8, t + 12).
-            const uint32_t p[4] = {mv_prmt(r[0], r[1], 0x5410u), mv_prmt(r[0], r[1], 0x7632u),
-                                   mv_prmt(r[2], r[3], 0x5410u), mv_prmt(r[2], r[3], 0x7632u)};
-            uint32_t m[2] = {}, m2[2] = {};
-            uint32_t b[NT][2];
-            if constexpr (I4) {
-                float s[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    s[j] = __uint_as_float(sw[j][h]);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const float v[4] = {bv[nt].x * s[0], bv[nt].y * s[1], bv[nt].z * s[2],
-                                        bv[nt].w * s[3]};
-                    float o[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if constexpr (CAREFUL) {
-                            o[j] = mv_term<T>(v[j], (nt * 8 + g) % T);
-                        } else {
-                            const float hi = trunc_bf16(v[j]), lo = v[j] - hi;
-                            o[j] = lo * pick[nt][1];
-                            if (T == 3)
-                                o[j] = fmaf(trunc_bf16(lo), pick[nt][2], o[j]);
-                            o[j] = fmaf(hi, pick[nt][0], o[j]);
-                        }
-                    }
-                    b[nt][0] = pack_bf16(o[0], o[1]);
-                    b[nt][1] = pack_bf16(o[2], o[3]);
+            for (int j = 0; j < 2; ++j) {
+                // byte k of the two rows' codes in the two halfwords
+                const uint32_t c = mv_prmt(sw[2 * j][h >> 1], sw[2 * j + 1][h >> 1],
+                                           sel | ((sel | 0x44u) << 8)) &
+                                   0x00ff00ffu;
+                if constexpr (CAREFUL) {
+                    const uint32_t lo = c & 255u, hi = c >> 16;
+                    m[j] = (lo ? 253u << 7 : 0u) | (hi ? 253u << 23 : 0u);
+                    m2[j] = (lo << 7) | (hi << 23);
+                } else {
+                    m[j] = c * 128u + ((126u << 7) | (126u << 23));
                 }
-            } else {
-                // 2^(code - 1) = 2^126 * scale as bf16, the weight's bits being
-                // 2^-126 of its value: the code's exponent field plus 126.
-                // Codes above 128 take 2^126 and then the scale, 0 is 0.
-                const uint32_t sel = ((h & 1) * 2 + (g >> 2)) * 0x11u;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    // byte k of the two rows' codes in the two halfwords
-                    const uint32_t c = mv_prmt(sw[2 * j][h >> 1], sw[2 * j + 1][h >> 1],
-                                               sel | ((sel | 0x44u) << 8)) &
-                                       0x00ff00ffu;
-                    if constexpr (CAREFUL) {
-                        const uint32_t lo = c & 255u, hi = c >> 16;
-                        m[j] = (lo ? 253u << 7 : 0u) | (hi ? 253u << 23 : 0u);
-                        m2[j] = (lo << 7) | (hi << 23);
-                    } else {
-                        m[j] = c * 128u + ((126u << 7) | (126u << 23));
-                    }
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    b[nt][0] = bx[nt][0], b[nt][1] = bx[nt][1];
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 uint32_t a[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if constexpr (I4) {
-                        const uint32_t v = ((p[j] >> (4 * q)) & 0x000f000fu) | 0x43004300u;
-                        a[j] = sub_bf16x2(v, 0x43084308u); // (128 + code) - 136
-                    } else {
-                        const uint32_t mag = q == 0   ? p[j] << 6
-                                             : q == 1 ? p[j] << 2
-                                             : q == 2 ? p[j] >> 2
-                                                      : p[j] >> 6;
-                        const uint32_t v = (mag & 0x01c001c0u) |
-                                           ((p[j] << (12 - 4 * q)) & 0x80008000u);
-                        a[j] = mul_bf16x2(v, m[j >> 1]);
-                        if constexpr (CAREFUL)
-                            a[j] = mul_bf16x2(a[j], m2[j >> 1]);
-                    }
+                    const uint32_t mag = q == 0   ? p[j] << 6
+                                         : q == 1 ? p[j] << 2
+                                         : q == 2 ? p[j] >> 2
+                                                  : p[j] >> 6;
+                    const uint32_t v = (mag & 0x01c001c0u) |
+                                       ((p[j] << (12 - 4 * q)) & 0x80008000u);
+                    a[j] = mul_bf16x2(v, m[j >> 1]);
+                    if constexpr (CAREFUL)
+                        a[j] = mul_bf16x2(a[j], m2[j >> 1]);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -823,7 +823,7 @@ template <int FMT, typename TX, int NT, bool GRAD> constexpr int mv_red_pitch() 
     return GRAD ? kMvCols + 1 : 36;
 }
 template <int FMT, typename TX, int NT, bool GRAD> constexpr int mv_red_size() {
-    return (GRAD ? 8 * NT : 8 * NT / MvTerms<FMT, TX, GRAD, false>::T) *
+    return (GRAD ? 8 * NT : 8 * NT / MvTerms<FMT, TX, GRAD>::T) *
            mv_red_pitch<FMT, TX, NT, GRAD>();
 }
 template <int FMT, typename TX, bool GRAD> __host__ __device__ constexpr int mv_x_pitch(int cols) {
@@ -879,9 +879,9 @@ __device__ __forceinline__ void mv_put(float *to, const float (&acc)[2][NT][4], 
             }
         }
 }
-// The gradient's: [part of a row][output].
-template <int RPITCH, int NT>
-__device__ __forceinline__ void mv_put_gradient(float *to, const float (&acc)[4][4][NT][4]) {
+// The gradient's: [part of a row][output], int4's two sums of a row as one.
+template <int RPITCH, int NT, int SUMS>
+__device__ __forceinline__ void mv_put_gradient(float *to, const float (&acc)[4][4][SUMS][4]) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
 #pragma unroll
     for (int h = 0; h < 4; ++h)
@@ -889,7 +889,10 @@ __device__ __forceinline__ void mv_put_gradient(float *to, const float (&acc)[4]
         for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float(&d)[4] = acc[h][q][nt];
+                float d[4];
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    d[s] = SUMS > NT ? acc[h][q][0][s] + acc[h][q][1][s] : acc[h][q][nt][s];
                 float *at = to + (nt * 8 + 2 * t) * RPITCH + h * 64 + 8 * g + q;
                 at[0] = d[0], at[RPITCH] = d[1];
                 at[4] = d[2], at[RPITCH + 4] = d[3];
@@ -908,12 +911,12 @@ struct MvUnit {
 // the main loop has no barrier (a stage takes a warp about 2 us).  The wk x
 // cluster partial sums of an output meet in (distributed) shared memory and are
 // added in a fixed order.
-template <int FMT, typename TX, int NT, bool GRAD, bool FINE>
+template <int FMT, typename TX, int NT, bool GRAD>
 __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
     matvec_q4_kernel(const MatvecArgs a, const MatvecPlan pl, const TX *__restrict__ x,
                      int64_t ldx, void *__restrict__ y, int64_t ldy) {
     using F = MvFormat<FMT>;
-    constexpr int T = MvTerms<FMT, TX, GRAD, FINE>::T, RP = 8 * NT / T, ST = mv_ring<NT, GRAD>();
+    constexpr int T = MvTerms<FMT, TX, GRAD>::T, RP = 8 * NT / T, ST = mv_ring<NT, GRAD>();
     constexpr int kMvWarps = mv_warps<NT, GRAD>(), kMvThreads = 32 * kMvWarps;
     constexpr int TILE = GRAD ? kMvCols : kMvRows, STEP = GRAD ? kMvRows : kMvCols;
     constexpr int RPITCH = mv_red_pitch<FMT, TX, NT, GRAD>();
@@ -1092,21 +1095,18 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
         const int tasks = tasks_of(cur);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            int col = nt * 8 + (lane >> 2);
-            if (GRAD && FMT == MVLLM_FMT_INT4_G64)
-                col = min(col / T, cur.n - 1);
-            else
-                col = min(col, cur.n * T - 1);
+            const int col = min(nt * 8 + (lane >> 2), cur.n * T - 1);
             xcol[nt] = xs + col * pitch + (lane & 3) * (GRAD ? 4 * XB : 16);
         }
         // The gradient's one task per warp keeps its sums to the end of the
         // unit; the forward's tasks leave theirs in shared memory one by one.
-        float accg[GRAD ? 4 : 1][GRAD ? 4 : 1][NT][4];
+        constexpr int SUMS = GRAD && FMT == MVLLM_FMT_INT4_G64 ? 2 : NT; // int4: of first parts, of others
+        float accg[GRAD ? 4 : 1][GRAD ? 4 : 1][SUMS][4];
         for (bool careful = false;; careful = true) {
             bool refilled = false;
             if constexpr (GRAD) {
 #pragma unroll
-                for (int i = 0; i < 16 * NT * 4; ++i)
+                for (int i = 0; i < 16 * SUMS * 4; ++i)
                     (&accg[0][0][0][0])[i] = 0.f;
             }
             for (int c0 = 0; c0 < nk; c0 += pl.chunk) {
@@ -1163,12 +1163,17 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
                             xat[nt] = xcol[nt] + step * (STEP * XB);
-                        if constexpr (GRAD)
-                            if (careful || (FMT == MVLLM_FMT_MXFP4 && mv_odd_codes(st, half)))
-                                mv_gradient<FMT, T, NT, true>(st, half, xat, accg);
+                        if constexpr (GRAD && FMT == MVLLM_FMT_INT4_G64) {
+                            if (careful)
+                                mv_gradient_int4<true>(st, xat[0], accg);
                             else
-                                mv_gradient<FMT, T, NT, false>(st, half, xat, accg);
-                        else if (common)
+                                mv_gradient_int4<false>(st, xat[0], accg);
+                        } else if constexpr (GRAD) {
+                            if (mv_odd_codes(st, half))
+                                mv_gradient_mxfp4<NT, true>(st, half, xat, accg);
+                            else
+                                mv_gradient_mxfp4<NT, false>(st, half, xat, accg);
+                        } else if (common)
                             mv_forward<FMT, TX, NT, true>(st, half, xat, ex, accf);
                         else
                             mv_forward<FMT, TX, NT, false>(
@@ -1183,7 +1188,7 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
                 break;
             float nan = 0.f; // NaN where a sum is, or where infinities meet
 #pragma unroll
-            for (int i = 0; i < (GRAD ? 16 * NT * 4 : 0); ++i)
+            for (int i = 0; i < (GRAD ? 16 * SUMS * 4 : 0); ++i)
                 nan += (&accg[0][0][0][0])[i];
             if (!__syncthreads_or(nan != nan))
                 break;
@@ -1196,7 +1201,7 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
             mv_wait<0>();
             __syncthreads(); // the ring is done with before the sums overlay it
             if (warp < tasks)
-                mv_put_gradient<RPITCH>(red + warp * RSIZE, accg);
+                mv_put_gradient<RPITCH, NT>(red + warp * RSIZE, accg);
             __syncthreads();
         } else {
             // A warp that is done goes on to the next unit's weights; its rows

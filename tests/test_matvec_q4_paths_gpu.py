@@ -38,3 +38,39 @@ def test_split_reduction_without_weights(moe, fmt):
             assert torch.equal(y, first), "the sums repeat to the bit"
         want, size = x[-1].double() @ M, x[-1].double().abs() @ M.abs()
         assert ((first[-1].double() - want).abs() <= (rows_in / 16 + 64) * 2.0 ** -22 * size).all()
+
+
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+@pytest.mark.parametrize("S,I,O", [(1, 7168, 2048), (3, 1000, 130), (7, 2050, 66), (16, 1536, 6144),
+                                   (40, 512, 1024)])
+def test_bf16_results_are_the_f32_ones_rounded(moe, S, I, O, fmt):
+    """The sums do not depend on the type they are rounded to: bf16 rows give
+    the same f32 sums whether these are stored or rounded once."""
+    gen = torch.Generator().manual_seed(S + I + O)
+    w, s = rc.packed(gen, fmt, O, I, "cuda")
+    for n, m, call in ((I, O, moe.matvec_q4_dev), (O, I, moe.matvec_q4_grad_dev)):
+        x = torch.randn(S, n, generator=gen).cuda().to(BF16)
+        wide, narrow = torch.empty(S, m, device="cuda"), torch.empty(S, m, device="cuda").to(BF16)
+        call(fmt, x, w, s, wide)
+        call(fmt, x, w, s, narrow)
+        assert torch.equal(narrow, wide.to(BF16))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+@pytest.mark.parametrize("n", [7168, 16384])
+def test_long_sums_are_as_exact_as_f32_products(moe, n, fmt, dtype):
+    """Sums over long rows, f32 results: the error in norm against 64 bits is no
+    larger than that of an f32 product of the decoded weights (1.5 times, the
+    spread of an error that is random)."""
+    S, m = 6, 512
+    gen = torch.Generator().manual_seed(n)
+    x = torch.randn(S, n, generator=gen).cuda().to(dtype)
+    for O, I, call in ((m, n, moe.matvec_q4_dev), (n, m, moe.matvec_q4_grad_dev)):
+        w, s = rc.packed(gen, fmt, O, I, "cuda", spread=0)
+        W = rc.decode(w, s, fmt, I)
+        W = W.T if O == m else W
+        y = torch.empty(S, m, device="cuda")
+        call(fmt, x, w, s, y)
+        want, plain = x.double() @ W, x.float() @ W.float()
+        assert (y.double() - want).norm() <= 1.5 * (plain.double() - want).norm()
