@@ -401,10 +401,18 @@ __device__ __forceinline__ float exp2_int(int e) {
 // (int4: in its nibble pair order), and 2^-e in ex.  f16's 30 binades hold a
 // row of activations with one e for all its columns; that is checked: where
 // every scale group's largest finite value (or zero) lies within 2^-12 of its
-// row's, `common` is returned and ex[row] = 2^-e, else e goes by group,
-// ex[group][row].  Either way a group's largest scaled value is at least 4,
-// and what the parts leave of an element is at most 2^-22 of it (nothing, for
-// bf16) or 2^-25, f16's last step: below 2^-26 of the group's largest.
+// row's, and that is below 2^31, `common` is returned and ex[row] = 2^-e, else
+// e goes by group, ex[group][row].  Either way the largest scaled value of a
+// group whose largest is at least 2^-112 is at least 4 (below, e stops at
+// 126), and what the parts leave of an element is at most 2^-22 of it (nothing,
+// for bf16) or 2^-25, f16's last step: below 2^-26 of the group's largest.
+//
+// The factors come in where no sum leaves f32's range before its result does:
+// by group, d 2^-e first and then the weights' scale; where a group's largest
+// is 2^112 or more (`wide`) 2^-e in two steps, before and after the scale.  A
+// common 2^-e follows after all columns, which is checked at the end: sums that
+// are not finite are taken again by group.  (Up to 2^31, what a scale below
+// 2^-126 loses before the factor stays below f32's smallest normal value.)
 //
 // The elements come first, as they are, to the places of their parts, which
 // take as many bytes (mv_fetch_rows, asynchronous where rows are aligned);
@@ -434,7 +442,7 @@ __device__ __forceinline__ void mv_fetch_rows(uint8_t *xs, int pitch, const TX *
 }
 template <int FMT, typename TX, int NT>
 __device__ __forceinline__ bool mv_stage_forward(uint8_t *xs, float *ex, int pitch, int n, int cols,
-                                                 bool try_common, uint32_t *row_max) {
+                                                 bool try_common, uint32_t *row_max, bool &wide) {
     constexpr int T = MvTerms<FMT, TX, false>::T, RP = 8 * NT / T;
     constexpr int GL = MvFormat<FMT>::G / 8; // lanes of a group
     using Groups = MvGroups<32 * mv_warps<NT, false>()>;
@@ -450,6 +458,7 @@ __device__ __forceinline__ bool mv_stage_forward(uint8_t *xs, float *ex, int pit
     // row_max[r]: bits of the row's largest finite value; [RP + r]: of its
     // smallest nonzero group maximum.
     bool common = false;
+    wide = false;
     if (try_common) {
         for (Groups at(cols / 8); at.r < n; at.next()) {
             float v[8];
@@ -472,7 +481,7 @@ __device__ __forceinline__ bool mv_stage_forward(uint8_t *xs, float *ex, int pit
         bool fits = true;
         if (int(threadIdx.x) < n) {
             const float m = __uint_as_float(row_max[threadIdx.x]);
-            fits = __uint_as_float(row_max[RP + threadIdx.x]) >= m * 0x1p-12f;
+            fits = __uint_as_float(row_max[RP + threadIdx.x]) >= m * 0x1p-12f && m < 0x1p31f;
             ex[threadIdx.x] = exp2_int(-mv_shift(m));
         }
         common = __syncthreads_and(fits);
@@ -489,6 +498,7 @@ __device__ __forceinline__ bool mv_stage_forward(uint8_t *xs, float *ex, int pit
             for (int o = 1; o < GL; o <<= 1)
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             sh = mv_shift(m);
+            wide |= m >= 0x1p112f;
             if ((at.q & (GL - 1)) == 0)
                 ex[(at.q / GL) * RP + at.r] = exp2_int(-sh);
         }
@@ -570,7 +580,8 @@ __device__ __forceinline__ void mv_int4x8(uint32_t w, uint32_t (&h)[4]) {
 // of every 32 columns, its own 8: their order along the MMA's K is the same
 // for both operands, so no nibble moves between lanes.  Each scale group's
 // sum starts from zero and is scaled into the f32 accumulator.
-template <int FMT, typename TX, int NT, bool COMMON>
+enum MvFactor { kMvGroup, kMvCommon, kMvWide }; // where 2^-e comes in (mv_stage_forward)
+template <int FMT, typename TX, int NT, MvFactor FACTOR>
 __device__ __forceinline__ void mv_forward(uint32_t st, int half, const uint32_t (&xs)[NT],
                                            const float *ex,
                                            float (&acc)[2][NT][4]) {
@@ -633,13 +644,26 @@ __device__ __forceinline__ void mv_forward(uint32_t st, int half, const uint32_t
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            if constexpr (COMMON) { // the columns' factors follow at the end
+            if constexpr (FACTOR == kMvCommon) { // the columns' factors follow at the end
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
                     ffma2(acc[mt][nt][0], acc[mt][nt][1], d[mt][nt][0], d[mt][nt][1],
                           sc[mt][0][gr]);
                     ffma2(acc[mt][nt][2], acc[mt][nt][3], d[mt][nt][2], d[mt][nt][3],
                           sc[mt][1][gr]);
+                }
+            } else if constexpr (FACTOR == kMvWide) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (T == 2 && (q & 1))
+                        continue;
+                    const float e = ex[gr * RP + (T == 1 ? nt * 8 + 2 * t + (q & 1) : nt * 4 + t)];
+                    const float e0 = fminf(e, 0x1p64f), e1 = fmaxf(e * 0x1p-64f, 1.f);
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt) {
+                        const float v = T == 1 ? d[mt][nt][q] : d[mt][nt][q] + d[mt][nt][q + 1];
+                        acc[mt][nt][q] = fmaf(v * e0 * sc[mt][q >> 1][gr], e1, acc[mt][nt][q]);
+                    }
                 }
             } else if constexpr (T == 1) {
                 const float2 e = *reinterpret_cast<const float2 *>(ex + gr * RP + nt * 8 + 2 * t);
@@ -844,11 +868,12 @@ __device__ __forceinline__ void mv_store(void *y, int f32, int64_t at, float v) 
 }
 
 // A task's partial sums to shared memory, [row of x][output] (f32 rows: their
-// two parts added), times the rows' factors where those were left out; on top
-// of what an earlier chunk left there when `add`.
+// two parts added), times the rows' factors where those were left out (`check`
+// becomes NaN where a sum before them is not finite); on top of what an earlier
+// chunk left there when `add`.
 template <int T, int RPITCH, int NT>
 __device__ __forceinline__ void mv_put(float *to, const float (&acc)[2][NT][4], const float *ex,
-                                       bool add) {
+                                       bool add, float &check) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
@@ -860,6 +885,7 @@ __device__ __forceinline__ void mv_put(float *to, const float (&acc)[2][NT][4], 
                 d[q] = acc[mt][nt][q];
             if (T == 1) {
                 if (ex) {
+                    check = fmaf(d[0] + d[1] + d[2] + d[3], 0.f, check);
                     const float2 e = *reinterpret_cast<const float2 *>(ex + nt * 8 + 2 * t);
                     d[0] *= e.x, d[1] *= e.y, d[2] *= e.x, d[3] *= e.y;
                 }
@@ -870,8 +896,9 @@ __device__ __forceinline__ void mv_put(float *to, const float (&acc)[2][NT][4], 
                 at[RPITCH + 8] = add ? at[RPITCH + 8] + d[3] : d[3];
             } else {
                 if (ex) {
-                    const float e = ex[nt * 4 + t];
-                    d[0] = (d[0] + d[1]) * e, d[2] = (d[2] + d[3]) * e;
+                    const float e = ex[nt * 4 + t], s0 = d[0] + d[1], s1 = d[2] + d[3];
+                    check = fmaf(s0 + s1, 0.f, check);
+                    d[0] = s0 * e, d[2] = s1 * e;
                 }
                 float *at = to + (nt * 4 + t) * RPITCH + mt * 16 + g;
                 at[0] = add ? at[0] + d[0] : d[0];
@@ -1062,7 +1089,7 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
     constexpr int XB = GRAD ? (FMT == MVLLM_FMT_INT4_G64 ? 4 : 2) : 2; // bytes of an element
     uint32_t xcol[NT];
     int staged = -1;     // the item whose only chunk is staged
-    bool common = false; // its rows have one power of two each
+    MvFactor factor = kMvGroup; // how its rows are scaled
     int turn = 0;        // the mail buffer of this unit
     __shared__ uint32_t row_max[GRAD ? 1 : 2 * RP];
     MvHeld<TX, NT> held; // gradient
@@ -1102,6 +1129,8 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
         // unit; the forward's tasks leave theirs in shared memory one by one.
         constexpr int SUMS = GRAD && FMT == MVLLM_FMT_INT4_G64 ? 2 : NT; // int4: of first parts, of others
         float accg[GRAD ? 4 : 1][GRAD ? 4 : 1][SUMS][4];
+        MvUnit next{};
+        float check = 0.f; // NaN where a sum before its factor is not finite
         for (bool careful = false;; careful = true) {
             bool refilled = false;
             if constexpr (GRAD) {
@@ -1111,6 +1140,7 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
             }
             for (int c0 = 0; c0 < nk; c0 += pl.chunk) {
                 if (cur.w && staged != cur.item) { // uniform over the CTA
+                    bool wide = false;
                     if constexpr (GRAD) {
                         __syncthreads(); // the last readers of x are done
                         mv_stage_gradient<FMT, TX, NT>(mv_smem + pl.off_x, pitch, x, ldx, cur.r0,
@@ -1133,11 +1163,14 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
                                 mv_wait<0>();
                         }
                         __syncthreads();
-                        common = mv_stage_forward<FMT, TX, NT>(
-                            mv_smem + pl.off_x, ex, pitch, cur.n, cols,
-                            pl.try_common && nk <= pl.chunk, row_max);
+                        factor = mv_stage_forward<FMT, TX, NT>(
+                                     mv_smem + pl.off_x, ex, pitch, cur.n, cols,
+                                     pl.try_common && nk <= pl.chunk, row_max, wide)
+                                     ? kMvCommon
+                                     : kMvGroup;
                     }
-                    __syncthreads();
+                    if (__syncthreads_or(wide))
+                        factor = kMvWide;
                     if (nk <= pl.chunk)
                         staged = cur.item;
                 }
@@ -1173,18 +1206,42 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
                                 mv_gradient_mxfp4<NT, true>(st, half, xat, accg);
                             else
                                 mv_gradient_mxfp4<NT, false>(st, half, xat, accg);
-                        } else if (common)
-                            mv_forward<FMT, TX, NT, true>(st, half, xat, ex, accf);
-                        else
-                            mv_forward<FMT, TX, NT, false>(
-                                st, half, xat, ex + step * (STEP / F::G) * RP, accf);
+                        } else {
+                            const float *at = ex + step * (STEP / F::G) * RP;
+                            if (factor == kMvCommon)
+                                mv_forward<FMT, TX, NT, kMvCommon>(st, half, xat, ex, accf);
+                            else if (factor == kMvGroup)
+                                mv_forward<FMT, TX, NT, kMvGroup>(st, half, xat, at, accf);
+                            else
+                                mv_forward<FMT, TX, NT, kMvWide>(st, half, xat, at, accf);
+                        }
                     }
                     __syncwarp();
                     if constexpr (!GRAD)
-                        mv_put<T, RPITCH>(red + task * RSIZE, accf, common ? ex : nullptr, c0 > 0);
+                        mv_put<T, RPITCH>(red + task * RSIZE, accf,
+                                          factor == kMvCommon ? ex : nullptr, c0 > 0, check);
                 }
             }
-            if (!GRAD || FMT != MVLLM_FMT_INT4_G64 || careful)
+            if constexpr (!GRAD) {
+                // A warp that is done goes on to the next unit's weights; its rows
+                // wait until their places are free.
+                __syncwarp();
+                if (u + 1 < u1) {
+                    next = decode(u + 1);
+                    prologue(next);
+                }
+                if (!__syncthreads_or(check != check))
+                    break;
+                // Again with the rows' common factors as every group's.
+                for (int i = RP + threadIdx.x; i < cols / F::G * RP; i += kMvThreads)
+                    ex[i] = ex[i % RP];
+                factor = kMvGroup, check = 0.f;
+                mv_wait<0>(); // the stage just asked for: its place is needed
+                __syncthreads();
+                prologue(cur);
+                continue;
+            }
+            if (FMT != MVLLM_FMT_INT4_G64 || careful)
                 break;
             float nan = 0.f; // NaN where a sum is, or where infinities meet
 #pragma unroll
@@ -1194,24 +1251,16 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
                 break;
             prologue(cur);
         }
-        MvUnit next{};
-        if (u + 1 < u1)
-            next = decode(u + 1);
         if constexpr (GRAD) {
+            if (u + 1 < u1)
+                next = decode(u + 1);
             mv_wait<0>();
             __syncthreads(); // the ring is done with before the sums overlay it
             if (warp < tasks)
                 mv_put_gradient<RPITCH, NT>(red + warp * RSIZE, accg);
             __syncthreads();
-        } else {
-            // A warp that is done goes on to the next unit's weights; its rows
-            // wait until their places are free.
-            __syncwarp();
-            if (u + 1 < u1)
-                prologue(next);
-            __syncthreads();
-            if (u + 1 < u1)
-                fetch(next);
+        } else if (u + 1 < u1) {
+            fetch(next);
         }
         // The CTA's own wk partial sums (and the gradient's parts) first.  With
         // one CTA per cluster that is the result; else it goes to the CTA that

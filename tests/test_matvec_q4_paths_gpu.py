@@ -74,3 +74,71 @@ def test_long_sums_are_as_exact_as_f32_products(moe, n, fmt, dtype):
         call(fmt, x, w, s, y)
         want, plain = x.double() @ W, x.float() @ W.float()
         assert (y.double() - want).norm() <= 1.5 * (plain.double() - want).norm()
+
+
+def rows_of(gen, exponents, n, dtype):
+    """Rows of normal values, each times its power of two."""
+    x = torch.randn(len(exponents), n, generator=gen)
+    return (x * torch.exp2(torch.tensor(exponents, dtype=torch.float32))[:, None]).cuda().to(dtype)
+
+
+def close(got, x, M, what):
+    """Terms pass through at most length / 16 + 64 additions, each off by 2^-22
+    of the magnitudes or, where they are that small, by half of f32's last step,
+    2^-149; the result rounds once."""
+    want, size = x.double() @ M, x.double().abs() @ M.abs()
+    n = (x.shape[1] / 16 + 64) * (2.0 ** -22 * size + 2.0 ** -150)
+    off = (got.double() - want).abs()
+    assert (off <= n + rc.half_step(got.dtype) * (want.abs() + n)).all(), what
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+@pytest.mark.parametrize("rows,scale", [([-100, -20, 0, 2], 109), ([0, -3], 116),
+                                        ([120, 100, 0, -30], -117), ([30, 31, 33], -60),
+                                        ([-126, -120], 30), ([118], -126)])
+@pytest.mark.parametrize("I,O", [(7168, 16384), (1024, 96)])
+def test_finite_results_of_far_scales(moe, I, O, rows, scale, fmt, dtype):
+    """Rows and scales at the two ends of f32's range whose results lie inside
+    it: the sums on the way stay finite too, in a product whose rows are
+    surveyed and in a short one."""
+    gen = torch.Generator().manual_seed(I + scale)
+    w, s = rc.packed(gen, fmt, O, I, "cuda", spread=0)
+    if fmt == INT4:
+        s = s * 2.0 ** 6 * 2.0 ** scale if scale < 120 else s
+    else:
+        s.fill_(127 + scale)
+    x = rows_of(gen, rows, I, dtype)
+    y = torch.empty(len(rows), O, device="cuda")
+    moe.matvec_q4_dev(fmt, x, w, s, y)
+    W = rc.decode(w, s, fmt, I)
+    want = x.double() @ W.T
+    live = want.abs() < 3e38
+    assert live.float().mean() > 0.9 and torch.isfinite(y[live]).all()
+    close(torch.where(live, y.double(), want), x, W.T, "forward")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+@pytest.mark.parametrize("I,O", [(7168, 16384), (192, 40)])
+def test_group_sums_beyond_f32(moe, I, O, fmt, dtype):
+    """Rows whose products with the codes leave f32's range before the scale
+    brings them back, beside rows that a factor in two steps must not lose."""
+    gen = torch.Generator().manual_seed(I)
+    w, s = rc.packed(gen, fmt, O, I, "cuda", spread=0)
+    w.fill_(0x77 if fmt == MXFP4 else 0xFF)  # every weight 6, or 7
+    if fmt == INT4:
+        s.fill_(2.0 ** -118)
+    else:
+        s.fill_(9)
+    x = torch.ones(4, I)
+    x[0] *= 2.0 ** 127
+    x[1] *= -(2.0 ** 126)
+    x[1, 64:] = 2.0 ** -100  # one group apart from the others
+    x[2] = torch.randn(I, generator=gen)
+    x[3] = 2.0 ** 90
+    x = x.cuda().to(dtype)
+    y = torch.empty(4, O, device="cuda")
+    moe.matvec_q4_dev(fmt, x, w, s, y)
+    assert torch.isfinite(y).all()
+    close(y, x, rc.decode(w, s, fmt, I).T, "forward")
