@@ -74,21 +74,23 @@ template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
     static constexpr int RING = WARPS * mv_ring<NT, GRAD>() * F::STAGE;
     static constexpr int RED = mv_red_size<FMT, TX, NT, GRAD>() * 4; // bytes of a task's sums
 
-    // Shared memory for `chunk` staged stages; fills the plan's offsets.
-    static int layout(MatvecPlan &p, int chunk, int ranks, int nb) {
-        const int cols = chunk * STEP, n = std::min(RP, p.rows_most), red = p.wo * p.wk * RED;
-        int at = mv_alias<GRAD>() ? std::max(RING, red) : RING;
+    // Shared memory for `chunk` staged stages, whose rows may pass 2^31 bytes;
+    // fills the plan's offsets, which hold where the answer fits the SM.
+    static int64_t layout(MatvecPlan &p, int chunk, int ranks, int nb) {
+        const int64_t cols = int64_t(chunk) * STEP;
+        const int n = std::min(RP, p.rows_most), red = p.wo * p.wk * RED;
+        int64_t at = mv_alias<GRAD>() ? std::max(RING, red) : RING;
         p.off_red = 0;
         if (!mv_alias<GRAD>())
-            p.off_red = at, at += red;
+            p.off_red = int(at), at += red;
         at = (at + 127) & ~127;
-        p.off_x = at;
+        p.off_x = int(at);
         at += n * T * mv_x_pitch<FMT, TX, GRAD>(cols);
-        p.off_ex = at, at += GRAD ? 0 : cols / F::G * RP * 4;
-        p.off_mail = at; // two buffers
+        p.off_ex = int(at), at += GRAD ? 0 : cols / F::G * RP * 4;
+        p.off_mail = int(at); // two buffers
         if (ranks > 1)
             at += 2 * ((p.wo * TILE / 32 * RP + ranks - 1) / ranks) * ranks * 128;
-        p.off_list = at, at += (nb + 1) * 4;
+        p.off_list = int(at), at += (nb + 1) * 4;
         p.chunk = chunk;
         return at;
     }
@@ -204,13 +206,14 @@ template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
                       void *y, int64_t ldy) {
         MatvecPlan &p = cut.p;
         const int ranks = cut.ranks;
-        const int smem = layout(p, p.chunk, ranks, a.nb);
+        const int64_t smem = layout(p, p.chunk, ranks, a.nb);
         if (p.range < 1 || smem > kMvSmem)
-            return host_fail(MVLLM_ERR_UNSUPPORTED, "matvec_q4: %d bytes of shared memory", smem);
+            return host_fail(MVLLM_ERR_UNSUPPORTED, "matvec_q4: %lld bytes of shared memory",
+                             static_cast<long long>(smem));
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(cut.grid);
         cfg.blockDim = dim3(THREADS);
-        cfg.dynamicSmemBytes = smem;
+        cfg.dynamicSmemBytes = size_t(smem);
         cfg.stream = st;
         cudaLaunchAttribute at[2];
         at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -67,7 +67,7 @@ constexpr int kMvRows = 32, kMvCols = 256; // weights of a warp's stage
 constexpr int kMvMaxExperts = 1024;
 constexpr int kMvMaxSide = 1 << 30; // rows and columns: steps past them stay in 32 bits
 
-// How a launch cuts its work, filled by the host (matvec_plan).
+// How a launch cuts its work, filled by the host (MvHost::plan).
 struct MatvecPlan {
     int N, K;      // outputs and reduction length: (O, I) forward, (I, O) gradient
     int range;     // outputs of a unit
@@ -850,7 +850,8 @@ template <int FMT, typename TX, int NT, bool GRAD> constexpr int mv_red_size() {
     return (GRAD ? 8 * NT : 8 * NT / MvTerms<FMT, TX, GRAD>::T) *
            mv_red_pitch<FMT, TX, NT, GRAD>();
 }
-template <int FMT, typename TX, bool GRAD> __host__ __device__ constexpr int mv_x_pitch(int cols) {
+template <int FMT, typename TX, bool GRAD, typename Int>
+__host__ __device__ constexpr Int mv_x_pitch(Int cols) {
     // Row pitch of the staged x: the lanes of one shared-memory phase fall
     // into different banks.
     if (!GRAD)

@@ -142,3 +142,23 @@ def test_group_sums_beyond_f32(moe, I, O, fmt, dtype):
     moe.matvec_q4_dev(fmt, x, w, s, y)
     assert torch.isfinite(y).all()
     close(y, x, rc.decode(w, s, fmt, I).T, "forward")
+
+
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+def test_reductions_past_the_address_arithmetic(moe, fmt):
+    """Rows whose staged form would pass 2^31 bytes: they are staged in chunks."""
+    n, m, S = (1 << 25) + 40, 6, 32
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for O, I, call in ((m, n, moe.matvec_q4_dev), (n, m, moe.matvec_q4_grad_dev)):
+        w = torch.randint(0, 256, (O, (I + 1) // 2), generator=g, dtype=torch.uint8, device="cuda")
+        if fmt == INT4:
+            s = torch.rand(O, (I + 63) // 64, generator=g, device="cuda") * 0.01 + 1e-4
+        else:
+            s = torch.randint(113, 126, (O, (I + 31) // 32), generator=g, dtype=torch.uint8,
+                              device="cuda")
+        W = rc.decode(w, s, fmt, I)
+        x = torch.randn(S, n, generator=g, device="cuda").to(BF16)
+        y = torch.empty(S, m, device="cuda")
+        call(fmt, x, w, s, y)
+        close(y, x, W.T if O == m else W, f"outputs {O}")
+        del W, x
