@@ -527,8 +527,10 @@ MVLLM_API int mvllm_moe_dense_ffn_dev(void *stream, int fmt, int T, int H, int O
  *      for all), an output's is at least its width.  tok_pos [T, KK], KK =
  *      K + n_shared <= 64, rows, rw, nr, xoff are mvllm_moe_permute_dev's.
  *      rw has rows_cap entries; positions outside [0, rows_cap) count as no
- *      slot; rows of an output that no position names (behind the last
- *      segment) are left as they were.  D, H, I, O <= 2^30.
+ *      slot, one that a token names twice counts twice, and of tokens that
+ *      name the same one dispatch and combine_grad keep one's row; rows of an
+ *      output that no position names (behind the last segment) are left as
+ *      they were.  D, H, I, O <= 2^30.
  *      Sums are f32 in a fixed order (results repeat to the bit) and round
  *      once.  Inputs and outputs may not overlap; calls that may run at the
  *      same time need a workspace each.  Stream-ordered, no host

@@ -173,13 +173,15 @@ struct WarpSlots {
             p1 = -1;
     }
     // Sorts the positions ascending over (lane, half) and returns their
-    // number: each value goes to the place its rank names.
+    // number: each value goes to the place its rank names.  Slots with the same
+    // position rank by slot, so that every place gets a value.
     __device__ __forceinline__ int sort(int KK, int *smem) {
+        const int lane = threadIdx.x & 31;
         int r0 = 0, r1 = 0;
         for (int u = 0; u < KK; ++u) {
             const int q = __shfl_sync(0xffffffffu, u < 32 ? p0 : p1, u & 31);
-            r0 += (q >= 0 && q < p0) ? 1 : 0;
-            r1 += (q >= 0 && q < p1) ? 1 : 0;
+            r0 += (q >= 0 && (u < lane ? q <= p0 : q < p0)) ? 1 : 0;
+            r1 += (q >= 0 && (u < lane + 32 ? q <= p1 : q < p1)) ? 1 : 0;
         }
         const int n = __popc(__ballot_sync(0xffffffffu, p0 >= 0)) +
                       __popc(__ballot_sync(0xffffffffu, p1 >= 0));
