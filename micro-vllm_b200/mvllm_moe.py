@@ -726,17 +726,25 @@ def _grid(t, name, dtype, shape):
     return _flat(t, name, dtype, 0)
 
 
+def _sizes(t, name):
+    """The two sizes of a matrix; the C entries take them as int."""
+    rows, cols = t.shape
+    if rows > 0x7fffffff or cols > 0x7fffffff:
+        raise ValueError(f"{name}: shape {(rows, cols)}, below 2^31 is needed")
+    return rows, cols
+
+
 def _slots(tok_pos):
     if tok_pos.dim() != 2:
         raise ValueError(f"tok_pos: shape {tuple(tok_pos.shape)}, [T, K + n_shared] is needed")
-    T, KK = tok_pos.shape
+    T, KK = _sizes(tok_pos, "tok_pos")
     return T, KK, _flat(tok_pos, "tok_pos", "torch.int32", T * KK)
 
 
 def _matrix(t, name):
     if t is None or t.dim() != 2:
         raise ValueError(f"{name}: a 2-D tensor is needed")
-    return t.shape
+    return _sizes(t, name)
 
 
 _raw_stream = None  # device index -> handle of torch's current stream
