@@ -721,8 +721,9 @@ def _flat(t, name, dtype, count):
 
 def _grid(t, name, dtype, shape):
     """Address of a contiguous device tensor of exactly this shape."""
-    if t.shape != shape:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, {shape} is needed")
+    if t is None or t.shape != shape:
+        raise ValueError(f"{name}: shape {None if t is None else tuple(t.shape)}, "
+                         f"{shape} is needed")
     return _flat(t, name, dtype, 0)
 
 
@@ -735,8 +736,8 @@ def _sizes(t, name):
 
 
 def _slots(tok_pos):
-    if tok_pos.dim() != 2:
-        raise ValueError(f"tok_pos: shape {tuple(tok_pos.shape)}, [T, K + n_shared] is needed")
+    if tok_pos is None or tok_pos.dim() != 2:
+        raise ValueError("tok_pos: a 2-D tensor [T, K + n_shared] is needed")
     T, KK = _sizes(tok_pos, "tok_pos")
     return T, KK, _flat(tok_pos, "tok_pos", "torch.int32", T * KK)
 
@@ -888,6 +889,8 @@ def matvec_q4_grad_dev(fmt, dy, w, scales, dx, stream=None):
 def _expert_matvec(entry, fmt, x, w, scales, nr, xoff, y, I, O, stream):
     if fmt not in (FMT_INT4_G64, FMT_MXFP4):
         raise ValueError(f"fmt {fmt}: FMT_INT4_G64 or FMT_MXFP4 is needed")
+    if nr is None or nr.numel() > 0x7fffffff:
+        raise ValueError("nr: the rows of each expert are needed")
     nb, cap = nr.numel(), x.shape[0]
     px, tx, ldx = _rows(x, "the input rows", cap, x.shape[1])
     py, ty, ldy = _rows(y, "the output rows", cap, y.shape[1], out=True)

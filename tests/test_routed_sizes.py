@@ -50,3 +50,18 @@ def test_sizes_past_32_bits_are_refused(lib):
                  lambda: lib.expert_matvec_q4_grad_dev(fmt, x, tab, tab, nr, nr, far_cols)):
         with pytest.raises(ValueError, match="2\\^31"):
             call()
+
+
+def test_missing_tensors_are_named(lib):
+    i32 = torch.int32
+    pos, x, rw, dwt = torch.zeros(4, 2, dtype=i32), torch.zeros(4, 8), torch.zeros(8), wide(4, 2)
+    nr, tab = torch.zeros(2, dtype=i32), torch.zeros(2, dtype=torch.int64)
+    router, scores, args = torch.zeros(2, 8), torch.zeros(4, 2), (nr, nr, nr)
+    for name, call in (
+            ("tok_pos", lambda: lib.dispatch_dev(x, None, x)),
+            ("dwt", lambda: lib.combine_grad_dev(x, x, rw, pos, pos, x, None)),
+            ("scores", lambda: lib.route_grad_dev(x, router, pos, None, dwt, *args, pos, x, None,
+                                                  workspace=x)),
+            ("nr", lambda: lib.expert_matvec_q4_dev(lib.FMT_INT4_G64, x, tab, tab, None, nr, x))):
+        with pytest.raises(ValueError, match=name):
+            call()
