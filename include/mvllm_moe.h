@@ -595,7 +595,8 @@ MVLLM_API int mvllm_matvec_q4_dev(void *stream, int fmt, const void *x, int x_dt
                                   int y_dtype, int64_t ldy);
 /* Its gradient for the rows, the weights being frozen: dx[r] = W^T dy[r],
  * dy [S, O], dx [S, I]; a pass serves 8 or 16 rows (2 or 5 where f32 rows meet
- * MXFP4).  The products dy * scale of int4 go in three bf16 parts, 24 bits. */
+ * MXFP4).  The products dy * scale of int4 go in three bf16 parts, 24 bits.
+ * An MXFP4 weight beyond f32's range (codes 253 and 254) counts as infinite. */
 MVLLM_API int mvllm_matvec_q4_grad_dev(void *stream, int fmt, const void *dy, int dy_dtype,
                                        int64_t lddy, const void *w, const void *scales, int S,
                                        int I, int O, void *dx, int dx_dtype, int64_t lddx);

@@ -715,7 +715,8 @@ __device__ __forceinline__ void mv_gradient_pairs(uint32_t st, int kb, int h, ui
 // the large sum left 6.8e-7 of the result over 16384 rows, where this leaves
 // 9e-8.  A product that is not finite comes out as NaN; the caller notices the
 // NaN in its sums and repeats the unit with CAREFUL, which keeps such a product
-// whole in its first part.
+// whole in its first part.  One of finite factors is three times bf16's largest
+// value there: infinite with any weight but 0, and 0 with that.
 template <bool CAREFUL>
 __device__ __forceinline__ void mv_gradient_int4(uint32_t st, uint32_t xs,
                                                  float (&acc)[4][4][2][4]) {
@@ -731,12 +732,15 @@ __device__ __forceinline__ void mv_gradient_int4(uint32_t st, uint32_t xs,
             float o[3][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float m = v[j] * __uint_as_float(lds32(st + kMvRows * 128 + 4 * h +
-                                                             (kb * 16 + t + 4 * j) * 16));
+                const float s = __uint_as_float(
+                    lds32(st + kMvRows * 128 + 4 * h + (kb * 16 + t + 4 * j) * 16));
+                const float m = v[j] * s;
                 if constexpr (CAREFUL) {
+                    const bool over = fabsf(v[j]) <= 3.402823466e38f &&
+                                      fabsf(s) <= 3.402823466e38f && fabsf(m) > 3.402823466e38f;
 #pragma unroll
-                    for (int k = 0; k < 3; ++k)
-                        o[k][j] = mv_term<3>(m, k);
+                    for (int k = 0; k < 3; ++k) // bf16's largest value
+                        o[k][j] = over ? copysignf(0x1.fep127f, m) : mv_term<3>(m, k);
                 } else { // the packing takes the upper halves
                     o[0][j] = m;
                     o[1][j] = m - trunc_bf16(m);

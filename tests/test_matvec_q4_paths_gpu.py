@@ -162,3 +162,23 @@ def test_reductions_past_the_address_arithmetic(moe, fmt):
         call(fmt, x, w, s, y)
         close(y, x, W.T if O == m else W, f"outputs {O}")
         del W, x
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradient_products_beyond_f32_meet_zero_weights(moe, dtype):
+    """Finite rows and int4 scales whose product passes f32's range: infinite in
+    the columns that have weights, 0 where all weights are 0."""
+    S, I, O = 3, 320, 64
+    code = torch.arange(I) % 16
+    w = (code[0::2] | (code[1::2] << 4)).to(torch.uint8).expand(O, -1).contiguous().cuda()
+    s = torch.full((O, I // 64), 2.0 ** 100, device="cuda")
+    dy = torch.ones(S, O) * 2.0 ** -110
+    dy[1] = 2.0 ** 60
+    dy[2, 1:] = 0  # one product alone
+    dy[2, 0] = -(2.0 ** 28)
+    dx = torch.empty(S, I, device="cuda")
+    moe.matvec_q4_grad_dev(INT4, dy.cuda().to(dtype), w, s, dx)
+    sign = (code - 8).sign().float().cuda()
+    inf = torch.where(sign == 0, torch.zeros_like(sign), sign * float("inf"))
+    assert torch.equal(dx[1], inf) and torch.equal(dx[2], -inf)
+    assert torch.equal(dx[0], (code - 8).cuda() * (O * 2.0 ** -10))
