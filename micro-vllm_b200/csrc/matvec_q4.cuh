@@ -706,37 +706,44 @@ __device__ __forceinline__ void mv_gradient_pairs(uint32_t st, int kb, int h, ui
     p[2] = mv_prmt(r[2], r[3], 0x5410u), p[3] = mv_prmt(r[2], r[3], 0x7632u);
 }
 
+// A stage's sums start from zero and are added to the task's in f32: the matrix
+// unit cuts off what lies below a sum's last bit, each time towards zero, which
+// over 16384 rows of far magnitudes left 1.2e-6 of the result where this leaves
+// 1.4e-7.
+
 // int4's f32 scale multiplies the row's value, and the product's three parts
 // (its upper 16 bits, those of what is left, the rest: 24 bits in all) are a
-// matrix instruction each.  (Two parts, 16 to 17 bits, show in a bf16 result:
-// ten times as many values one step off, 309 in place of 392 us on 512 rows of
-// 160 experts of 1536 x 6144.)  The first parts have sums of their own: the
-// matrix unit cuts what lies below a sum's last bit, and small parts added to
-// the large sum left 6.8e-7 of the result over 16384 rows, where this leaves
-// 9e-8.  A product that is not finite comes out as NaN; the caller notices the
-// NaN in its sums and repeats the unit with CAREFUL, which keeps such a product
-// whole in its first part.  One of finite factors is three times bf16's largest
-// value there: infinite with any weight but 0, and 0 with that.
+// matrix instruction each, smallest first.  (Two parts, 16 to 17 bits, show in a
+// bf16 result: ten times as many values one step off, 309 in place of 392 us on
+// 512 rows of 160 experts of 1536 x 6144.)  A product that is not finite comes
+// out as NaN; the caller notices the NaN in its sums and repeats the unit with
+// CAREFUL, which keeps such a product whole in its first part.  One of finite
+// factors is three times bf16's largest value there: infinite with any weight
+// but 0, and 0 with that.
 template <bool CAREFUL>
 __device__ __forceinline__ void mv_gradient_int4(uint32_t st, uint32_t xs,
-                                                 float (&acc)[4][4][2][4]) {
+                                                 float (&acc)[4][4][1][4]) {
     const int t = threadIdx.x & 3;
+    float v[2][4]; // the rows' values
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-        const uint4 x = lds128(xs + kb * 64); // the rows' values
-        const float v[4] = {__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z),
-                            __uint_as_float(x.w)};
+        const uint4 x = lds128(xs + kb * 64);
+        v[kb][0] = __uint_as_float(x.x), v[kb][1] = __uint_as_float(x.y);
+        v[kb][2] = __uint_as_float(x.z), v[kb][3] = __uint_as_float(x.w);
+    }
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            uint32_t p[4], b[3][2];
+    for (int h = 0; h < 4; ++h) {
+        uint32_t a[4][2][4], b[2][3][2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
             float o[3][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float s = __uint_as_float(
                     lds32(st + kMvRows * 128 + 4 * h + (kb * 16 + t + 4 * j) * 16));
-                const float m = v[j] * s;
+                const float m = v[kb][j] * s;
                 if constexpr (CAREFUL) {
-                    const bool over = fabsf(v[j]) <= 3.402823466e38f &&
+                    const bool over = fabsf(v[kb][j]) <= 3.402823466e38f &&
                                       fabsf(s) <= 3.402823466e38f && fabsf(m) > 3.402823466e38f;
 #pragma unroll
                     for (int k = 0; k < 3; ++k) // bf16's largest value
@@ -749,23 +756,34 @@ __device__ __forceinline__ void mv_gradient_int4(uint32_t st, uint32_t xs,
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                b[0][j] = mv_prmt(__float_as_uint(o[0][2 * j]), __float_as_uint(o[0][2 * j + 1]),
-                                  0x7632u);
-                b[1][j] = mv_prmt(__float_as_uint(o[1][2 * j]), __float_as_uint(o[1][2 * j + 1]),
-                                  0x7632u);
-                b[2][j] = pack_bf16(o[2][2 * j], o[2][2 * j + 1]);
+                b[kb][0][j] = mv_prmt(__float_as_uint(o[0][2 * j]),
+                                      __float_as_uint(o[0][2 * j + 1]), 0x7632u);
+                b[kb][1][j] = mv_prmt(__float_as_uint(o[1][2 * j]),
+                                      __float_as_uint(o[1][2 * j + 1]), 0x7632u);
+                b[kb][2][j] = pack_bf16(o[2][2 * j], o[2][2 * j + 1]);
             }
+            uint32_t p[4];
             mv_gradient_pairs(st, kb, h, p);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                uint32_t a[4];
+            for (int q = 0; q < 4; ++q)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) // (128 + code) - 136
-                    a[j] = sub_bf16x2(((p[j] >> (4 * q)) & 0x000f000fu) | 0x43004300u, 0x43084308u);
-                mma_bf16_16816(acc[h][q][1], a[0], a[1], a[2], a[3], b[2][0], b[2][1]);
-                mma_bf16_16816(acc[h][q][0], a[0], a[1], a[2], a[3], b[0][0], b[0][1]);
-                mma_bf16_16816(acc[h][q][1], a[0], a[1], a[2], a[3], b[1][0], b[1][1]);
-            }
+                    a[q][kb][j] = sub_bf16x2(((p[j] >> (4 * q)) & 0x000f000fu) | 0x43004300u,
+                                             0x43084308u);
+        }
+        float d[4][4] = {};
+#pragma unroll
+        for (int k = 2; k >= 0; --k)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    mma_bf16_16816(d[q], a[q][kb][0], a[q][kb][1], a[q][kb][2], a[q][kb][3],
+                                   b[kb][k][0], b[kb][k][1]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            ffma2(acc[h][q][0][0], acc[h][q][0][1], d[q][0], d[q][1], 1.f);
+            ffma2(acc[h][q][0][2], acc[h][q][0][3], d[q][2], d[q][3], 1.f);
         }
     }
 }
@@ -777,60 +795,66 @@ template <int NT, bool CAREFUL>
 __device__ __forceinline__ void mv_gradient_mxfp4(uint32_t st, int half, const uint32_t (&xs)[NT],
                                                   float (&acc)[4][4][NT][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    uint32_t b[2][NT][2]; // the same for every column
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-        uint32_t sw[4][2];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint2 v = lds64(st + kMvRows * 128 + (kb * 16 + t + 4 * j) * 16 + half);
-            sw[j][0] = v.x, sw[j][1] = v.y;
-        }
-        uint32_t b[NT][2]; // the same for every column
+    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const uint2 v = lds64(xs[nt] + kb * 32);
-            b[nt][0] = v.x, b[nt][1] = v.y;
+            b[kb][nt][0] = v.x, b[kb][nt][1] = v.y;
         }
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            uint32_t p[4], m[2], m2[2] = {};
-            mv_gradient_pairs(st, kb, h, p);
-            // 2^(code - 1) = 2^126 * scale as bf16, the weight's bits being
-            // 2^-126 of its value: the code's exponent field plus 126.
-            // Codes above 128 take 2^126 and then the scale, 0 is 0.
-            const uint32_t sel = ((h & 1) * 2 + (g >> 2)) * 0x11u;
+    for (int h = 0; h < 4; ++h) {
+        uint32_t p[2][4], m[2][2], m2[2][2] = {};
+        // 2^(code - 1) = 2^126 * scale as bf16, the weight's bits being 2^-126 of
+        // its value: the code's exponent field plus 126.  Codes above 128 take
+        // 2^126 and then the scale, 0 is 0.
+        const uint32_t sel = ((h & 1) * 2 + (g >> 2)) * 0x11u;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            mv_gradient_pairs(st, kb, h, p[kb]);
+            const uint32_t codes = st + kMvRows * 128 + (kb * 16 + t) * 16 + half + 4 * (h >> 1);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 // byte k of the two rows' codes in the two halfwords
-                const uint32_t c = mv_prmt(sw[2 * j][h >> 1], sw[2 * j + 1][h >> 1],
+                const uint32_t c = mv_prmt(lds32(codes + 128 * j), lds32(codes + 128 * j + 64),
                                            sel | ((sel | 0x44u) << 8)) &
                                    0x00ff00ffu;
                 if constexpr (CAREFUL) {
                     const uint32_t lo = c & 255u, hi = c >> 16;
-                    m[j] = (lo ? 253u << 7 : 0u) | (hi ? 253u << 23 : 0u);
-                    m2[j] = (lo << 7) | (hi << 23);
+                    m[kb][j] = (lo ? 253u << 7 : 0u) | (hi ? 253u << 23 : 0u);
+                    m2[kb][j] = (lo << 7) | (hi << 23);
                 } else {
-                    m[j] = c * 128u + ((126u << 7) | (126u << 23));
+                    m[kb][j] = c * 128u + ((126u << 7) | (126u << 23));
                 }
             }
+        }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 4; ++q) {
+            float d[NT][4] = {};
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
                 uint32_t a[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t mag = q == 0   ? p[j] << 6
-                                         : q == 1 ? p[j] << 2
-                                         : q == 2 ? p[j] >> 2
-                                                  : p[j] >> 6;
-                    const uint32_t v = (mag & 0x01c001c0u) |
-                                       ((p[j] << (12 - 4 * q)) & 0x80008000u);
-                    a[j] = mul_bf16x2(v, m[j >> 1]);
+                    const uint32_t w = p[kb][j];
+                    const uint32_t mag = q == 0   ? w << 6
+                                         : q == 1 ? w << 2
+                                         : q == 2 ? w >> 2
+                                                  : w >> 6;
+                    const uint32_t v = (mag & 0x01c001c0u) | ((w << (12 - 4 * q)) & 0x80008000u);
+                    a[j] = mul_bf16x2(v, m[kb][j >> 1]);
                     if constexpr (CAREFUL)
-                        a[j] = mul_bf16x2(a[j], m2[j >> 1]);
+                        a[j] = mul_bf16x2(a[j], m2[kb][j >> 1]);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
-                    mma_bf16_16816(acc[h][q][nt], a[0], a[1], a[2], a[3], b[nt][0], b[nt][1]);
+                    mma_bf16_16816(d[nt], a[0], a[1], a[2], a[3], b[kb][nt][0], b[kb][nt][1]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                ffma2(acc[h][q][nt][0], acc[h][q][nt][1], d[nt][0], d[nt][1], 1.f);
+                ffma2(acc[h][q][nt][2], acc[h][q][nt][3], d[nt][2], d[nt][3], 1.f);
             }
         }
     }
@@ -911,9 +935,9 @@ __device__ __forceinline__ void mv_put(float *to, const float (&acc)[2][NT][4], 
             }
         }
 }
-// The gradient's: [part of a row][output], int4's two sums of a row as one.
-template <int RPITCH, int NT, int SUMS>
-__device__ __forceinline__ void mv_put_gradient(float *to, const float (&acc)[4][4][SUMS][4]) {
+// The gradient's: [part of a row][output].
+template <int RPITCH, int NT>
+__device__ __forceinline__ void mv_put_gradient(float *to, const float (&acc)[4][4][NT][4]) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
 #pragma unroll
     for (int h = 0; h < 4; ++h)
@@ -921,10 +945,7 @@ __device__ __forceinline__ void mv_put_gradient(float *to, const float (&acc)[4]
         for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float d[4];
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-                    d[s] = SUMS > NT ? acc[h][q][0][s] + acc[h][q][1][s] : acc[h][q][nt][s];
+                const float(&d)[4] = acc[h][q][nt];
                 float *at = to + (nt * 8 + 2 * t) * RPITCH + h * 64 + 8 * g + q;
                 at[0] = d[0], at[RPITCH] = d[1];
                 at[4] = d[2], at[RPITCH + 4] = d[3];
@@ -1132,15 +1153,14 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
         }
         // The gradient's one task per warp keeps its sums to the end of the
         // unit; the forward's tasks leave theirs in shared memory one by one.
-        constexpr int SUMS = GRAD && FMT == MVLLM_FMT_INT4_G64 ? 2 : NT; // int4: of first parts, of others
-        float accg[GRAD ? 4 : 1][GRAD ? 4 : 1][SUMS][4];
+        float accg[GRAD ? 4 : 1][GRAD ? 4 : 1][NT][4];
         MvUnit next{};
         float check = 0.f; // NaN where a sum before its factor is not finite
         for (bool careful = false;; careful = true) {
             bool refilled = false;
             if constexpr (GRAD) {
 #pragma unroll
-                for (int i = 0; i < 16 * SUMS * 4; ++i)
+                for (int i = 0; i < 16 * NT * 4; ++i)
                     (&accg[0][0][0][0])[i] = 0.f;
             }
             for (int c0 = 0; c0 < nk; c0 += pl.chunk) {
@@ -1250,7 +1270,7 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
                 break;
             float nan = 0.f; // NaN where a sum is, or where infinities meet
 #pragma unroll
-            for (int i = 0; i < (GRAD ? 16 * SUMS * 4 : 0); ++i)
+            for (int i = 0; i < (GRAD ? 16 * NT * 4 : 0); ++i)
                 nan += (&accg[0][0][0][0])[i];
             if (!__syncthreads_or(nan != nan))
                 break;
@@ -1262,7 +1282,7 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
             mv_wait<0>();
             __syncthreads(); // the ring is done with before the sums overlay it
             if (warp < tasks)
-                mv_put_gradient<RPITCH, NT>(red + warp * RSIZE, accg);
+                mv_put_gradient<RPITCH>(red + warp * RSIZE, accg);
             __syncthreads();
         } else if (u + 1 < u1) {
             fetch(next);

@@ -182,3 +182,28 @@ def test_gradient_products_beyond_f32_meet_zero_weights(moe, dtype):
     inf = torch.where(sign == 0, torch.zeros_like(sign), sign * float("inf"))
     assert torch.equal(dx[1], inf) and torch.equal(dx[2], -inf)
     assert torch.equal(dx[0], (code - 8).cuda() * (O * 2.0 ** -10))
+
+
+def exact_as_f32(got, x, M, what):
+    """No further off in norm, row by row, than an f32 product of the decoded
+    weights (1.5 times) or one rounding of the result."""
+    want, plain = x.double() @ M, x.float() @ M.float()
+    off, most = (got.double() - want).norm(dim=1), 1.5 * (plain.double() - want).norm(dim=1)
+    assert (off <= most + 2.0 ** -24 * want.norm(dim=1)).all(), what
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+@pytest.mark.parametrize("S,n,m", [(8, 7168, 512), (40, 16384, 512), (3, 65536, 256)])
+def test_sums_of_far_magnitudes(moe, S, n, m, fmt, dtype):
+    """Rows and scales over 24 binades: no bits of a sum are cut off on the way."""
+    gen = torch.Generator().manual_seed(n)
+    x = torch.randn(S, n, generator=gen) * torch.exp2(
+        torch.randint(-6, 7, (S, n), generator=gen).float())
+    x = x.cuda().to(dtype)
+    for O, I, call in ((m, n, moe.matvec_q4_dev), (n, m, moe.matvec_q4_grad_dev)):
+        w, s = rc.packed(gen, fmt, O, I, "cuda", spread=6)
+        W = rc.decode(w, s, fmt, I)
+        y = torch.empty(S, m, device="cuda")
+        call(fmt, x, w, s, y)
+        exact_as_f32(y, x, W.T if O == m else W, f"outputs {O}")
