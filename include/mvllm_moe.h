@@ -615,6 +615,14 @@ MVLLM_API int mvllm_moe_matvec_q4_grad_dev(void *stream, int fmt, int nb, const 
                                            const void *const *scales, int I, int O, void *dx,
                                            int dx_dtype, int64_t lddx);
 
+/* How these products cut a call of `rows` rows of nb matrices: plan[0] rows of
+ * a pass over a matrix, [1] CTAs of a cluster, [2] outputs of a unit, [3] parts
+ * of the reduction a CTA's warps take, [4] the CTA's stages of it (256 columns;
+ * gradient: 32 rows), [5] stages whose rows are held at a time, [6] whether the
+ * rows are surveyed for one scale each, [7] CTAs.  No launch. */
+MVLLM_API int mvllm_matvec_q4_plan(int fmt, int grad, int x_dtype, int nb, int rows, int I, int O,
+                                   int *plan);
+
 /* Health check of the bounded device waits that every pipeline kernel uses:
  * runs one small kernel that waits on an mbarrier one thread completes and
  * then on one that nothing completes.  *completed = 1 when the first wait

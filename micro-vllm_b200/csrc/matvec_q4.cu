@@ -173,7 +173,8 @@ template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
         return MVLLM_OK;
     }
 
-    // The rule's answer by sizes; asking it takes longer than a small product.
+    // The rule's answer by sizes: asking it takes the host 5 to 60 us, as long as
+    // a small product; a new number of rows is a new size.
     static int cut_for(const MatvecPlan &p, int nb, const DeviceScope &dev, MvCut &cut) {
         static std::mutex mu;
         static std::map<std::array<int, 5>, MvCut> seen;
@@ -202,10 +203,16 @@ template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
         return reinterpret_cast<const void *>(matvec_q4_kernel<FMT, TX, NT, GRAD>);
     }
 
+    // Launches a cut, or describes it in `told` (mvllm_matvec_q4_plan).
     static int launch(cudaStream_t st, const MatvecArgs &a, MvCut cut, const void *x, int64_t ldx,
-                      void *y, int64_t ldy) {
+                      void *y, int64_t ldy, int *told) {
         MatvecPlan &p = cut.p;
         const int ranks = cut.ranks;
+        if (told) {
+            const int is[8] = {RP, ranks, p.range, p.wk, p.slice, p.chunk, p.try_common, cut.grid};
+            std::copy(is, is + 8, told);
+            return MVLLM_OK;
+        }
         const int64_t smem = layout(p, p.chunk, ranks, a.nb);
         if (p.range < 1 || smem > kMvSmem)
             return host_fail(MVLLM_ERR_UNSUPPORTED, "matvec_q4: %lld bytes of shared memory",
@@ -236,7 +243,7 @@ template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
 // 160 experts of 20, 6144 -> 1536, 614 and 462.
 template <int FMT, typename TX, bool GRAD>
 int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, const DeviceScope &dev,
-                const void *x, int64_t ldx, void *y, int64_t ldy) {
+                const void *x, int64_t ldx, void *y, int64_t ldy, int *told) {
     constexpr int T = MvTerms<FMT, TX, GRAD>::T;
     constexpr bool NARROW = GRAD && FMT == MVLLM_FMT_INT4_G64;
     using One = MvHost<FMT, TX, 1, GRAD>;
@@ -254,27 +261,41 @@ int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, const
         if (int rc = Four::cut_for(p, a.nb, dev, four))
             return rc;
     if (one.ns <= two.ns && one.ns <= four.ns)
-        return One::launch(st, a, one, x, ldx, y, ldy);
+        return One::launch(st, a, one, x, ldx, y, ldy, told);
     if (two.ns <= four.ns)
-        return Two::launch(st, a, two, x, ldx, y, ldy);
-    return Four::launch(st, a, four, x, ldx, y, ldy);
+        return Two::launch(st, a, two, x, ldx, y, ldy, told);
+    return Four::launch(st, a, four, x, ldx, y, ldy, told);
 }
 
 template <int FMT, typename TX>
 int matvec_way(cudaStream_t st, bool grad, const MatvecArgs &a, const MatvecPlan &p,
-               const DeviceScope &dev, const void *x, int64_t ldx, void *y, int64_t ldy) {
+               const DeviceScope &dev, const void *x, int64_t ldx, void *y, int64_t ldy,
+               int *told) {
     if (!grad)
-        return matvec_rows<FMT, TX, false>(st, a, p, dev, x, ldx, y, ldy);
-    return matvec_rows<FMT, TX, true>(st, a, p, dev, x, ldx, y, ldy);
+        return matvec_rows<FMT, TX, false>(st, a, p, dev, x, ldx, y, ldy, told);
+    return matvec_rows<FMT, TX, true>(st, a, p, dev, x, ldx, y, ldy, told);
+}
+
+int matvec_type(cudaStream_t st, bool grad, const MatvecArgs &a, const MatvecPlan &p,
+                const DeviceScope &dev, const void *x, bool fx, int64_t ldx, void *y, int64_t ldy,
+                int *told) {
+    if (a.fmt == MVLLM_FMT_INT4_G64)
+        return fx ? matvec_way<MVLLM_FMT_INT4_G64, float>(st, grad, a, p, dev, x, ldx, y, ldy, told)
+                  : matvec_way<MVLLM_FMT_INT4_G64, bf>(st, grad, a, p, dev, x, ldx, y, ldy, told);
+    return fx ? matvec_way<MVLLM_FMT_MXFP4, float>(st, grad, a, p, dev, x, ldx, y, ldy, told)
+              : matvec_way<MVLLM_FMT_MXFP4, bf>(st, grad, a, p, dev, x, ldx, y, ldy, told);
+}
+
+bool matvec_sizes(const MatvecArgs &a, int x_dtype) {
+    return (a.fmt == MVLLM_FMT_INT4_G64 || a.fmt == MVLLM_FMT_MXFP4) && a.I >= 1 && a.O >= 1 &&
+           a.I <= kMvMaxSide && a.O <= kMvMaxSide && a.rows >= 0 && a.rows <= kMvMaxSide &&
+           (x_dtype == MVLLM_DTYPE_F32 || x_dtype == MVLLM_DTYPE_BF16);
 }
 
 int matvec_any(const char *who, void *stream, bool grad, const MatvecArgs &a, const void *x,
                int x_dtype, int64_t ldx, void *y, int y_dtype, int64_t ldy) {
     const int out = grad ? a.I : a.O;
-    if ((a.fmt != MVLLM_FMT_INT4_G64 && a.fmt != MVLLM_FMT_MXFP4) ||
-        (a.rows > 0 && (!x || !y)) || a.I < 1 || a.O < 1 || a.I > kMvMaxSide ||
-        a.O > kMvMaxSide || a.rows < 0 || a.rows > kMvMaxSide || ldx < 0 || ldy < out ||
-        (x_dtype != MVLLM_DTYPE_F32 && x_dtype != MVLLM_DTYPE_BF16) ||
+    if (!matvec_sizes(a, x_dtype) || (a.rows > 0 && (!x || !y)) || ldx < 0 || ldy < out ||
         (y_dtype != MVLLM_DTYPE_F32 && y_dtype != MVLLM_DTYPE_BF16))
         return host_fail(MVLLM_ERR_INVALID, "%s: invalid arguments", who);
     DeviceScope dev;
@@ -290,15 +311,11 @@ int matvec_any(const char *who, void *stream, bool grad, const MatvecArgs &a, co
     const uint64_t ey = p.y_f32 ? 4 : 2;
     p.y_vec = ((reinterpret_cast<uintptr_t>(y) | (a.rows > 1 ? uint64_t(ldy) * ey : 0)) &
                (4 * ey - 1)) == 0;
-    const bool fx = x_dtype == MVLLM_DTYPE_F32, i4 = a.fmt == MVLLM_FMT_INT4_G64;
+    const bool fx = x_dtype == MVLLM_DTYPE_F32;
     const uint64_t pitch = a.rows > 1 ? uint64_t(ldx) * (fx ? 4 : 2) : 0;
     p.x_vec = ((reinterpret_cast<uintptr_t>(x) | pitch) & 15u) == 0;
     try { // the plans' tables allocate
-        if (i4)
-            return fx ? matvec_way<MVLLM_FMT_INT4_G64, float>(st, grad, a, p, dev, x, ldx, y, ldy)
-                      : matvec_way<MVLLM_FMT_INT4_G64, bf>(st, grad, a, p, dev, x, ldx, y, ldy);
-        return fx ? matvec_way<MVLLM_FMT_MXFP4, float>(st, grad, a, p, dev, x, ldx, y, ldy)
-                  : matvec_way<MVLLM_FMT_MXFP4, bf>(st, grad, a, p, dev, x, ldx, y, ldy);
+        return matvec_type(st, grad, a, p, dev, x, fx, ldx, y, ldy, nullptr);
     } catch (...) {
         return host_fail(MVLLM_ERR_NOMEM, "%s: out of host memory", who);
     }
@@ -318,7 +335,7 @@ int matvec_experts(const char *who, void *stream, bool grad, int fmt, int nb, co
                    int x_dtype, int64_t ldx, int rows_cap, const int *nr, const int *xoff,
                    const void *const *wt, const void *const *st, int I, int O, void *y,
                    int y_dtype, int64_t ldy) {
-    if (!wt || !st || !nr || !xoff || nb < 1 || nb > 1024)
+    if (!wt || !st || !nr || !xoff || nb < 1 || nb > kMvMaxExperts)
         return host_fail(MVLLM_ERR_INVALID, "%s: invalid arguments", who);
     MatvecArgs a{};
     a.fmt = fmt, a.I = I, a.O = O, a.wt = wt, a.st = st, a.nr = nr, a.xoff = xoff;
@@ -329,6 +346,25 @@ int matvec_experts(const char *who, void *stream, bool grad, int fmt, int nb, co
 } // namespace
 
 extern "C" {
+
+int mvllm_matvec_q4_plan(int fmt, int grad, int x_dtype, int nb, int rows, int I, int O,
+                         int *plan) {
+    MatvecArgs a{};
+    a.fmt = fmt, a.I = I, a.O = O, a.rows = rows, a.nb = nb;
+    if (!matvec_sizes(a, x_dtype) || rows < 1 || nb < 1 || nb > kMvMaxExperts || !plan)
+        return host_fail(MVLLM_ERR_INVALID, "matvec_q4_plan: invalid arguments");
+    DeviceScope dev;
+    if (int rc = dev.enter())
+        return rc;
+    MatvecPlan p{};
+    p.N = grad ? I : O, p.K = grad ? O : I, p.rows_most = rows;
+    try {
+        return matvec_type(nullptr, grad != 0, a, p, dev, nullptr, x_dtype == MVLLM_DTYPE_F32, 0,
+                           nullptr, 0, plan);
+    } catch (...) {
+        return host_fail(MVLLM_ERR_NOMEM, "matvec_q4_plan: out of host memory");
+    }
+}
 
 int mvllm_matvec_q4_dev(void *stream, int fmt, const void *x, int x_dtype, int64_t ldx,
                         const void *w, const void *scales, int S, int I, int O, void *y,

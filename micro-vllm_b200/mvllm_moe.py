@@ -56,7 +56,7 @@ C_SYMBOLS = (
     "mvllm_moe_layer_partial_peer_dev", "mvllm_moe_dispatch_dev", "mvllm_moe_dispatch_grad_dev",
     "mvllm_moe_combine_dev", "mvllm_moe_combine_grad_dev", "mvllm_moe_route_grad_workspace",
     "mvllm_moe_route_grad_dev", "mvllm_matvec_q4_dev", "mvllm_matvec_q4_grad_dev",
-    "mvllm_moe_matvec_q4_dev", "mvllm_moe_matvec_q4_grad_dev",
+    "mvllm_moe_matvec_q4_dev", "mvllm_moe_matvec_q4_grad_dev", "mvllm_matvec_q4_plan",
 )
 PHASES = ("permute", "gather", "plan", "expert_phase1", "expert_phase2", "combine")
 
@@ -160,6 +160,7 @@ def lib():
                                             ld]),
             "mvllm_moe_matvec_q4_grad_dev": (i, [vp, i, i, vp, i, ld, i, vp, vp, vp, vp, i, i, vp,
                                                  i, ld]),
+            "mvllm_matvec_q4_plan": (i, [i] * 7 + [vp]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)
@@ -914,3 +915,14 @@ def expert_matvec_q4_grad_dev(fmt, dy, w, scales, nr, xoff, dx, stream=None):
     expert_matvec_q4_dev's rows."""
     _expert_matvec(lib().mvllm_moe_matvec_q4_grad_dev, fmt, dy, w, scales, nr, xoff, dx,
                    _matrix(dx, "dx")[1], _matrix(dy, "dy")[1], stream)
+
+
+Q4_PLAN = ("rows", "cluster", "outputs", "parts", "stages", "held", "surveyed", "ctas")
+
+
+def matvec_q4_plan(fmt, dtype, rows, I, O, nb=1, grad=False) -> dict:
+    """How the products above cut a call of these sizes, x_dtype `dtype`
+    (DTYPE_F32 or DTYPE_BF16), nb matrices."""
+    plan = (C.c_int * len(Q4_PLAN))()
+    _check(lib().mvllm_matvec_q4_plan(fmt, int(bool(grad)), dtype, nb, rows, I, O, plan))
+    return dict(zip(Q4_PLAN, plan))

@@ -207,3 +207,104 @@ def test_sums_of_far_magnitudes(moe, S, n, m, fmt, dtype):
         y = torch.empty(S, m, device="cuda")
         call(fmt, x, w, s, y)
         exact_as_f32(y, x, W.T if O == m else W, f"outputs {O}")
+
+
+def product(moe, fmt, x, y, w, s, grad):
+    (moe.matvec_q4_grad_dev if grad else moe.matvec_q4_dev)(fmt, x, w, s, y)
+
+
+def plan_of(moe, fmt, dtype, S, I, O, nb=1, grad=False):
+    return moe.matvec_q4_plan(fmt, moe.DTYPE_F32 if dtype == F32 else moe.DTYPE_BF16, S, I, O, nb,
+                              grad)
+
+
+# Type, rows, sizes, and the rows of a pass of a plan that surveys the rows.
+SURVEYED = [(BF16, 1, 7168, 16384, 8), (BF16, 12, 7168, 16384, 16), (BF16, 32, 1024, 65536, 32),
+            (F32, 4, 7168, 16384, 4), (F32, 8, 7168, 16384, 8), (F32, 12, 7168, 16384, 16),
+            (F32, 32, 1024, 65536, 16)]
+
+
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+@pytest.mark.parametrize("dtype,S,I,O,rows", SURVEYED)
+def test_surveyed_rows(moe, dtype, S, I, O, rows, fmt):
+    """A plan that gives a row one scale where the row's range allows it: rows
+    that fit, one that does not, rows of zeros, and rows that are not finite."""
+    plan = plan_of(moe, fmt, dtype, S, I, O)
+    assert plan["surveyed"] and plan["rows"] == rows and plan["held"] == plan["stages"]
+    gen = torch.Generator().manual_seed(S + I)
+    w, s = rc.packed(gen, fmt, O, I, "cuda", spread=1)
+    M = rc.decode(w, s, fmt, I).T
+    x = torch.randn(S, I, generator=gen).cuda()
+    y = torch.empty(S, O, device="cuda")
+    for kind in ("fits", "zeros", "does not", "not finite"):
+        z = x.clone()
+        if kind != "fits":
+            z[:, 64:192] = 0  # whole groups
+            z[S // 2] = z[S // 2] if S == 1 else 0
+        if kind == "does not":
+            z[S - 1, 256:320] *= 2.0 ** -14
+        z = z.to(dtype)
+        if kind == "not finite":
+            z[S - 1, 300] = float("inf")
+            z[0, 301] = float("nan")
+        moe.matvec_q4_dev(fmt, z, w, s, y)
+        if kind != "not finite":
+            exact_as_f32(y, z, M, kind)
+        else:
+            assert torch.isnan(y[0]).all()
+            want = z.double() @ M
+            if S > 1:
+                exact_as_f32(y[1:-1], z[1:-1], M, kind)
+                assert torch.equal(torch.isnan(y[-1]), torch.isnan(want[-1]))
+                live = ~torch.isnan(want[-1])
+                assert torch.equal(y[-1][live].double(), want[-1][live])
+
+
+# Type, rows, sizes and direction whose plan stages the rows in chunks.
+CHUNKED = [(BF16, 32, 16384, 4096, False), (BF16, 64, 16384, 4096, False),
+           (F32, 16, 7168, 16384, False), (F32, 64, 16384, 4096, False),
+           (BF16, 32, 1536, 32768, True), (F32, 32, 512, 65536, True),
+           (BF16, 12, 4096, 16384, True)]
+
+
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+@pytest.mark.parametrize("dtype,S,I,O,grad", CHUNKED)
+def test_rows_in_chunks(moe, dtype, S, I, O, grad, fmt):
+    if fmt == INT4 or not grad:
+        plan = plan_of(moe, fmt, dtype, S, I, O, grad=grad)
+        assert plan["held"] < plan["stages"]
+    gen = torch.Generator().manual_seed(S + I)
+    w, s = rc.packed(gen, fmt, O, I, "cuda", spread=1)
+    W = rc.decode(w, s, fmt, I)
+    n, m, M = (O, I, W) if grad else (I, O, W.T)
+    x = torch.randn(S, n, generator=gen)
+    x[:, ::7] *= 2.0 ** 9
+    x[1] = 0
+    x = x.cuda().to(dtype)
+    y = torch.empty(S, m, device="cuda")
+    product(moe, fmt, x, y, w, s, grad)
+    exact_as_f32(y, x, M, "chunks")
+
+
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+@pytest.mark.parametrize("dtype,S", [(BF16, 64), (BF16, 200), (F32, 64), (F32, 200)])
+def test_many_experts_rows(moe, dtype, S, fmt):
+    """Uneven segments of 16 experts, forward and gradient."""
+    E, I, O = 16, 7168, 2048
+    gen = torch.Generator().manual_seed(S)
+    w, s = rc.packed(gen, fmt, E * O, I, "cuda", spread=1)
+    tab, sct = (torch.tensor([t[e * O].data_ptr() for e in range(E)], device="cuda")
+                for t in (w, s))
+    nr = torch.bincount(torch.randint(0, E, (S,), generator=gen), minlength=E)
+    nr[3], nr[5] = nr[3] + nr[5], 0
+    xoff = (torch.cumsum(nr, 0) - nr).tolist()
+    n32, o32 = nr.int().cuda(), torch.tensor(xoff, dtype=torch.int32, device="cuda")
+    for n, m, call in ((I, O, moe.expert_matvec_q4_dev), (O, I, moe.expert_matvec_q4_grad_dev)):
+        x = torch.randn(S, n, generator=gen).cuda().to(dtype)
+        y = torch.full((S, m), 7.0, device="cuda")
+        call(fmt, x, tab, sct, n32, o32, y)
+        for e in range(E):
+            part = slice(xoff[e], xoff[e] + int(nr[e]))
+            W = rc.decode(w[e * O:(e + 1) * O], s[e * O:(e + 1) * O], fmt, I)
+            if int(nr[e]):
+                exact_as_f32(y[part], x[part], W.T if m == O else W, f"expert {e}")

@@ -1,4 +1,6 @@
 """Sizes that the Python entries of the routed steps refuse, without a GPU."""
+import ctypes
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -65,3 +67,16 @@ def test_missing_tensors_are_named(lib):
             ("nr", lambda: lib.expert_matvec_q4_dev(lib.FMT_INT4_G64, x, tab, tab, None, nr, x))):
         with pytest.raises(ValueError, match=name):
             call()
+
+
+def test_plans_refuse_what_the_products_refuse(lib):
+    plan = (ctypes.c_int * 8)()
+    good = [lib.FMT_INT4_G64, 0, lib.DTYPE_F32, 1, 2, 64, 64, plan]
+    entry = lib.lib().mvllm_matvec_q4_plan
+    if not lib.available():
+        assert entry(*good) == lib.ERR_NOT_INIT
+    for at, bad in ((0, 0), (0, 8), (2, 7), (3, 0), (3, 1025), (4, 0), (4, (1 << 30) + 1), (5, 0),
+                    (6, (1 << 30) + 1), (7, None)):
+        args = list(good)
+        args[at] = bad
+        assert entry(*args) == lib.ERR_INVALID, at
