@@ -585,11 +585,12 @@ MVLLM_API int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype,
                                        size_t workspace_bytes);
 /* Few rows times a 4-bit matrix (fmt 4 or 7): y[r] = W x[r] for S rows, y
  * [S, O], in tolerance mode: f32 sums in another order than
- * mvllm_matmul_dev's, f32 rows of x in two f16 parts (22 bits beside the
- * largest value of their scale group).  A pass over the weights serves up to
- * 32 rows (16 in f32); any S runs, but hundreds of rows per matrix are the
- * tensor-core path's work (mvllm_moe_layer_dev).  Every alignment and odd I
- * run; packed rows of 16-byte multiples run fastest. */
+ * mvllm_matmul_dev's; of an f32 value 22 bits, a bf16 value whole, but no finer
+ * than 2^-38 (bf16: 2^-27) of the largest value of its scale group, from 2^-112
+ * on.  A pass over the weights serves up to 32 rows (16 in f32); any S runs, but
+ * hundreds of rows per matrix are the tensor-core path's work
+ * (mvllm_moe_layer_dev).  Every alignment and odd I run; packed rows of 16-byte
+ * multiples run fastest. */
 MVLLM_API int mvllm_matvec_q4_dev(void *stream, int fmt, const void *x, int x_dtype, int64_t ldx,
                                   const void *w, const void *scales, int S, int I, int O, void *y,
                                   int y_dtype, int64_t ldy);

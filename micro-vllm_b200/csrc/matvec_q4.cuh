@@ -405,7 +405,9 @@ __device__ __forceinline__ float exp2_int(int e) {
 // e goes by group, ex[group][row].  Either way the largest scaled value of a
 // group whose largest is at least 2^-112 is at least 4 (below, e stops at
 // 126), and what the parts leave of an element is at most 2^-22 of it (nothing,
-// for bf16) or 2^-25, f16's last step: below 2^-26 of the group's largest.
+// for bf16) or half of f16's last step.  That is 2^-25 for bf16, 2^-27 of the
+// group's largest; f32's second part is held times 2^11, so 2^-36 there, 2^-38
+// of the group's largest.
 //
 // The factors come in where no sum leaves f32's range before its result does:
 // by group, d 2^-e first and then the weights' scale; where a group's largest
@@ -507,8 +509,9 @@ __device__ __forceinline__ bool mv_stage_forward(uint8_t *xs, float *ex, int pit
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             v[k] *= sc;
-            l[k] = fabsf(v[k]) <= 3.402823466e38f ? v[k] - __half2float(__float2half_rn(v[k]))
-                                                   : 0.f;
+            l[k] = fabsf(v[k]) <= 3.402823466e38f
+                       ? (v[k] - __half2float(__float2half_rn(v[k]))) * 0x1p11f
+                       : 0.f;
         }
 #pragma unroll
         for (int term = 0; term < T; ++term) {
@@ -580,6 +583,9 @@ __device__ __forceinline__ void mv_int4x8(uint32_t w, uint32_t (&h)[4]) {
 // of every 32 columns, its own 8: their order along the MMA's K is the same
 // for both operands, so no nibble moves between lanes.  Each scale group's
 // sum starts from zero and is scaled into the f32 accumulator.
+// The sum of an f32 row's two parts, the second 2^11 times what it stands for.
+__device__ __forceinline__ float mv_both(float d0, float d1) { return fmaf(d1, 0x1p-11f, d0); }
+
 enum MvFactor { kMvGroup, kMvCommon, kMvWide }; // where 2^-e comes in (mv_stage_forward)
 template <int FMT, typename TX, int NT, MvFactor FACTOR>
 __device__ __forceinline__ void mv_forward(uint32_t st, int half, const uint32_t (&xs)[NT],
@@ -661,7 +667,8 @@ __device__ __forceinline__ void mv_forward(uint32_t st, int half, const uint32_t
                     const float e0 = fminf(e, 0x1p64f), e1 = fmaxf(e * 0x1p-64f, 1.f);
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt) {
-                        const float v = T == 1 ? d[mt][nt][q] : d[mt][nt][q] + d[mt][nt][q + 1];
+                        const float v = T == 1 ? d[mt][nt][q]
+                                               : mv_both(d[mt][nt][q], d[mt][nt][q + 1]);
                         acc[mt][nt][q] = fmaf(v * e0 * sc[mt][q >> 1][gr], e1, acc[mt][nt][q]);
                     }
                 }
@@ -678,9 +685,9 @@ __device__ __forceinline__ void mv_forward(uint32_t st, int half, const uint32_t
                 const float e = ex[gr * RP + nt * 4 + t];
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
-                    acc[mt][nt][0] = fmaf((d[mt][nt][0] + d[mt][nt][1]) * e, sc[mt][0][gr],
+                    acc[mt][nt][0] = fmaf(mv_both(d[mt][nt][0], d[mt][nt][1]) * e, sc[mt][0][gr],
                                           acc[mt][nt][0]);
-                    acc[mt][nt][2] = fmaf((d[mt][nt][2] + d[mt][nt][3]) * e, sc[mt][1][gr],
+                    acc[mt][nt][2] = fmaf(mv_both(d[mt][nt][2], d[mt][nt][3]) * e, sc[mt][1][gr],
                                           acc[mt][nt][2]);
                 }
             }
@@ -925,7 +932,8 @@ __device__ __forceinline__ void mv_put(float *to, const float (&acc)[2][NT][4], 
                 at[RPITCH + 8] = add ? at[RPITCH + 8] + d[3] : d[3];
             } else {
                 if (ex) {
-                    const float e = ex[nt * 4 + t], s0 = d[0] + d[1], s1 = d[2] + d[3];
+                    const float e = ex[nt * 4 + t], s0 = mv_both(d[0], d[1]),
+                                s1 = mv_both(d[2], d[3]);
                     check = fmaf(s0 + s1, 0.f, check);
                     d[0] = s0 * e, d[2] = s1 * e;
                 }

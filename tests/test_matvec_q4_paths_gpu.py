@@ -308,3 +308,24 @@ def test_many_experts_rows(moe, dtype, S, fmt):
             W = rc.decode(w[e * O:(e + 1) * O], s[e * O:(e + 1) * O], fmt, I)
             if int(nr[e]):
                 exact_as_f32(y[part], x[part], W.T if m == O else W, f"expert {e}")
+
+
+@pytest.mark.parametrize("dtype,below", [(F32, 24), (BF16, 18)])
+@pytest.mark.parametrize("fmt", [INT4, MXFP4])
+@pytest.mark.parametrize("S,I,O", [(1, 32, 40), (5, 1000, 96), (4, 7168, 16384), (40, 512, 96)])
+def test_small_values_beside_an_outlier(moe, S, I, O, fmt, dtype, below):
+    """In every scale group one value that its weights, all 0, leave out, and the
+    others far below it: these keep their bits."""
+    gen = torch.Generator().manual_seed(I)
+    w, s = rc.packed(gen, fmt, O, I, "cuda", spread=0)
+    x = torch.randn(S, I, generator=gen) * 2.0 ** -below
+    x[:, ::32] = 1.0
+    at = torch.arange(0, (I + 1) // 2, 16, device="cuda")  # the bytes of columns 0, 32, ..
+    w[:, at] = (w[:, at] & 0xF0) | (8 if fmt == INT4 else 0)
+    x = x.cuda().to(dtype)
+    y = torch.empty(S, O, device="cuda")
+    moe.matvec_q4_dev(fmt, x, w, s, y)
+    close(y, x, rc.decode(w, s, fmt, I).T, "forward")
+    exact = x.double() @ rc.decode(w, s, fmt, I).T
+    # 22 bits of each value: random, and below 2^-20 of a sum's norm
+    assert (y.double() - exact).norm() <= 2.0 ** -20 * exact.norm()
