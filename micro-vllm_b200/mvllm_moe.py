@@ -688,6 +688,7 @@ def _dtype_name(dtype):
 
 
 _dtype_names = {}
+_MOST = 0x7fffffff  # the C entries take sizes as int
 _ROW_DTYPES = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16}
 
 
@@ -728,25 +729,22 @@ def _grid(t, name, dtype, shape):
     return _flat(t, name, dtype, 0)
 
 
-def _sizes(t, name):
-    """The two sizes of a matrix; the C entries take them as int."""
-    rows, cols = t.shape
-    if rows > 0x7fffffff or cols > 0x7fffffff:
-        raise ValueError(f"{name}: shape {(rows, cols)}, below 2^31 is needed")
-    return rows, cols
-
-
 def _slots(tok_pos):
     if tok_pos is None or tok_pos.dim() != 2:
         raise ValueError("tok_pos: a 2-D tensor [T, K + n_shared] is needed")
-    T, KK = _sizes(tok_pos, "tok_pos")
+    T, KK = tok_pos.shape
+    if T > _MOST or KK > _MOST:
+        raise ValueError(f"tok_pos: shape {(T, KK)}, below 2^31 is needed")
     return T, KK, _flat(tok_pos, "tok_pos", "torch.int32", T * KK)
 
 
 def _matrix(t, name):
     if t is None or t.dim() != 2:
         raise ValueError(f"{name}: a 2-D tensor is needed")
-    return _sizes(t, name)
+    rows, cols = t.shape
+    if rows > _MOST or cols > _MOST:
+        raise ValueError(f"{name}: shape {(rows, cols)}, below 2^31 is needed")
+    return rows, cols
 
 
 _raw_stream = None  # device index -> handle of torch's current stream
@@ -890,7 +888,7 @@ def matvec_q4_grad_dev(fmt, dy, w, scales, dx, stream=None):
 def _expert_matvec(entry, fmt, x, w, scales, nr, xoff, y, I, O, stream):
     if fmt not in (FMT_INT4_G64, FMT_MXFP4):
         raise ValueError(f"fmt {fmt}: FMT_INT4_G64 or FMT_MXFP4 is needed")
-    if nr is None or nr.numel() > 0x7fffffff:
+    if nr is None or nr.numel() > _MOST:
         raise ValueError("nr: the rows of each expert are needed")
     nb, cap = nr.numel(), x.shape[0]
     px, tx, ldx = _rows(x, "the input rows", cap, x.shape[1])
