@@ -101,11 +101,13 @@ template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
     // stages that a CTA's warps take one after another, at the rate of its
     // share of the memory or of what its warps dequantise, and the unit's own
     // cost, with the partial sums it adds up; and the rows that are staged.
-    // The constants (ns, bytes and elements per ns of a CTA) were fitted to 272
-    // measured shapes of both formats and directions, 1 to 1024 rows: its answer
-    // is 3% slower than the best of about 60 cuts of each on average.  (Rows
+    // The constants (ns, bytes and elements per ns of a CTA) are a fit by hand to
+    // times of 272 shapes of both formats and directions, 1 to 1024 rows, about 60
+    // cuts of each: the answer was 3% slower than the best on average.  (Rows
     // staged at 20 elements per ns and 1500 ns a unit, first guesses, left 11%
-    // and up to twice the time.)
+    // and up to twice the time.)  int4's gradient, three matrix instructions a
+    // product, has its own rate and unit cost from 7 shapes, 1 to 768 rows, where
+    // the answer is 0 to 16% slower than the best.
     static int plan(MvCut &cut, int nb, const DeviceScope &dev) {
         MatvecPlan &p = cut.p;
         const double items = expected_passes(p.rows_most, nb, RP);
@@ -239,8 +241,8 @@ template <int FMT, typename TX, int NT, bool GRAD> struct MvHost {
 // 16 or 32 operand columns (gradient: 8 or 16; int4's: 8, its parts' sums need
 // the registers) hold them, as many as that for more.  Experts, whose rows
 // differ, take the width whose plan has the lowest estimate: 48 experts of 16
-// rows on average, 7168 -> 2048, take 183 us by 16 rows a pass and 253 by 32,
-// 160 experts of 20, 6144 -> 1536, 614 and 462.
+// rows on average, 7168 -> 2048, take 208 us by 16 rows a pass and 252 by 32,
+// 160 experts of 20, 6144 -> 1536, 499 and 600.
 template <int FMT, typename TX, bool GRAD>
 int matvec_rows(cudaStream_t st, const MatvecArgs &a, const MatvecPlan &p, const DeviceScope &dev,
                 const void *x, int64_t ldx, void *y, int64_t ldy, int *told) {

@@ -10,12 +10,13 @@
 // The weights are read once per pass of up to 32 rows, 4.5 bits each, so the
 // floor is their bytes; each decodes to an operand of m16n8k16 matrix
 // instructions, which take the rows as the narrow side.  One row of 7168 ->
-// 65536 streams at 4.7 TB/s, 72% of a copy; 7168 -> 16384 (60 MB) takes 17 us
-// for 1 row, 20 for 8, 31 for 16 and 63 for 32.  Beyond the memory it is the
-// decoding that bounds: 520 instructions per stage of a warp for 8 rows, 970
-// to 1290 for 32, issued on 58% and 35% of the cycles; the matrix pipe is busy
-// for 25 to 36%.  Short products are bound by their start: 6 to 7 us for 8 MB,
-// of which the rows' way to the operands is about half.
+// 65536 streams at 4.8 TB/s, 73% of a copy; 7168 -> 16384 (60 MB) takes 17 to
+// 18 us for 1 row, 20 for 8, 32 for 16 and 64 for 32.  Beyond the memory it is
+// the decoding that bounds: 490 to 550 instructions per stage of a warp for 8
+// rows, 1260 for 32 (1100 in the gradient, 8 rows), issued on 54 to 57% and 38%
+// (43 to 52%) of the cycles; the matrix pipe is busy for 26 to 31%.  Short
+// products are bound by their start: 6.9 us for 8 MB, of which the rows' way to
+// the operands is about half.
 #pragma once
 
 #include "row_kernels.cuh"
@@ -53,11 +54,11 @@ __device__ __forceinline__ bool matvec_expert(const MatvecArgs &a, int e, const 
 // Warps of a CTA (one CTA per SM) and stages of a warp's ring.  The forward
 // product is bound by the instructions of the dequantisation and wants as many
 // warps to interleave as registers and the staged rows leave room for: with 16
-// warps 16 rows take 7168 -> 16384 in 39 us in place of 35 (registers spill),
-// with 12 warps 32 rows in 91 in place of 70 (the staged rows come in more
-// chunks).  The gradient holds 64 or 128 sums per lane; cut to 128 columns a
-// task it fits 12 or 16 warps, which took 450 and 490 us in place of 385 on 160
-// experts of 1536 x 6144.
+// warps 16 rows take 7168 -> 16384 in 38 us in place of 32 (registers spill),
+// with 12 warps 32 rows in 84 in place of 64 (the staged rows come in more
+// chunks).  The gradient holds 64 or 128 sums per lane; 12 warps with rings of
+// three stages spill, 513 us in place of 397 on 160 experts of 1536 x 6144 (int4;
+// MXFP4 342 in place of 326).
 template <int NT, bool GRAD> constexpr int mv_warps() {
     return GRAD || NT == 4 ? 8 : NT == 2 ? 12 : 16;
 }
@@ -561,7 +562,8 @@ __device__ __forceinline__ void mv_stage_gradient(uint8_t *xs, int pitch, const 
     });
 }
 
-// int4x8_to_f16x8 with one shift for eight codes: a nibble in bits 4..7 of a
+// int4x8_to_f16x8 with one shift for eight codes, by the published reading of a
+// nibble through f16's exponent (1024 + n in its low mantissa bits): a nibble in bits 4..7 of a
 // halfword reads as 1024 + 16 n, which one multiply-add turns into n - 8.
 __device__ __forceinline__ void mv_int4x8(uint32_t w, uint32_t (&h)[4]) {
     const uint32_t u = w >> 8, m0 = 0x000f000fu, m1 = 0x00f000f0u, one = 0x64006400u;
@@ -1143,7 +1145,7 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
     };
     MvUnit cur{};
     // A cluster's units follow one another, so that an item's rows are staged
-    // once for its ranges (48 experts of 5 rows, 7168 -> 2048: 111 us, 130 with
+    // once for its ranges (48 experts of 5 rows, 7168 -> 2048: 111 us; 130 with
     // the clusters taking units in turn).
     const int each = total / clusters, more = total - each * clusters;
     const int u0 = each * cluster + min(cluster, more), u1 = u0 + each + (cluster < more);
@@ -1303,7 +1305,7 @@ __global__ void __launch_bounds__(32 * mv_warps<NT, GRAD>(), 1)
         // An item is (row, block of 32 outputs), eight lanes of four outputs each;
         // warps take four at a time.  It is owned by rank item % ranks, there in
         // slot item / ranks * ranks + sender.  (Distributed shared memory takes
-        // 16 bytes a lane better than 4: 16 rows of 7168 -> 16384 in 31 us, 35
+        // 16 bytes a lane better than 4: 16 rows of 7168 -> 16384 in 31 us then, 35
         // with four times the stores.)
         const int outs = min(pl.range, pl.N - cur.out0), blocks = (outs + 31) / 32;
         const int all = blocks * cur.n, sub = lane >> 3, o4 = (lane & 7) * 4;

@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(kRgThreads)
 // kRgCols columns, an expert, `block` of its rows); each warp takes the next
 // one, and has four rows' loads under way: 32 warps per SM so hide more of the
 // gathers' latency than 16 with eight rows each (97 against 103 us on 65536
-// slots of 384 experts, H 7168, bf16).  Items run by groups of eight column
+// slots spread evenly over 384 experts, H 7168, bf16; 112 where they are uneven).
+// Items run
 // blocks, so the columns of x that all experts gather from (16 T kRgCols bytes
 // in bf16) stay in L2.  An expert of several items leaves its partial sums in
 // the workspace, and the warp that arrives last adds them in order; one without

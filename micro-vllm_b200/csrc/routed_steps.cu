@@ -320,7 +320,7 @@ int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t l
         a.counters = E * ncol + 1;
         // Long row blocks leave fewer partial sums, short ones more items to
         // share: 64 rows, doubled up to 256 while 24 items per SM remain.
-        // (65536 slots of 384 experts, H 7168, by 256 rows: 97 us; 32768 of 64,
+        // (65536 slots evenly over 384 experts, H 7168, by 256 rows: 97 us; 32768 of 64,
         // H 2048: 28 by 64 or 128, 36 by 256; 512 rows cost uneven experts 12 us
         // more.)
         a.block = kRgRows;
