@@ -157,9 +157,8 @@ __global__ void __launch_bounds__(kRgThreads)
 // one, and has four rows' loads under way: 32 warps per SM so hide more of the
 // gathers' latency than 16 with eight rows each (97 against 103 us on 65536
 // slots spread evenly over 384 experts, H 7168, bf16; 112 where they are uneven).
-// Items run
-// blocks, so the columns of x that all experts gather from (16 T kRgCols bytes
-// in bf16) stay in L2.  An expert of several items leaves its partial sums in
+// Items run by groups of eight column blocks, so the columns of x that all
+// experts gather from (16 T kRgCols bytes in bf16) stay in L2.  An expert of several items leaves its partial sums in
 // the workspace, and the warp that arrives last adds them in order; one without
 // rows gets zeros.  Bound by the latency of the gathers, a third of whose
 // sectors miss the near L2; issue slots stand at 52%.  (Rows through a ring of
