@@ -569,11 +569,12 @@ MVLLM_API int mvllm_moe_combine_grad_dev(void *stream, const void *dout, int dou
  * token rows, dx[t] = sum_k dz_k router[idx[t, k]], and to the router,
  * drouter[e] = sum over the tokens routed to e of dz x[t], where dz is the
  * gradient of the logit through score_fn, the clamp at 0, the division by the
- * weights' sum and routed_scale.  scores [T, E], idx: its outputs (ids outside
- * [0, E) carry nothing); the choice of ids and the bias have no gradient.
- * nr, xoff, rows, tok_pos: the permutation of that idx and its weights.  dx
- * (dx_dtype) or drouter (f32 [E, H], contiguous) may be NULL; both are added
- * to when accumulate.  E <= 1024, K <= 32. */
+ * weights' sum (none where that is 0 or NaN and the weights are equal) and
+ * routed_scale.  scores [T, E], idx: its outputs (ids outside [0, E) carry
+ * nothing); the choice of ids and the bias have no gradient.  nr, xoff, rows,
+ * tok_pos: the permutation of that idx and its weights.  dx (dx_dtype) or
+ * drouter (f32 [E, H], contiguous) may be NULL; both are added to when
+ * accumulate.  E <= 1024, K <= 32. */
 MVLLM_API size_t mvllm_moe_route_grad_workspace(int T, int H, int E, int K);
 MVLLM_API int mvllm_moe_route_grad_dev(void *stream, const void *x, int x_dtype, int64_t ldx,
                                        int T, int H, const float *router, int E, int K,

@@ -4,7 +4,8 @@
 // choice s + bias, m_k = max(s[idx_k], 0), M = sum_k m_k and
 // wt_k = c m_k / M (c = routed_scale).  The bias only selects.  Backward,
 // with g_k = c dwt_k:
-//   dm_k = (g_k - sum_j g_j m_j / M) / M          (0 where m_k or M is 0)
+//   dm_k = (g_k - sum_j g_j m_j / M) / M          (0 where m_k is 0, or where
+//                         M is 0 or NaN: the forward pass has wt_k = c / K there)
 //   dz_k = dm_k s'(z_k),  s' = s (1 - s)                     sigmoid
 //                         s' = (1 - e^(-s^2)) / (2 s)        sqrt(softplus),
 // the second from softplus' = sigmoid(z) = 1 - e^(-softplus) and s^2 =
@@ -52,13 +53,14 @@ __device__ __forceinline__ float route_slot_grad(const RouteGradArgs &a, int64_t
         e = -1;
     float m = 0.f, g = 0.f;
     if (e >= 0) {
-        m = fmaxf(a.scores[t * a.E + e], 0.f);
+        m = a.scores[t * a.E + e];
+        m = m < 0.f ? 0.f : m; // NaN stays, as in the forward pass
         g = a.scale * a.dwt[t * a.K + lane];
     }
     float M = 0.f, G = 0.f; // sums in slot order, the same on every lane
     for (int k = 0; k < a.K; ++k)
         M += __shfl_sync(0xffffffffu, m, k);
-    const bool live = e >= 0 && m > 0.f;
+    const bool live = e >= 0 && m > 0.f && M > 0.f;
     const float w = live ? m / M : 0.f;
     for (int k = 0; k < a.K; ++k)
         G = fmaf(__shfl_sync(0xffffffffu, g, k), __shfl_sync(0xffffffffu, w, k), G);

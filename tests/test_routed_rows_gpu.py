@@ -108,3 +108,35 @@ def test_few_tokens_of_wide_rows(moe, T, K):
             dots, size = (seen * y[:R].double()).sum(1), (seen * y[:R].double()).abs().sum(1)
             t, k, at = rc.slots(plan)
             assert ((dwt[t, k].double() - dots[at]).abs() <= (D / 32 + 48) * U * size[at]).all()
+
+
+@pytest.mark.parametrize("score_fn", [0, 1])
+def test_tokens_whose_weights_are_constant(moe, score_fn):
+    """Where the chosen scores' sum is 0 or NaN the forward pass gives every
+    choice the same weight: such a token has no gradient, the others theirs."""
+    T, K, E, H = 24, 3, 8, 64
+    c = routed(moe, T, K, E, H)
+    args = [c[k] for k in ("x", "router", "idx", "scores", "dwt")]
+    idx, scores = c["idx"].long(), c["scores"]
+    chosen = [t for t in range(T) if int(idx[t, 0]) >= 0]
+    a, b = chosen[2], chosen[7]
+    scores[a, idx[a]] = 0.0
+    scores[b, idx[b, 1]] = float("nan")
+    two = torch.tensor([a, b], device="cuda")
+    choice = torch.zeros(2, E, device="cuda").scatter_(1, idx[two], 1.0)
+    ids, wt = torch.empty(2, K, dtype=torch.int32, device="cuda"), torch.empty(2, K, device="cuda")
+    moe.topk_dev(choice, K, ids, wt, mix=scores[two].contiguous())
+    assert torch.equal(wt, torch.full_like(wt, 1 / K)), "the forward pass"
+    p = c["plan"]
+    dx, dr = torch.full((T, H), 7.0, device="cuda"), torch.empty(E, H, device="cuda")
+    moe.route_grad_dev(*args, p["nr"], p["xoff"], p["rows"], p["tok_pos"], dx, dr,
+                       score_fn=score_fn)
+    assert (dx[a] == 0).all() and (dx[b] == 0).all()
+    clean = scores.clone()
+    clean[a] = clean[b] = 0.5
+    dwt = c["dwt"].clone()
+    dwt[a] = dwt[b] = 0
+    want_x, want_r, _ = rc.route_grad(c["x"], c["router"], c["idx"], clean, dwt, score_fn, 1.0)
+    n = (2 * K + 16) * U
+    assert (dx.double() - want_x).norm() <= n * want_x.norm()
+    assert (dr.double() - want_r).norm() <= n * want_r.norm()
